@@ -142,6 +142,42 @@ int yapd_attn_paged_block_noalloc(const void* q, const void* kv_pool, int64_t n_
                                   const int32_t* counts, int n_slots, float scale, int causal, void* out,
                                   void* stream);
 
+/* Attention with a sliding window and sink tokens over the paged KV cache.
+ * Query i of row r stands at position p = kv_len[r] - n(r) + i (n(r) = the
+ * row's query count) and sees key j iff j < hi and (j < sinks or j > p -
+ * window), hi = p + 1 (causal != 0) or kv_len[r] (causal = 0: a block step's
+ * later positions too).  out = softmax(q K^T * scale) V over the keys seen; a
+ * query that sees none gets zeros.  It has no counterpart in the reference.
+ *   q: bf16, token t's head h at t * q_tok_stride + h * 64; out: bf16 [n_q, H,
+ *   64], which must not overlap q or the pool.  q_start NULL: row r's queries
+ *   are tokens r * max_q .. (n_q = rows * max_q).  q_start (device int32
+ *   [rows + 1], not decreasing): row r's are tokens [q_start[r],
+ *   q_start[r+1]), at most max_q of them (further ones are left out); a row may
+ *   have none; output rows of no row's are not written.
+ *   kv_len (device int32 [rows]) counts the row's keys, its queries' own
+ *   included; it is clamped to 16 * table_cols.  Pages wholly outside the keys
+ *   seen are never read into a result: their table entries may be anything.
+ *   K and V have to be finite where any query of the call's row sees them.
+ *   max_kv: the host's upper bound of kv_len (16 * table_cols where unknown);
+ *   it only decides how the work is cut, not what is computed.
+ * The work is cut by sizes the host knows and the device lengths alone, so
+ * a captured launch follows kv_len and q_start from replay to replay.  How
+ * it is cut (and with it the order of a query's sums) depends on the call's
+ * sizes.  With few queries over many keys the keys are cut into parts joined
+ * by a second launch: workspace then holds yapd_attn_window_workspace() floats
+ * (0: not needed, may be NULL), 16-byte aligned, not shared by calls that may
+ * overlap.  window >= 1, sinks >= 0, H a multiple of 4, scale > 0. */
+int yapd_attn_window(const void* q, int64_t q_tok_stride, const void* kv_pool, int64_t n_pages,
+                     const int32_t* page_table, int table_stride, int table_cols, const int32_t* kv_len,
+                     const int32_t* q_start, int rows, int max_q, int n_q, int n_heads, int window, int sinks,
+                     int causal, int max_kv, float scale, float* workspace, int64_t workspace_floats, void* out,
+                     void* stream);
+
+/* Floats of workspace that yapd_attn_window needs for a call of these sizes
+ * (packed: whether it is given q_start); 0 if none, -1 on a bad argument. */
+int64_t yapd_attn_window_workspace(int rows, int max_q, int n_q, int packed, int n_heads, int window, int sinks,
+                                   int max_kv);
+
 /* ------------------------------------------------------------------------ *
  * (b) bf16 MFMA projections (nn.Linear layout: C = A W^T, fp32 accumulate).
  * K must be a multiple of 64; A, W 16-byte aligned with leading dims

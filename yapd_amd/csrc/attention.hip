@@ -30,6 +30,7 @@
 #include <vector>
 
 #include "attention.h"
+#include "attn_tile.h"
 #include "common.h"
 #include "kv_layout.h"
 #include "lds_dma.h"
@@ -67,41 +68,6 @@ __device__ __forceinline__ int2 row_queries(const int32_t* q_start, int n_q, int
   if (q_start == nullptr) return make_int2(r * bl, bl);
   const int qs = min(max(q_start[r], 0), n_q);
   return make_int2(qs, min(max(q_start[r + 1] - qs, 0), min(bl, n_q - qs)));
-}
-
-__device__ __forceinline__ u32x4_t load16(const uint16_t* p) {
-  return *reinterpret_cast<const u32x4_t*>(p);
-}
-
-// K/V pages are streamed once per step: non-temporal loads keep them from
-// evicting the q / K / V lines the QKV GEMM has just written, whose
-// write-back would otherwise land in the middle of this stream (measured
-// 195 -> 179 us per layer right after the QKV GEMM).
-__device__ __forceinline__ u32x4_t load16_stream(const uint16_t* p) {
-  return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
-}
-
-// Lane l combined with lane l ^ 16 (l ^ 32): v_permlane16_swap (32_swap) of a
-// value with itself returns the two halves of every exchanged pair, so the
-// max or sum of its two results is the pair's in both lanes -- a VALU
-// exchange instead of an LDS permute.
-__device__ __forceinline__ float2 swap16(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float2 swap32(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float max_xor16_32(float v) {
-  const float2 a = swap16(v);
-  const float2 b = swap32(fmaxf(a.x, a.y));
-  return fmaxf(b.x, b.y);
-}
-__device__ __forceinline__ float sum_xor16_32(float v) {
-  const float2 a = swap16(v);
-  const float2 b = swap32(a.x + a.y);
-  return b.x + b.y;
 }
 
 // One 32-key chunk of a 16-query tile: S^T = K Q^T, the online-softmax step, O^T += V^T P^T.  A lane

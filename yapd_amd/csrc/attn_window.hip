@@ -1,0 +1,495 @@
+// Paged-KV attention with a sliding window and sink tokens.
+//
+// Query i of row r stands at position p = kv_len[r] - n_q(r) + i and sees key
+// j iff  j < hi  and  (j < sinks  or  j > p - window),  hi = p + 1 (causal) or
+// kv_len[r] (block: the later positions of its own block too):
+//   out = sum_j softmax_j(scale q . k_j) v_j   over the visible j.
+// What a step reads is bounded by window + sinks keys a row, so it needs no
+// host plan: every workgroup derives its key range from the device lengths,
+// and a captured launch follows them as they grow.
+//
+// A row's queries are cut into tiles of 16 NQT; a tile's visible keys are a
+// list of 32-key chunks: the sinks' chunks, then those from the first query's
+// window on.  The list is cut into `parts` (workgroups) and each part into KS
+// runs (waves); runs join in LDS, parts through a workspace and a second
+// launch.  Chunk arithmetic is that of the paged block attention: S^T = K Q^T
+// and O^T += V^T P^T on v_mfma_f32_16x16x32_bf16, every lane owning one query.
+#include <algorithm>
+#include <cmath>
+
+#include "attn_tile.h"
+#include "common.h"
+#include "kv_layout.h"
+
+namespace yapd {
+namespace {
+
+constexpr int kChunk = 32;        // keys per inner step (two pages)
+constexpr int kCap = 1 << 30;     // window and sinks are held to this: p - window stays inside int32
+
+struct WindowParams {
+  const uint16_t* q;    // token t, head h at t * q_stride + h * 64
+  int64_t q_stride;
+  const uint16_t* pool;
+  int64_t n_pages;
+  const int32_t* table;
+  int table_stride, table_cols;
+  const int32_t* kv_len;
+  const int32_t* q_start;  // [rows + 1], or NULL: row r's queries are r * max_q ..
+  int rows, max_q, n_q, H;
+  int window, sinks, causal;
+  int parts;
+  float* part_o;   // [parts, n_q, H, 64]
+  float* part_ml;  // [parts, n_q, H, 2]
+  float scale_log2;
+  uint16_t* out;  // [n_q, H, 64]
+};
+
+// A tile of one row's queries: rows qs .. qs + qc - 1 of q / out at positions p0, p0 + 1, ...
+struct Tile {
+  int row, qs, qc, p0, kvl;
+};
+
+__device__ __forceinline__ int first_query(const WindowParams& P, int r) {
+  return min(max(P.q_start[r], 0), P.n_q);
+}
+
+// Tile `slot` of the launch.  Uniform rows have ceil(max_q / TQ) slots each;
+// of packed rows, row r's tiles start at slot f(r) = q_start[r] / TQ + r: its
+// ceil(n / TQ) tiles end at or before f(r + 1), and f grows with r, so the row
+// is found by a 64-way search.  false: the slot holds no query.
+template <int TQ>
+__device__ __forceinline__ bool find_tile(const WindowParams& P, int slot, int lane, Tile& t) {
+  int first;
+  if (P.q_start == nullptr) {
+    const int per = (P.max_q + TQ - 1) / TQ;
+    t.row = slot / per;
+    t.qs = t.row * P.max_q;
+    t.qc = P.max_q;
+    first = (slot - t.row * per) * TQ;
+  } else {
+    int base = 0, n = P.rows;
+    while (n > 1) {
+      const int step = (n + 63) / 64;
+      const int i = lane * step;
+      const bool le = i < n && first_query(P, base + min(i, n - 1)) / TQ + base + i <= slot;
+      const int at = (max(__popcll(__ballot(le)), 1) - 1) * step;
+      base += at;
+      n = min(step, n - at);
+    }
+    t.row = base;
+    t.qs = first_query(P, base);
+    t.qc = min(max(first_query(P, base + 1) - t.qs, 0), P.max_q);
+    first = (slot - t.qs / TQ - base) * TQ;
+  }
+  if (first < 0 || first >= t.qc) return false;
+  t.kvl = min(max(P.kv_len[t.row], 0), P.table_cols * kPageSize);
+  t.p0 = t.kvl - t.qc + first;
+  t.qs += first;
+  t.qc = min(TQ, t.qc - first);
+  return true;
+}
+
+// The chunks (of C keys) that some query of a tile sees: list entry c is chunk
+// c below n_sink, chunk skip + c from there on.
+struct ChunkList {
+  int lo, hi;  // keys seen: [0, sinks) and [lo, hi), both below hi
+  int n_sink, skip, n;
+  __device__ __forceinline__ ChunkList(const WindowParams& P, const Tile& t, int C) {
+    const int last = t.p0 + t.qc - 1;
+    lo = max(t.p0 - P.window + 1, 0);
+    hi = max(P.causal ? min(t.kvl, last + 1) : t.kvl, 0);
+    const int cb = min(lo, hi) / C, ce = (hi + C - 1) / C;
+    n_sink = min((min(P.sinks, hi) + C - 1) / C, cb);
+    skip = cb - n_sink;
+    n = n_sink + ce - cb;
+  }
+  __device__ __forceinline__ int chunk(int c) const { return c < n_sink ? c : c + skip; }
+};
+
+// The row's page ids, 64 at a time: lane i holds the page of table column
+// base + i (clamped), and a chunk picks its pages with readlane.
+struct Pages {
+  const int32_t* tab;
+  int last_page, max_page, lane, base, v;
+  __device__ __forceinline__ Pages(const WindowParams& P, const Tile& t, int first, int lane_)
+      : tab(P.table + static_cast<int64_t>(t.row) * P.table_stride),
+        last_page(max((t.kvl + kPageSize - 1) / kPageSize - 1, 0)),
+        max_page(static_cast<int>(min(P.n_pages - 1, int64_t{0x7fffffff}))), lane(lane_) {
+    load(min(first, last_page));
+  }
+  __device__ __forceinline__ void load(int b) {
+    base = b;
+    v = tab[min(base + lane, last_page)];
+    asm volatile("" ::"v"(v));  // complete here: later uses wait on no load
+  }
+  __device__ __forceinline__ int operator()(int pi) {
+    pi = min(pi, last_page);
+    if (pi - base >= 64) load(pi);  // uniform: pi is the same for the wave, and never falls
+    return min(max(__builtin_amdgcn_readlane(v, pi - base), 0), max_page);  // a bad table entry cannot fault
+  }
+};
+
+constexpr int kWaveFloats = 4 * 64 * 4;  // a wave's O^T tile in LDS: fragment mt of lane l at (mt * 64 + l) * 4
+
+template <int NQT, int KS, int HPW>
+__global__ __launch_bounds__(64 * KS * HPW) void attn_window_kernel(const WindowParams P) {
+  constexpr int TQ = 16 * NQT;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int ks = wave % KS, hsub = wave / KS;
+  const int groups = P.H / HPW;
+  const int item = static_cast<int>(blockIdx.x) / groups;
+  const int h = (static_cast<int>(blockIdx.x) - item * groups) * HPW + hsub;
+  const int slot = item / P.parts, part = item - slot * P.parts;
+  Tile t;
+  if (!find_tile<TQ>(P, slot, lane, t)) return;  // the whole workgroup
+  const int g = lane >> 4, n = lane & 15;
+  const int H = P.H;
+  const ChunkList cl(P, t, kChunk);
+
+  // Q^T fragments (B operand): lane holds Q[q = qt*16 + n][hd = s*32 + 8g .. +7]
+  bf16x8_t qf[NQT][2];
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      u32x4_t v = {0u, 0u, 0u, 0u};
+      if (qt * 16 + n < t.qc) v = load16(P.q + (t.qs + qt * 16 + n) * P.q_stride + h * kHeadDim + s * 32 + 8 * g);
+      qf[qt][s] = as_bf16x8(v);
+    }
+  }
+  f32x4_t o[NQT][4];
+  float m[NQT], l[NQT];
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) {
+    m[qt] = -INFINITY;
+    l[qt] = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) o[qt][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // this wave's run of the list
+  const int64_t runs = static_cast<int64_t>(P.parts) * KS, run = static_cast<int64_t>(part) * KS + ks;
+  const int c0 = static_cast<int>(cl.n * run / runs), c1 = static_cast<int>(cl.n * (run + 1) / runs);
+  if (c0 < c1) {
+    Pages page_of(P, t, cl.chunk(c0) * (kChunk / kPageSize), lane);
+    // Key served by row n of S^T tile i: 8*(n/4) + 4i + n%4, so that lane group g
+    // ends up holding keys 8g .. 8g+7 of the chunk.
+    const int key_t0 = 8 * (n >> 2) + (n & 3);
+    auto load_chunk = [&](int k0, u32x4_t (&kf)[2][2], u32x4_t (&vf)[4]) {
+      const int pi0 = k0 / kPageSize;
+      const int64_t pg0 = page_of(pi0), pg1 = page_of(pi0 + 1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = key_t0 + 4 * i;
+        const int64_t pg = key < kPageSize ? pg0 : pg1;
+        const uint16_t* kp = P.pool + k_offset(pg, h, H, key & (kPageSize - 1), 8 * g);
+        kf[i][0] = load16_stream(kp);
+        kf[i][1] = load16_stream(kp + 32);
+      }
+      const int64_t pg = g < 2 ? pg0 : pg1;
+      const uint16_t* vp = P.pool + v_offset(pg, h, H, 8 * (g & 1), n);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) vf[mt] = load16_stream(vp + 16 * mt * kPageSize);
+    };
+    const int last = t.p0 + t.qc - 1;
+    const int all_lo = last - P.window + 1;                 // keys from here on are in every query's window
+    const int all_hi = P.causal ? min(t.kvl, t.p0 + 1) : t.kvl;  // keys below are before every query's end
+
+    u32x4_t kf[2][2], vf[4], kn[2][2], vn[4];
+    load_chunk(cl.chunk(c0) * kChunk, kf, vf);
+    for (int c = c0; c < c1; ++c) {
+      const int k0 = cl.chunk(c) * kChunk;
+      if (c + 1 < c1) load_chunk(cl.chunk(c + 1) * kChunk, kn, vn);
+      const bool mask = k0 + kChunk > all_hi || (k0 < all_lo && k0 + kChunk > P.sinks);
+      if (mask) {
+        // V of keys that no query of the tile sees (behind the window, past the
+        // end, stale slots of the last page): cleared, so 0 * V is never NaN
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int key = k0 + 8 * g + 2 * w;
+          const bool see0 = key < cl.hi && (key >= cl.lo || key < P.sinks);
+          const bool see1 = key + 1 < cl.hi && (key + 1 >= cl.lo || key + 1 < P.sinks);
+          const uint32_t keep = (see0 ? 0x0000ffffu : 0u) | (see1 ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) vf[mt][w] &= keep;
+        }
+      }
+#pragma unroll
+      for (int qt = 0; qt < NQT; ++qt) {
+        f32x4_t s[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kf[i][0]), qf[qt][0],
+                                                         f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+          s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kf[i][1]), qf[qt][1], s[i], 0, 0, 0);
+        }
+        // s[i][j] = S[q = n][key 8g + 4i + j]
+        float sv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sv[i] = s[i >> 2][i & 3] * P.scale_log2;
+        if (mask) {  // uniform
+          const int p = t.p0 + qt * 16 + n;
+          const int q_hi = P.causal ? min(t.kvl, p + 1) : t.kvl, q_lo = p - P.window + 1;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int key = k0 + 8 * g + i;
+            sv[i] = key < q_hi && (key >= q_lo || key < P.sinks) ? sv[i] : -INFINITY;
+          }
+        }
+        float cm = sv[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) cm = fmaxf(cm, sv[i]);
+        cm = max_xor16_32(cm);
+        const float mn = fmaxf(m[qt], cm);
+        // no key seen yet: exponents against 0 give alpha = 0 and p = 0 instead of NaN
+        const float mref = mn == -INFINITY ? 0.f : mn;
+        const float alpha = __builtin_amdgcn_exp2f(m[qt] - mref);
+        float p[8], ps = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(sv[i] - mref);
+          ps += p[i];
+        }
+        l[qt] = l[qt] * alpha + ps;
+        m[qt] = mn;
+        // P in bf16: the operand type of the product with V (a rounding of 2^-9 of each weight, averaged over keys)
+        u32x4_t pw;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) pw[w] = pack_bf16x2(p[2 * w], p[2 * w + 1]);
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          o[qt][mt] *= alpha;
+          o[qt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(vf[mt]), as_bf16x8(pw), o[qt][mt], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        kf[i][0] = kn[i][0];
+        kf[i][1] = kn[i][1];
+      }
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) vf[mt] = vn[mt];
+    }
+  }
+
+  // o[qt][mt][j] = O^T[hd = 16mt + 4g + j][q = qt*16 + n].  With KS runs: their
+  // O^T, m and l go to LDS, and wave ks joins the fragments mt = ks, ks + KS, ..
+  __shared__ __attribute__((aligned(16))) float s_o[KS > 1 ? HPW * KS * kWaveFloats : 4];
+  __shared__ float s_ml[KS > 1 ? HPW * KS * 32 : 2];
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) {
+    const int q = qt * 16 + n;
+    const int64_t token = t.qs + q;
+    float M = m[qt], L = sum_xor16_32(l[qt]);
+    auto finish = [&](int mt, f32x4_t acc) {
+      if (q >= t.qc) return;
+      const int64_t at = (token * H + h) * kHeadDim + 16 * mt + 4 * g;
+      if (P.parts == 1) {
+        // L = 0 only for a query that sees no key (an empty row): zeros, not NaN
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        u32x2_t w2;
+        w2[0] = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+        w2[1] = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+        *reinterpret_cast<u32x2_t*>(P.out + at) = w2;
+      } else {
+        *reinterpret_cast<f32x4_t*>(P.part_o + static_cast<int64_t>(part) * P.n_q * H * kHeadDim + at) = acc;
+        if (mt == 0 && g == 0) {
+          float* ml = P.part_ml + (static_cast<int64_t>(part) * P.n_q * H + token * H + h) * 2;
+          ml[0] = M;
+          ml[1] = L;
+        }
+      }
+    };
+    if constexpr (KS == 1) {
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) finish(mt, o[qt][mt]);
+    } else {
+      float* so = s_o + hsub * KS * kWaveFloats;
+      float* sml = s_ml + hsub * KS * 32;
+      if (qt > 0) __syncthreads();  // the previous tile has been read
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+        *reinterpret_cast<f32x4_t*>(so + ks * kWaveFloats + (mt * 64 + lane) * 4) = o[qt][mt];
+      if (g == 0) {
+        sml[ks * 32 + n] = M;
+        sml[ks * 32 + 16 + n] = L;
+      }
+      __syncthreads();
+      M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < KS; ++w) M = fmaxf(M, sml[w * 32 + n]);
+      const float mref = M == -INFINITY ? 0.f : M;
+      float sc[KS];
+      L = 0.f;
+#pragma unroll
+      for (int w = 0; w < KS; ++w) {
+        sc[w] = __builtin_amdgcn_exp2f(sml[w * 32 + n] - mref);
+        L += sc[w] * sml[w * 32 + 16 + n];
+      }
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        if (mt % KS != ks) continue;
+        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < KS; ++w)
+          acc += sc[w] * *reinterpret_cast<const f32x4_t*>(so + w * kWaveFloats + (mt * 64 + lane) * 4);
+        finish(mt, acc);
+      }
+    }
+  }
+}
+
+// Joins the parts of every query: thread (query, head, 4 head-dim values).
+__global__ __launch_bounds__(256) void attn_window_join_kernel(const WindowParams P) {
+  const int lane = threadIdx.x & 63;
+  const int per = 256 / 16;  // (query, head) pairs of a workgroup
+  const int64_t pair = static_cast<int64_t>(blockIdx.x) * per + (threadIdx.x >> 4);
+  const int64_t row_q = pair / P.H;
+  const int h = static_cast<int>(pair - row_q * P.H);
+  const int r = static_cast<int>(row_q / P.max_q), i = static_cast<int>(row_q - static_cast<int64_t>(r) * P.max_q);
+  if (r >= P.rows) return;
+  int qs = r * P.max_q, qc = P.max_q;
+  if (P.q_start != nullptr) {
+    qs = first_query(P, r);
+    qc = min(max(first_query(P, r + 1) - qs, 0), P.max_q);
+  }
+  if (i >= qc) return;
+  const int64_t step = static_cast<int64_t>(P.n_q) * P.H;
+  const int64_t at = static_cast<int64_t>(qs + i) * P.H + h;
+  float M = -INFINITY;
+  for (int s = 0; s < P.parts; ++s) M = fmaxf(M, P.part_ml[(s * step + at) * 2]);
+  const float mref = M == -INFINITY ? 0.f : M;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  float L = 0.f;
+  for (int s = 0; s < P.parts; ++s) {
+    const float w = __builtin_amdgcn_exp2f(P.part_ml[(s * step + at) * 2] - mref);
+    L += w * P.part_ml[(s * step + at) * 2 + 1];
+    acc += w * *reinterpret_cast<const f32x4_t*>(P.part_o + (s * step + at) * kHeadDim + (lane & 15) * 4);
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  u32x2_t w2;
+  w2[0] = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  w2[1] = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+  *reinterpret_cast<u32x2_t*>(P.out + at * kHeadDim + (lane & 15) * 4) = w2;
+}
+
+// How a call is cut: 16 * nqt queries a tile, ks waves to a part's chunks, parts.
+struct Cut {
+  int nqt, ks, parts;
+  int64_t slots;
+};
+
+constexpr int64_t kWavesWanted = 2048;  // two a SIMD
+
+Cut cut_of(int rows, int max_q, int n_q, bool packed, int n_heads, int window, int sinks, int max_kv) {
+  Cut c;
+  c.nqt = std::min((max_q + 15) / 16, 4);
+  const int tq = 16 * c.nqt;
+  c.slots = packed ? n_q / tq + static_cast<int64_t>(rows) : static_cast<int64_t>(rows) * ((max_q + tq - 1) / tq);
+  const int64_t tiles = std::min<int64_t>(c.slots, (n_q + tq - 1) / tq + rows);
+  const int64_t keys = std::min<int64_t>(max_kv, static_cast<int64_t>(window) + sinks + tq);
+  const int64_t chunks = (keys + kChunk - 1) / kChunk + 1;
+  const int64_t waves = tiles * n_heads;
+  c.ks = waves * 4 <= kWavesWanted && chunks >= 8 ? 8 : waves <= kWavesWanted && chunks >= 4 ? 4 : 1;
+  // more parts only where eight waves are not enough, each with eight chunks a wave
+  const int64_t want = (kWavesWanted + waves * c.ks - 1) / (waves * c.ks);
+  c.parts = c.ks < 8 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, chunks / (8 * c.ks))));
+  return c;
+}
+
+template <int NQT>
+void launch_tiles(const WindowParams& P, const Cut& c, hipStream_t st) {
+  const int64_t items = c.slots * P.parts;
+  if (c.ks == 8)
+    hipLaunchKernelGGL((attn_window_kernel<NQT, 8, 1>), dim3(items * P.H), dim3(512), 0, st, P);
+  else if (c.ks == 4)
+    hipLaunchKernelGGL((attn_window_kernel<NQT, 4, 1>), dim3(items * P.H), dim3(256), 0, st, P);
+  else
+    hipLaunchKernelGGL((attn_window_kernel<NQT, 1, 4>), dim3(items * (P.H / 4)), dim3(256), 0, st, P);
+}
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int window_checks(int rows, int max_q, int n_q, int n_heads, int window, int sinks, int max_kv) {
+  YAPD_REQUIRE(rows >= 1 && max_q >= 1 && n_q >= 1, "attn_window: need rows, max_q and n_q >= 1 (got %d, %d, %d)", rows,
+               max_q, n_q);
+  YAPD_REQUIRE(n_heads >= 4 && n_heads % 4 == 0 && n_heads <= 1024,
+               "attn_window: n_heads must be a multiple of 4, at most 1024 (got %d)", n_heads);
+  YAPD_REQUIRE(window >= 1 && sinks >= 0, "attn_window: need window >= 1 and sinks >= 0 (got %d, %d)", window, sinks);
+  YAPD_REQUIRE(max_kv >= 1, "attn_window: max_kv must be >= 1 (got %d)", max_kv);
+  return YAPD_OK;
+}
+
+}  // namespace
+}  // namespace yapd
+
+extern "C" int64_t yapd_attn_window_workspace(int rows, int max_q, int n_q, int packed, int n_heads, int window,
+                                              int sinks, int max_kv) {
+  if (yapd::window_checks(rows, max_q, n_q, n_heads, window, sinks, max_kv) != YAPD_OK) return -1;
+  const yapd::Cut c = yapd::cut_of(rows, max_q, n_q, packed != 0, n_heads, window, sinks, max_kv);
+  return c.parts == 1 ? 0 : static_cast<int64_t>(c.parts) * n_q * n_heads * (yapd::kHeadDim + 2);
+}
+
+extern "C" int yapd_attn_window(const void* q, int64_t q_tok_stride, const void* kv_pool, int64_t n_pages,
+                                const int32_t* page_table, int table_stride, int table_cols, const int32_t* kv_len,
+                                const int32_t* q_start, int rows, int max_q, int n_q, int n_heads, int window, int sinks,
+                                int causal, int max_kv, float scale, float* workspace, int64_t workspace_floats,
+                                void* out, void* stream) {
+  YAPD_REQUIRE(q && kv_pool && page_table && kv_len && out, "attn_window: NULL pointer");
+  if (int rc = yapd::window_checks(rows, max_q, n_q, n_heads, window, sinks, max_kv)) return rc;
+  YAPD_REQUIRE(yapd::al16(q) && yapd::al16(kv_pool) && yapd::al16(out),
+               "attn_window: q, kv_pool and out must be 16-byte aligned");
+  YAPD_REQUIRE(q_tok_stride >= static_cast<int64_t>(n_heads) * yapd::kHeadDim && q_tok_stride % 8 == 0,
+               "attn_window: q_tok_stride must be a multiple of 8, at least n_heads * 64");
+  YAPD_REQUIRE(n_pages >= 1 && table_cols >= 1 && table_stride >= table_cols, "attn_window: empty pool or table");
+  YAPD_REQUIRE(table_cols <= yapd::kCap / yapd::kPageSize, "attn_window: table_cols must be at most 2^26");
+  YAPD_REQUIRE(q_start != nullptr || n_q == static_cast<int64_t>(rows) * max_q,
+               "attn_window: without q_start n_q must be rows * max_q");
+  YAPD_REQUIRE(std::isfinite(scale) && scale > 0.f, "attn_window: scale must be finite and > 0");
+  const yapd::Cut c = yapd::cut_of(rows, max_q, n_q, q_start != nullptr, n_heads, window, sinks, max_kv);
+  YAPD_REQUIRE(c.slots * c.parts * n_heads < (int64_t{1} << 22), "attn_window: too many tiles for one launch");
+  const int64_t tokens = static_cast<int64_t>(c.parts) * n_q * n_heads;
+  YAPD_REQUIRE(c.parts == 1 || (workspace && yapd::al16(workspace) &&
+                                workspace_floats >= tokens * (yapd::kHeadDim + 2)),
+               "attn_window: the workspace must be 16-byte aligned and hold %lld floats",
+               static_cast<long long>(tokens * (yapd::kHeadDim + 2)));
+  yapd::WindowParams P;
+  P.q = static_cast<const uint16_t*>(q);
+  P.q_stride = q_tok_stride;
+  P.pool = static_cast<const uint16_t*>(kv_pool);
+  P.n_pages = n_pages;
+  P.table = page_table;
+  P.table_stride = table_stride;
+  P.table_cols = table_cols;
+  P.kv_len = kv_len;
+  P.q_start = q_start;
+  P.rows = rows;
+  P.max_q = std::min(max_q, n_q);
+  P.n_q = n_q;
+  P.H = n_heads;
+  P.window = std::min(window, yapd::kCap);
+  P.sinks = std::min(sinks, yapd::kCap);
+  P.causal = causal != 0;
+  P.parts = c.parts;
+  P.part_o = workspace;
+  P.part_ml = c.parts == 1 ? nullptr : workspace + tokens * yapd::kHeadDim;
+  P.scale_log2 = scale * 1.4426950408889634f;
+  P.out = static_cast<uint16_t*>(out);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (c.nqt) {
+    case 1: yapd::launch_tiles<1>(P, c, st); break;
+    case 2: yapd::launch_tiles<2>(P, c, st); break;
+    case 3: yapd::launch_tiles<3>(P, c, st); break;
+    default: yapd::launch_tiles<4>(P, c, st); break;
+  }
+  YAPD_LAUNCH_CHECK("attn_window_kernel launch");
+  if (c.parts > 1) {
+    const int64_t pairs = static_cast<int64_t>(rows) * P.max_q * n_heads;
+    hipLaunchKernelGGL(yapd::attn_window_join_kernel, dim3(static_cast<unsigned>((pairs + 15) / 16)), dim3(256), 0, st,
+                       P);
+    YAPD_LAUNCH_CHECK("attn_window_join_kernel launch");
+  }
+  return YAPD_OK;
+}

@@ -39,6 +39,10 @@ _SIGNATURES = {
     "yapd_attn_paged_block_noalloc": (c_int, [
         c_void, c_void, c_i64, c_void, c_int, c_int, c_void, c_int, c_int, c_int, c_void, c_int, c_void, c_int,
         c_void, c_int, c_float, c_int, c_void, c_void]),
+    "yapd_attn_window": (c_int, [
+        c_void, c_i64, c_void, c_i64, c_void, c_int, c_int, c_void, c_void, c_int, c_int, c_int, c_int, c_int, c_int,
+        c_int, c_int, c_float, c_void, c_i64, c_void, c_void]),
+    "yapd_attn_window_workspace": (c_i64, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "yapd_kv_write": (c_int, [c_void, c_void, c_i64, c_i64, c_void, c_i64, c_void, c_int, c_int, c_void, c_int,
                               c_int, c_int, c_void]),
     "yapd_kv_gather": (c_int, [c_void, c_i64, c_void, c_int, c_int, c_int, c_void, c_void, c_void]),
@@ -292,6 +296,87 @@ def attn_paged_block(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, k
         kv_len.data_ptr(),
         rows, bl, H, work.data_ptr(), int(work.shape[0]), ptr(merge), n_merge, None, ptr(part_o), ptr(part_ml),
         n_slots, float(scale), int(bool(causal)), out.data_ptr(), stream_ptr(dev)))
+
+
+WINDOW_CAP = 2**30  # windows, sinks and lengths from here on are taken as this
+
+
+def attn_window(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, out: torch.Tensor,
+                scale: float, *, window: int, sinks: int = 0, causal: bool = True,
+                q_start: Optional[torch.Tensor] = None, max_q: Optional[int] = None, max_kv: Optional[int] = None,
+                workspace: Optional[torch.Tensor] = None) -> None:
+    """``out = softmax(q K^T * scale) V`` over each row's pages with a sliding window and sink tokens.
+
+    Query ``i`` of a row with ``n`` queries stands at position ``p = kv_len - n + i`` and sees key
+    ``j`` iff ``j < hi`` and (``j < sinks`` or ``j > p - window``), with ``hi = p + 1`` (``causal``) or
+    ``kv_len`` (a block step).  Queries are ``[rows, bl, H, 64]``, or packed ``[n_q, H, 64]`` with the
+    device ``q_start [rows + 1]`` (int32, not decreasing): row ``r`` has rows ``q_start[r]`` up to
+    ``q_start[r + 1]`` of ``q`` and ``out``, at most ``max_q`` of them; rows of ``out`` that belong to no
+    row are left as they were.  ``q`` may be a view with packed heads and any token stride (a slice of
+    a fused QKV buffer); ``out`` is contiguous and must not overlap ``q``.
+
+    Lengths are read on the device: no plan, and a captured call follows them.  ``max_q`` and
+    ``max_kv`` are the host's upper bounds (default: all queries, all positions the table maps).
+    Few queries over many keys need a float32 ``workspace``
+    (``yapd_attn_window_workspace``), allocated here unless given.
+    """
+    dev = q.device
+    if q.is_cuda and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):  # the launch goes to the current device
+            return attn_window(q, pool, table, kv_len, out, scale, window=window, sinks=sinks, causal=causal,
+                               q_start=q_start, max_q=max_q, max_kv=max_kv, workspace=workspace)
+    require_cuda(q, "q", torch.bfloat16, dev, contiguous=False)
+    shape, stride = q.shape, q.stride()
+    packed = q_start is not None
+    require(q.numel() == 0 or (stride[-1] == 1 and len(shape) >= 2 and stride[-2] == 64), "q's heads must be packed")
+    if packed:
+        require(len(shape) == 3 and shape[2] == 64, "packed q must be [n_q, H, 64]")
+        n_q, H, _ = shape
+        require_cuda(q_start, "q_start", torch.int32, dev)
+        rows = q_start.numel() - 1
+        require(rows >= 0, "q_start must be [rows + 1]")
+        if max_q is None:
+            max_q = n_q
+        require(n_q == 0 or rows == 0 or max_q >= 1, "max_q must be >= 1")
+        tok = stride[0] if n_q > 1 else H * 64
+    else:
+        require(len(shape) == 4 and shape[3] == 64, "q must be [rows, bl, H, 64] (or [n_q, H, 64] with q_start)")
+        rows, bl, H, _ = shape
+        n_q = rows * bl
+        require(max_q is None or max_q == bl, "max_q is given by q's shape unless q is packed")
+        max_q = bl
+        tok = stride[1] if bl > 1 else stride[0] if rows > 1 else H * 64
+        require(rows <= 1 or stride[0] == bl * tok, "q's rows must follow each other")
+    require_cuda(pool, "pool", torch.bfloat16, dev)
+    if not (pool.dim() == 4 and pool.shape[1] == 2 and pool.shape[2] == H and pool.shape[3] == 1024):
+        raise ValueError("pool must be [pages, 2, H, 16*64]")
+    require_cuda(table, "table", torch.int32, dev, contiguous=False)
+    require(table.dim() == 2 and table.shape[0] >= rows and (table.shape[1] == 1 or table.stride(1) == 1),
+            "table must be [>= rows, max_pages] with unit column stride")
+    require(rows <= 1 or table.stride(0) >= table.shape[1], "table rows must not overlap")
+    require_cuda(kv_len, "kv_len", torch.int32, dev)
+    require(kv_len.numel() >= rows, "kv_len must have rows entries")
+    require_cuda(out, "out", torch.bfloat16, dev)
+    require(out.shape == shape, "out must match q")
+    require(window >= 1 and sinks >= 0, "need window >= 1 and sinks >= 0")
+    if n_q == 0 or rows == 0:
+        return
+    cols = table.shape[1]
+    require(cols >= 1, "the table maps no page")
+    window, sinks = min(int(window), WINDOW_CAP), min(int(sinks), WINDOW_CAP)
+    kv_max = cols * 16 if max_kv is None else min(int(max_kv), cols * 16)
+    require(kv_max >= 1, "max_kv must be >= 1")
+    max_q = min(int(max_q), n_q)
+    lib = load_library()
+    need = lib.yapd_attn_window_workspace(rows, max_q, n_q, packed, H, window, sinks, kv_max)
+    if need > 0 and workspace is None:
+        workspace = torch.empty(need, dtype=torch.float32, device=dev)
+    if workspace is not None:
+        require_cuda(workspace, "workspace", torch.float32, dev)
+    check(lib.yapd_attn_window(
+        q.data_ptr(), tok, pool.data_ptr(), pool.shape[0], table.data_ptr(), max(table.stride(0), cols), cols,
+        kv_len.data_ptr(), ptr(q_start), rows, max_q, n_q, H, window, sinks, causal, kv_max, scale, ptr(workspace),
+        0 if workspace is None else workspace.numel(), out.data_ptr(), stream_ptr(dev)))
 
 
 def kv_write(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: torch.Tensor,
