@@ -101,6 +101,16 @@ int yapd_kv_write(const void* k, const void* v, int64_t k_tok_stride, int64_t v_
 int yapd_kv_gather(const void* kv_pool, int64_t n_pages, const int32_t* table_row, int table_len, int kv_len,
                    int n_heads, void* k_out, void* v_out, void* stream);
 
+/* Copies whole pages inside every layer's pool: kv_pools[l][dst[i]] =
+ * kv_pools[l][src[i]] for l < n_layers, i < n_pairs (a fork's partial last
+ * page, a prefix, a compaction).  kv_pools (pool addresses), src and dst are
+ * host arrays, read before the call returns.  A source may repeat; a page that is
+ * the destination of two pairs, or a source and a destination, is refused, so
+ * the result does not depend on the order of the copies.  n_pairs = 0 launches
+ * nothing.  It has no counterpart in the reference. */
+int yapd_kv_copy_pages(void* const* kv_pools, int n_layers, int64_t n_pages, int n_heads, const int32_t* src,
+                       const int32_t* dst, int n_pairs, void* stream);
+
 /* Host-side planner (CPU only, no GPU call): cuts each row's kv_len keys
  * into work items of whole 32-key chunks so that ~target_items items exist,
  * none shorter than min_split_keys (>= 32) unless the whole row is, longest

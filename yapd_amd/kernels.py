@@ -46,6 +46,7 @@ _SIGNATURES = {
     "yapd_kv_write": (c_int, [c_void, c_void, c_i64, c_i64, c_void, c_i64, c_void, c_int, c_int, c_void, c_int,
                               c_int, c_int, c_void]),
     "yapd_kv_gather": (c_int, [c_void, c_i64, c_void, c_int, c_int, c_int, c_void, c_void, c_void]),
+    "yapd_kv_copy_pages": (c_int, [c_void, c_int, c_i64, c_int, c_void, c_void, c_int, c_void]),
     "yapd_gemm_bf16": (c_int, [c_void, c_i64, c_void, c_i64, c_int, c_int, c_int, c_void, c_i64, c_void]),
     "yapd_gemm_bf16_residual": (c_int, [c_void, c_i64, c_void, c_i64, c_int, c_int, c_int, c_void, c_i64, c_void]),
     "yapd_gemm_head_shift": (c_int, [c_void, c_void, c_int, c_int, c_int, c_void, c_i64, c_int, c_void, c_i64,
@@ -411,6 +412,55 @@ def kv_gather(pool: torch.Tensor, table_row: torch.Tensor, kv_len: int):
     check(load_library().yapd_kv_gather(pool.data_ptr(), pool.shape[0], table_row.data_ptr(), table_row.numel(),
                                         int(kv_len), H, k.data_ptr(), v.data_ptr(), stream_ptr(dev)))
     return k, v
+
+
+def pool_pointers(pools):
+    """The device addresses of every layer's pool as the array :func:`kv_copy_pages` hands on, and the
+    pools' common shape and device, checked."""
+    require(len(pools) >= 1, "no pools")
+    shape, dev = pools[0].shape, pools[0].device
+    require(len(shape) == 4 and shape[0] >= 1 and shape[1] == 2 and shape[3] == 1024, "pools must be [pages, 2, H, 16*64]")
+    for p in pools:
+        require_cuda(p, "pool", torch.bfloat16, dev)
+        if p.shape != shape:
+            raise ValueError("every layer's pool must have the same shape")
+    return (c_void * len(pools))(*[p.data_ptr() for p in pools]), shape, dev
+
+
+def page_ids(ids, name: str):
+    """Host page ids (a sequence of integers or an integer array) as int32."""
+    import numpy as np
+    if isinstance(ids, torch.Tensor):
+        require(not ids.is_cuda, f"{name} must be host integers, not a GPU tensor")
+        ids = ids.numpy()
+    a = np.asarray(ids)
+    if a.dtype != np.int32:
+        require(a.size == 0 or (a.dtype.kind in "iu" and bool((a >= 0).all()) and bool((a < 2**31).all())),
+                f"{name} must be page ids (integers of [0, 2^31))")
+        a = a.astype(np.int32)
+    require(a.ndim == 1, f"{name} must be one-dimensional")
+    return np.ascontiguousarray(a)
+
+
+def kv_copy_pages(pools, src, dst) -> None:
+    """``pool[dst[i]] = pool[src[i]]`` for every pair ``i`` in every layer's pool of ``pools``, in one
+    launch (per 64 layers and 384 pairs).
+
+    ``src`` and ``dst`` are host page ids.  A source may repeat (a fork); a page that is the
+    destination of two pairs, or a source and a destination, is refused, so the result does not
+    depend on the order of the copies."""
+    kv_copy_pages_at(*pool_pointers(pools), src, dst)
+
+
+def kv_copy_pages_at(ptrs, shape, dev: torch.device, src, dst) -> None:
+    """:func:`kv_copy_pages` on what :func:`pool_pointers` gave for pools that are still alive."""
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):  # the launch goes to the current device
+            return kv_copy_pages_at(ptrs, shape, dev, src, dst)
+    src, dst = page_ids(src, "src"), page_ids(dst, "dst")
+    require(src.size == dst.size, "src and dst must have the same length")
+    check(load_library().yapd_kv_copy_pages(ptrs, len(ptrs), shape[0], shape[2], src.ctypes.data, dst.ctypes.data,
+                                            src.size, stream_ptr(dev)))
 
 
 # --------------------------------------------------------------------------- #

@@ -7,6 +7,10 @@ zero-filled pool ``[pages, 2, H, 16*64]`` (layout in csrc/kv_layout.h), rows
 map positions to pages through an int32 table that may be any permutation of
 pool pages, and the attention work list is built once per block by the
 native planner (``yapd_attn_plan``) and uploaded.
+
+:class:`SharedPagedKV` maps pages on demand instead of a slice per row: rows
+share a prefix by reference count, pages behind an attention window go back to
+the pool, and the pool is compacted.
 """
 
 from __future__ import annotations
@@ -55,17 +59,20 @@ class PagedKV:
         self.device = torch.device(device)
         self.n_pages = int(n_pages) if n_pages is not None else self.n_rows * self.pages_per_row
         kernels.require(self.n_pages >= self.n_rows * self.pages_per_row, "pool smaller than rows * pages_per_row")
-        self.pools: List[torch.Tensor] = [
-            torch.zeros(self.n_pages, 2, self.n_heads, PAGE_SIZE * HEAD_DIM, dtype=torch.bfloat16,
-                        device=self.device)
-            for _ in range(self.n_layers)
-        ]
+        self._make_pools()
         order = np.arange(self.n_pages, dtype=np.int32)
         if shuffle_seed is not None:
             order = np.random.default_rng(shuffle_seed).permutation(self.n_pages).astype(np.int32)
         take = order[: self.n_rows * self.pages_per_row]
         self.table_host = take.reshape(self.n_rows, self.pages_per_row).copy()
         self.table = torch.from_numpy(self.table_host).to(self.device)
+
+    def _make_pools(self) -> None:
+        self.pools: List[torch.Tensor] = [
+            torch.zeros(self.n_pages, 2, self.n_heads, PAGE_SIZE * HEAD_DIM, dtype=torch.bfloat16,
+                        device=self.device)
+            for _ in range(self.n_layers)
+        ]
 
     @property
     def bytes_per_layer(self) -> int:
@@ -81,13 +88,206 @@ class PagedKV:
         self.table[a].copy_(self.table[b])
         self.table[b].copy_(tmp)
 
+    def copy_pages(self, src, dst) -> None:
+        """``pool[dst[i]] = pool[src[i]]`` in every layer's pool for host page ids (see
+        :func:`kernels.kv_copy_pages`), on the current stream; torch's index operations on the CPU."""
+        if self.device.type == "cuda":
+            kernels.kv_copy_pages(self.pools, src, dst)
+            return
+        src, dst = (torch.as_tensor(np.asarray(x, dtype=np.int64)) for x in (src, dst))
+        for pool in self.pools:
+            pool.index_copy_(0, dst, pool.index_select(0, src))
+
     def copy_row_pages(self, src_row: int, dst_row: int, n_positions: int) -> None:
         """Copy the pages holding positions ``[0, n_positions)`` of one row to another, every layer."""
         npg = (n_positions + PAGE_SIZE - 1) // PAGE_SIZE
-        src = to_device_async(self.table_host[src_row, :npg], torch.int64, self.device)
-        dst = to_device_async(self.table_host[dst_row, :npg], torch.int64, self.device)
+        src, dst = self.table_host[src_row, :npg].copy(), self.table_host[dst_row, :npg].copy()
+        targets = set(dst.tolist())
+        if len(targets) == len(dst) and targets.isdisjoint(src.tolist()):
+            self.copy_pages(src, dst)
+            return
+        # rows that share pages: every source is read before any page is written
+        src_t, dst_t = (to_device_async(x, torch.int64, self.device) for x in (src, dst))
         for pool in self.pools:
-            pool.index_copy_(0, dst, pool.index_select(0, src))
+            pool.index_copy_(0, dst_t, pool.index_select(0, src_t))
+
+
+class SharedPagedKV(PagedKV):
+    """A paged KV cache whose rows map pages on demand and share them by reference count.
+
+    A row maps a page when :meth:`reserve` first covers one of its positions; :meth:`fork` gives other
+    rows the same pages (the partial last one as a copy of their own); :meth:`release` and
+    :meth:`release_before` give pages back; :meth:`compact` moves the mapped pages to the pool's front.
+    Table entries that map nothing name page 0, which is never handed out: it takes stray writes and
+    holds nothing.  Attention must not see positions whose page was released (``kernels.attn_window``
+    does not, for a window no longer than what was kept).
+
+    The bookkeeping is on the host and takes effect at once; table uploads and page copies go to the
+    current stream, which has to be the one (or ordered with the one) that the cache is used on.  Not
+    for use inside a graph capture; a captured launch reads the tables and pools, whose addresses stay.
+    """
+
+    def __init__(self, *, n_layers: int, n_rows: int, pages_per_row: int, n_heads: int, device: torch.device,
+                 n_pages: int):
+        """``n_pages`` counts the pool's pages, page 0 included; a row maps at most ``pages_per_row``."""
+        kernels.require(n_layers >= 1 and n_rows >= 1 and pages_per_row >= 1 and n_heads >= 1 and n_pages >= 2,
+                        "need at least one layer, row, page per row and head, and two pages")
+        self.n_layers = int(n_layers)
+        self.n_rows = int(n_rows)
+        self.pages_per_row = int(pages_per_row)
+        self.n_heads = int(n_heads)
+        self.device = torch.device(device)
+        self.n_pages = int(n_pages)
+        self._make_pools()
+        if self.device.type == "cuda":
+            self._handle = kernels.pool_pointers(self.pools)
+        self.table_host = np.zeros((self.n_rows, self.pages_per_row), dtype=np.int32)
+        self.table = torch.zeros(self.n_rows, self.pages_per_row, dtype=torch.int32, device=self.device)
+        self._refs = np.zeros(self.n_pages, dtype=np.int32)
+        self._refs[0] = 1
+        self._free = list(range(self.n_pages - 1, 0, -1))  # the lowest free page is handed out first
+
+    @property
+    def free_pages(self) -> int:
+        """Pages that :meth:`reserve` and :meth:`fork` can still take."""
+        return len(self._free)
+
+    def refcount(self, page: int) -> int:
+        """Rows that map ``page``."""
+        return int(self._refs[page])
+
+    def copy_pages(self, src, dst) -> None:
+        if self.device.type == "cuda":
+            kernels.kv_copy_pages_at(*self._handle, src, dst)
+        else:
+            super().copy_pages(src, dst)
+
+    # ------------------------------------------------------------------ #
+
+    def _check_row(self, row: int) -> None:
+        kernels.require(0 <= row < self.n_rows, f"row {row} outside [0, {self.n_rows})")
+
+    def _take(self, n: int) -> List[int]:
+        if n > len(self._free):
+            raise RuntimeError(f"the pool is out of pages: {n} needed, {len(self._free)} free")
+        return [self._free.pop() for _ in range(n)]
+
+    def _drop(self, pages: np.ndarray) -> None:
+        """One reference of each page (ids of mapped entries, repeats allowed) is gone."""
+        np.subtract.at(self._refs, pages, 1)
+        gone = np.unique(pages)
+        self._free.extend(gone[self._refs[gone] == 0][::-1].tolist())
+
+    def _upload(self, rows: Sequence[int]) -> None:
+        a, b = min(rows), max(rows) + 1
+        copy_from_host_async(self.table[a:b], self.table_host[a:b].copy())
+
+    def reserve(self, row: int, begin: int, end: int) -> None:
+        """Map positions ``[begin, end)`` of ``row`` to pages that no other row shares, so that they can be
+        written: an unmapped page is taken from the pool, a shared one replaced by a copy.  Raises
+        ``RuntimeError``, with nothing changed, if the pool has too few pages left."""
+        self._check_row(row)
+        kernels.require(0 <= begin <= end <= self.pages_per_row * PAGE_SIZE,
+                        f"positions [{begin}, {end}) outside what a row maps")
+        if begin == end:
+            return
+        c0, c1 = begin // PAGE_SIZE, (end - 1) // PAGE_SIZE + 1
+        now = self.table_host[row, c0:c1]
+        new = np.nonzero((now == 0) | (self._refs[now] > 1))[0]
+        if not len(new):
+            return
+        old, pages = now[new].copy(), np.asarray(self._take(len(new)), dtype=np.int32)
+        self.table_host[row, c0 + new] = pages
+        self._refs[pages] = 1
+        shared = old != 0
+        if shared.any():
+            self.copy_pages(old[shared], pages[shared])
+            self._drop(old[shared])
+        self._upload([row])
+
+    def fork(self, src_row: int, dst_rows: Sequence[int], n_positions: int) -> None:
+        """Give every row of ``dst_rows`` (rows that map nothing) the first ``n_positions`` positions of
+        ``src_row``: whole pages are shared, a partial last page is copied, one copy a row, all in one
+        launch.  What of the source was released stays unmapped."""
+        rows = [int(r) for r in dst_rows]
+        for r in (src_row, *rows):
+            self._check_row(r)
+        kernels.require(len(set(rows)) == len(rows) and src_row not in rows, "a fork's rows must be distinct")
+        kernels.require(0 <= n_positions <= self.pages_per_row * PAGE_SIZE, "n_positions outside what a row maps")
+        kernels.require(not self.table_host[rows].any(), "a fork's destination rows must map nothing")
+        if not rows or n_positions == 0:
+            return
+        whole, part = divmod(n_positions, PAGE_SIZE)
+        tail = int(self.table_host[src_row, whole]) if part else 0
+        own = self._take(len(rows)) if tail else []
+        shared = self.table_host[src_row, :whole]
+        self.table_host[rows, :whole] = shared
+        self._refs[shared[shared != 0]] += len(rows)
+        if tail:
+            self.table_host[rows, whole] = own
+            self._refs[own] = 1
+            self.copy_pages([tail] * len(own), own)
+        self._upload(rows)
+
+    def release(self, row: int) -> None:
+        """Unmap every page of ``row``."""
+        self._release(row, np.arange(self.pages_per_row))
+
+    def release_before(self, row: int, position: int, sinks: int = 0) -> None:
+        """Unmap the pages of ``row`` whose positions all lie in ``[sinks, position)``: what a window that
+        begins at ``position``, with ``sinks`` first tokens kept, no longer sees.  Nothing for a ``position``
+        of 0 or less."""
+        kernels.require(sinks >= 0, "sinks must be >= 0")
+        first = (sinks + PAGE_SIZE - 1) // PAGE_SIZE
+        self._release(row, np.arange(first, min(position // PAGE_SIZE, self.pages_per_row)))
+
+    def _release(self, row: int, cols: np.ndarray) -> None:
+        self._check_row(row)
+        cols = cols[self.table_host[row, cols] != 0]
+        if not len(cols):
+            return
+        self._drop(self.table_host[row, cols])
+        self.table_host[row, cols] = 0
+        self._upload([row])
+
+    def compact(self) -> int:
+        """Move the mapped pages to the pool's front (one launch, and an upload of the table); returns how
+        many pages are in use, page 0 included: pages from there on hold nothing."""
+        live = np.nonzero(self._refs)[0]
+        n = len(live)
+        src = live[live >= n]
+        if len(src):
+            dst = np.nonzero(self._refs[:n] == 0)[0]  # as many holes in front as pages behind
+            self.copy_pages(src, dst)
+            where = np.arange(self.n_pages, dtype=np.int32)
+            where[src] = dst
+            self.table_host = where[self.table_host]
+            self._refs[dst] = self._refs[src]
+            self._refs[src] = 0
+            self._upload([0, self.n_rows - 1])
+        self._free = list(range(self.n_pages - 1, n - 1, -1))
+        return n
+
+    def copy_row_pages(self, src_row: int, dst_row: int, n_positions: int) -> None:
+        """Positions ``[0, n_positions)`` of ``src_row`` as pages of ``dst_row``'s own; what the destination
+        mapped there is given back.  Unmapped source pages stay unmapped."""
+        self._check_row(src_row)
+        self._check_row(dst_row)
+        kernels.require(0 <= n_positions <= self.pages_per_row * PAGE_SIZE, "n_positions outside what a row maps")
+        if src_row == dst_row or n_positions == 0:
+            return
+        cols = np.arange((n_positions + PAGE_SIZE - 1) // PAGE_SIZE)
+        src = self.table_host[src_row, cols]
+        mapped = src != 0
+        own = self._take(int(mapped.sum()))
+        old = self.table_host[dst_row, cols]
+        new = np.zeros_like(src)
+        new[mapped] = own
+        self._refs[own] = 1
+        self.copy_pages(src[mapped], own)
+        self.table_host[dst_row, cols] = new
+        self._drop(old[old != 0])
+        self._upload([dst_row])
 
 
 class AttnPlan:
