@@ -80,6 +80,25 @@ int yapd_score_cfg_pmi_unmask(
     int32_t* n_mask_after_out, uint8_t* hit_eos_out, void* stream);
 
 
+/* Log probabilities of given tokens, with the entropy and the best
+ * alternatives of each position (what ranks candidates of one utterance; the
+ * reference has no counterpart).  logits: bf16 (wide = 0) or fp32 (wide = 1),
+ * element (row, pos, v) at row * seq_stride + pos * pos_stride + v, aligned to
+ * its type only; any strides (a 16-byte granule that holds an element of a row
+ * may be read whole).  With lse = ln sum_v e^(x_v):
+ *   logprob[i] = x_token - lse (token < 0: 0, a position without a token;
+ *     token >= vocab: NaN),  entropy[i] = -sum_v p_v ln p_v (0 ln 0 = 0),
+ *   top_token[i][0..top_k) the largest logits' indices, ties the lowest index
+ *   first, and top_logprob their log probabilities.  0 <= top_k <= 32, <= vocab.
+ * -inf logits have probability 0.  A row that holds a NaN or +inf, or -inf
+ * alone, has NaN for every probability; its top tokens rank NaN as -inf.
+ * Sums are fp32 and in a fixed order: the same call gives the same bits.
+ * tokens int64, outputs fp32 and int64, [rows * bl] and [rows * bl, top_k]
+ * (NULL allowed with top_k = 0).  One launch, no workspace. */
+int yapd_token_logprobs(const void* logits, int wide, int64_t seq_stride, int64_t pos_stride, int rows, int bl,
+                        int vocab, const int64_t* tokens, int top_k, float* logprob, float* entropy,
+                        float* top_logprob, int64_t* top_token, void* stream);
+
 /* ------------------------------------------------------------------------ *
  * Paged KV pool (one per layer): bf16 [n_pages][2][H][16*64]; plane 0 holds
  * K (token-major inside a head), plane 1 holds V transposed inside a head.

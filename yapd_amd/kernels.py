@@ -32,6 +32,8 @@ _SIGNATURES = {
         c_void, c_i64, c_i64, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
         c_void, c_void, c_void, c_void, c_void, c_void, c_int, c_float, c_int, c_i64, c_i64,
         c_float, c_int, c_u64, c_u64, c_void, c_void, c_void, c_void, c_void, c_void, c_void]),
+    "yapd_token_logprobs": (c_int, [c_void, c_int, c_i64, c_i64, c_int, c_int, c_int, c_void, c_int, c_void, c_void,
+                                    c_void, c_void, c_void]),
     "yapd_attn_plan": (c_int, [c_void, c_int, c_int, c_int, c_void, c_int, c_void, c_int, c_void, c_void, c_void]),
     "yapd_attn_paged_block": (c_int, [
         c_void, c_void, c_i64, c_void, c_int, c_int, c_void, c_int, c_int, c_int, c_void, c_int, c_void, c_int,
@@ -227,6 +229,47 @@ def score_cfg_pmi_unmask(
         out["sampled"].data_ptr(), out["pmi"].data_ptr(), out["unmask"].data_ptr(),
         out["xt_out"].data_ptr(), out["n_mask_after"].data_ptr(), out["hit_eos"].data_ptr(),
         stream_ptr(dev)))
+
+
+TOP_MAX = 32  # alternatives of a position that token_logprobs returns at most
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor,
+                   top_logprob: Optional[torch.Tensor] = None, top_token: Optional[torch.Tensor] = None) -> None:
+    """Log probabilities of ``tokens`` under ``logits``, the entropy and the best alternatives
+    (``yapd_token_logprobs``), into caller tensors.
+
+    ``logits`` is bf16 or fp32 ``[n, V]`` or ``[rows, bl, V]`` with a unit last stride (any others);
+    ``tokens`` (int64), ``logprob`` and ``entropy`` (fp32) have its leading shape, ``top_logprob``
+    (fp32) and ``top_token`` (int64) ``[..., k]`` with ``0 <= k <= 32``.  A token below 0 marks a position
+    without one (log probability 0), one past the vocabulary gives NaN."""
+    dev = logits.device
+    if logits.is_cuda and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):  # the launch goes to the current device
+            return token_logprobs(logits, tokens, logprob, entropy, top_logprob, top_token)
+    wide = logits.dtype == torch.float32
+    require_cuda(logits, "logits", torch.float32 if wide else torch.bfloat16, dev, contiguous=False)
+    shape = logits.shape
+    require(len(shape) in (2, 3) and (shape[-1] <= 1 or logits.stride(-1) == 1),
+            "logits must be [n, V] or [rows, bl, V] with unit last stride")
+    lead = shape[:-1]
+    require_cuda(tokens, "tokens", torch.int64, dev)
+    require_cuda(logprob, "logprob", torch.float32, dev)
+    require_cuda(entropy, "entropy", torch.float32, dev)
+    require(tokens.shape == lead and logprob.shape == lead and entropy.shape == lead,
+            "tokens, logprob and entropy must have the logits' leading shape")
+    k = 0
+    if top_logprob is not None or top_token is not None:
+        require(top_logprob is not None and top_token is not None, "top_logprob and top_token come together")
+        require_cuda(top_logprob, "top_logprob", torch.float32, dev)
+        require_cuda(top_token, "top_token", torch.int64, dev)
+        k = top_token.shape[-1]
+        require(top_logprob.shape == top_token.shape and top_token.shape[:-1] == lead,
+                "top_logprob and top_token must be [..., k] on the logits' leading shape")
+    seq, pos, rows, bl = (logits.stride(0), 0, shape[0], 1) if len(lead) == 1 else (*logits.stride()[:2], *lead)
+    check(load_library().yapd_token_logprobs(
+        logits.data_ptr(), wide, seq, pos, rows, bl, shape[-1], tokens.data_ptr(), k, logprob.data_ptr(),
+        entropy.data_ptr(), ptr(top_logprob), ptr(top_token), stream_ptr(dev)))
 
 
 # --------------------------------------------------------------------------- #

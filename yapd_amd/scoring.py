@@ -65,6 +65,33 @@ class ScoreResult:
     hit_eos: torch.Tensor       # [pairs] uint8
 
 
+@dataclass
+class TokenLogprobs:
+    logprob: torch.Tensor                # [...] fp32     ln p(token); 0 where the token is below 0
+    entropy: torch.Tensor                # [...] fp32     in nats
+    top_logprob: Optional[torch.Tensor]  # [..., k] fp32  largest first (None for top_k = 0)
+    top_token: Optional[torch.Tensor]    # [..., k] int64 ties: the lowest index first
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
+    """``ln softmax(logits)`` at ``tokens``, with the entropy and the ``top_k`` (at most 32) best
+    alternatives of every position, in one pass over the logits (``yapd_token_logprobs``).
+
+    ``logits`` is bf16 or fp32, ``[n, V]`` or ``[rows, bl, V]`` with a unit last stride; ``tokens`` int64
+    of its leading shape (below 0: a position without a token, e.g. padding).  Logits of -inf have
+    probability 0.  Summed over its tokens, a candidate's log probability ranks it among others."""
+    lead = tuple(logits.shape[:-1])
+    dev = logits.device
+    logprob, entropy = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
+    top_logprob = top_token = None
+    if top_k:
+        kernels.require(1 <= top_k <= kernels.TOP_MAX, f"top_k must be in [0, {kernels.TOP_MAX}]")
+        top_logprob = torch.empty(*lead, top_k, dtype=torch.float32, device=dev)
+        top_token = torch.empty(*lead, top_k, dtype=torch.int64, device=dev)
+    kernels.token_logprobs(logits, tokens, logprob, entropy, top_logprob, top_token)
+    return TokenLogprobs(logprob, entropy, top_logprob, top_token)
+
+
 class BlockScorer:
     """Persistent buffers + launcher for one block size and batch.
 
