@@ -20,6 +20,7 @@
 #include "attn_tile.h"
 #include "common.h"
 #include "kv_layout.h"
+#include "lds_dma.h"
 
 namespace yapd {
 namespace {
@@ -341,6 +342,205 @@ __global__ __launch_bounds__(64 * KS * HPW) void attn_window_kernel(const Window
   }
 }
 
+// Long runs of queries: a workgroup takes 128 queries of one head, 32 a wave,
+// and brings 64-key chunks through LDS, where the four waves share them; three
+// chunks are in flight, one barrier a chunk.  v_mfma_f32_32x32x16_bf16: S^T = K Q^T
+// (M = keys, N = queries) leaves a lane one query and half of a tile's keys;
+// K rows are permuted so that those are 8 consecutive keys per 16, the operand
+// of O^T += V^T P^T, and 8 consecutive bf16 of a V^T row of a page.
+//
+// LDS: K rows of 128 bytes, 16-byte piece c of key j in slot c ^ (j / 2 & 7); V^T
+// pages of 64 x 32 bytes, the halves swapped where hd & 8: the 16 lanes of a
+// phase of a fragment read fill 16 distinct slots.
+constexpr int kTileQ = 128, kTileChunk = 64, kStages = 3;
+constexpr int kStage = 2 * kTileChunk * kHeadDim * 2;  // bytes
+
+template <int LATER>
+__device__ __forceinline__ void chunk_wait() {  // this wave's loads but the last LATER, and its LDS reads; then everyone's
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
+}
+
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_window_tile_kernel(const WindowParams P) {
+  // dynamic: only the direct loads write it, which the compiler does not see as writes of a static array
+  extern __shared__ __attribute__((aligned(16))) char ring[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int item = static_cast<int>(blockIdx.x) / P.H;
+  const int h = static_cast<int>(blockIdx.x) - item * P.H;
+  const int slot = item / P.parts, part = item - slot * P.parts;
+  Tile t;
+  if (!find_tile<kTileQ>(P, slot, lane, t)) return;  // the whole workgroup
+  const int g = lane >> 5, n = lane & 31;
+  const int H = P.H;
+  const ChunkList cl(P, t, kTileChunk);
+  const int c0 = static_cast<int>(static_cast<int64_t>(cl.n) * part / P.parts);
+  const int c1 = static_cast<int>(static_cast<int64_t>(cl.n) * (part + 1) / P.parts);
+  const int q = wave * 32 + n;  // this lane's query of the tile
+
+  // Q^T fragments (B operand): lane holds Q[q][hd = 16s + 8g .. +7]
+  bf16x8_t qf[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    u32x4_t v = {0u, 0u, 0u, 0u};
+    if (q < t.qc) v = load16(P.q + (t.qs + q) * P.q_stride + h * kHeadDim + s * 16 + 8 * g);
+    qf[s] = as_bf16x8(v);
+  }
+#pragma unroll
+  for (int s = 0; s < 4; ++s) asm volatile("" ::"v"(qf[s]));  // complete before the counted waits begin
+
+  Pages page_of(P, t, cl.chunk(c0) * (kTileChunk / kPageSize), lane);
+  // Wave w brings page w of a chunk: 2 KB of K and 2 KB of V^T, 1 KB an instruction.
+  uint32_t k_ofs[2], v_ofs;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) k_ofs[j] = (lane >> 3) * 128 + 16 * ((lane & 7) ^ ((4 * j + (lane >> 4)) & 7));
+  v_ofs = (lane >> 1) * 32 + 16 * ((lane & 1) ^ (lane >> 4 & 1));
+  const uint32_t k_plane = static_cast<uint32_t>(kv_plane_offset(0, 0, h, H) * 2);
+  const uint32_t v_plane = static_cast<uint32_t>(kv_plane_offset(0, 1, h, H) * 2);
+  auto issue = [&](int c, int st) {
+    const int pi = cl.chunk(c) * (kTileChunk / kPageSize) + wave;
+    const __amdgpu_buffer_rsrc_t rs = buffer_from(P.pool + kv_plane_offset(page_of(pi), 0, 0, H));
+    char* to = ring + st * kStage + wave * 2048;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) load_lds16(rs, k_ofs[j], k_plane + j * 1024, to + j * 1024);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) load_lds16(rs, v_ofs, v_plane + j * 1024, to + kStage / 2 + j * 1024);
+  };
+
+  f32x16_t o[2];
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt) o[mt] = f32x16_t{};
+  float m = -INFINITY, l = 0.f;
+  // row n of an S^T tile: key 16 (n / 16) + 8 (n / 4 & 1) + 4 (n / 8 & 1) + n % 4 of its 32
+  const int key_n = 16 * (n >> 4) + 8 * (n >> 2 & 1) + 4 * (n >> 3 & 1) + (n & 3);
+  const int k_row = key_n * 128, k_sw = key_n >> 1 & 7;
+  const int v_row = n * 32 + 16 * (g ^ (n >> 3 & 1));
+  const int p = t.p0 + q;
+  const int q_hi = P.causal ? min(t.kvl, p + 1) : t.kvl, q_lo = p - P.window + 1;
+  // of this wave's queries: what all see, what any sees
+  const int w_first = t.p0 + wave * 32, w_last = t.p0 + min(wave * 32 + 31, t.qc - 1);
+  const bool w_any = wave * 32 < t.qc;
+  const int all_hi = P.causal ? min(t.kvl, w_first + 1) : t.kvl, all_lo = w_last - P.window + 1;
+  const int any_hi = P.causal ? min(t.kvl, w_last + 1) : t.kvl, any_lo = w_first - P.window + 1;
+
+  if (c0 < c1) issue(c0, 0);
+  if (c0 + 1 < c1) issue(c0 + 1, 1);
+  int st = 0;
+  for (int c = c0; c < c1; ++c) {
+    // chunk c has landed, and every wave has read chunk c - 1: its stage takes chunk c + 2
+    if (c + 1 < c1)
+      chunk_wait<4>();
+    else
+      chunk_wait<0>();
+    if (c + 2 < c1) issue(c + 2, st == 0 ? 2 : st - 1);
+    const char* kb = ring + st * kStage;
+    const char* vb = kb + kStage / 2;
+    st = st == 2 ? 0 : st + 1;
+    const int k0 = cl.chunk(c) * kTileChunk;
+    if (!w_any || k0 >= any_hi || (k0 + kTileChunk <= any_lo && k0 >= P.sinks)) continue;  // no query of this wave sees it
+    f32x16_t s[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s[i] = f32x16_t{};
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+        s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            as_bf16x8(*reinterpret_cast<const u32x4_t*>(kb + i * 4096 + k_row + 16 * ((2 * ks + g) ^ k_sw))), qf[ks], s[i],
+            0, 0, 0);
+    }
+    // s[i][e] = S[q][key 32i + 16 (e / 8) + 8g + e % 8]
+    const bool mask = k0 + kTileChunk > all_hi || (k0 < all_lo && k0 + kTileChunk > P.sinks);
+    if (mask) {  // uniform
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = k0 + 32 * i + 16 * (e >> 3) + 8 * g + (e & 7);
+          s[i][e] = key < q_hi && (key >= q_lo || key < P.sinks) ? s[i][e] : -INFINITY;
+        }
+      }
+    }
+    float cm = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int e = 1; e < 16; ++e) cm = fmaxf(cm, fmaxf(s[0][e], s[1][e]));
+    const float2 both = swap32(cm);
+    const float mn = fmaxf(m, fmaxf(both.x, both.y));
+    // no key seen yet: exponents against 0 give alpha = 0 and p = 0 instead of NaN
+    const float mref = mn == -INFINITY ? 0.f : mn * P.scale_log2;
+    const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, P.scale_log2, -mref));
+    float ps = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], P.scale_log2, -mref));
+        ps += s[i][e];
+      }
+    }
+    l = l * alpha + ps;
+    m = mn;
+    o[0] *= alpha;
+    o[1] *= alpha;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {  // 16 keys: a page
+      u32x4_t pw;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) pw[w] = pack_bf16x2(s[kk >> 1][8 * (kk & 1) + 2 * w], s[kk >> 1][8 * (kk & 1) + 2 * w + 1]);
+      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+      if (mask) {
+        // V of keys that no query of the tile sees: cleared, so 0 * V is never NaN
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int key = k0 + 16 * kk + 8 * g + 2 * w;
+          const bool see0 = key < cl.hi && (key >= cl.lo || key < P.sinks);
+          const bool see1 = key + 1 < cl.hi && (key + 1 >= cl.lo || key + 1 < P.sinks);
+          keep[w] = (see0 ? 0x0000ffffu : 0u) | (see1 ? 0xffff0000u : 0u);
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        u32x4_t vf = *reinterpret_cast<const u32x4_t*>(vb + kk * 2048 + mt * 1024 + v_row);
+        if (mask) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) vf[w] &= keep[w];
+        }
+        o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(vf), as_bf16x8(pw), o[mt], 0, 0, 0);
+      }
+    }
+  }
+  const float2 lb = swap32(l);
+  const float L = lb.x + lb.y;
+  if (q >= t.qc) return;
+  // o[mt][e] = O^T[hd = 32mt + 8 (e / 4) + 4g + e % 4][q]
+  const int64_t token = t.qs + q, at = (token * H + h) * kHeadDim + 4 * g;
+  if (P.parts == 1) {
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // no key seen: zeros, not NaN
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        u32x2_t w2;
+        w2[0] = pack_bf16x2(o[mt][4 * b] * inv, o[mt][4 * b + 1] * inv);
+        w2[1] = pack_bf16x2(o[mt][4 * b + 2] * inv, o[mt][4 * b + 3] * inv);
+        *reinterpret_cast<u32x2_t*>(P.out + at + 32 * mt + 8 * b) = w2;
+      }
+    }
+  } else {
+    float* po = P.part_o + static_cast<int64_t>(part) * P.n_q * H * kHeadDim + at;
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        *reinterpret_cast<f32x4_t*>(po + 32 * mt + 8 * b) =
+            f32x4_t{o[mt][4 * b], o[mt][4 * b + 1], o[mt][4 * b + 2], o[mt][4 * b + 3]};
+    }
+    if (g == 0) {
+      float* ml = P.part_ml + (static_cast<int64_t>(part) * P.n_q * H + token * H + h) * 2;
+      ml[0] = m * P.scale_log2;  // as the other form has it
+      ml[1] = L;
+    }
+  }
+}
+
 // Joins the parts of every query: thread (query, head, 4 head-dim values).
 __global__ __launch_bounds__(256) void attn_window_join_kernel(const WindowParams P) {
   const int lane = threadIdx.x & 63;
@@ -375,9 +575,10 @@ __global__ __launch_bounds__(256) void attn_window_join_kernel(const WindowParam
   *reinterpret_cast<u32x2_t*>(P.out + at * kHeadDim + (lane & 15) * 4) = w2;
 }
 
-// How a call is cut: 16 * nqt queries a tile, ks waves to a part's chunks, parts.
+// How a call is cut: tq queries a tile (16, 32, 48, 64, or kTileQ: the tile
+// kernel), ks waves to a part's chunks, parts.
 struct Cut {
-  int nqt, ks, parts;
+  int tq, ks, parts;
   int64_t slots;
 };
 
@@ -385,12 +586,19 @@ constexpr int64_t kWavesWanted = 2048;  // two a SIMD
 
 Cut cut_of(int rows, int max_q, int n_q, bool packed, int n_heads, int window, int sinks, int max_kv) {
   Cut c;
-  c.nqt = std::min((max_q + 15) / 16, 4);
-  const int tq = 16 * c.nqt;
+  c.tq = max_q <= 64 ? (max_q + 15) / 16 * 16 : kTileQ;
+  const int tq = c.tq;
   c.slots = packed ? n_q / tq + static_cast<int64_t>(rows) : static_cast<int64_t>(rows) * ((max_q + tq - 1) / tq);
   const int64_t tiles = std::min<int64_t>(c.slots, (n_q + tq - 1) / tq + rows);
   const int64_t keys = std::min<int64_t>(max_kv, static_cast<int64_t>(window) + sinks + tq);
   const int64_t chunks = (keys + kChunk - 1) / kChunk + 1;
+  if (tq == kTileQ) {
+    // parts of at least 16 chunks of 64 keys while there are fewer workgroups than CUs
+    c.ks = 1;
+    const int64_t want = (256 + tiles * n_heads - 1) / (tiles * n_heads);
+    c.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, chunks / 32)));
+    return c;
+  }
   const int64_t waves = tiles * n_heads;
   c.ks = waves * 4 <= kWavesWanted && chunks >= 8 ? 8 : waves <= kWavesWanted && chunks >= 4 ? 4 : 1;
   // more parts only where eight waves are not enough, each with eight chunks a wave
@@ -478,11 +686,14 @@ extern "C" int yapd_attn_window(const void* q, int64_t q_tok_stride, const void*
   P.scale_log2 = scale * 1.4426950408889634f;
   P.out = static_cast<uint16_t*>(out);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  switch (c.nqt) {
-    case 1: yapd::launch_tiles<1>(P, c, st); break;
-    case 2: yapd::launch_tiles<2>(P, c, st); break;
-    case 3: yapd::launch_tiles<3>(P, c, st); break;
-    default: yapd::launch_tiles<4>(P, c, st); break;
+  switch (c.tq) {
+    case 16: yapd::launch_tiles<1>(P, c, st); break;
+    case 32: yapd::launch_tiles<2>(P, c, st); break;
+    case 48: yapd::launch_tiles<3>(P, c, st); break;
+    case 64: yapd::launch_tiles<4>(P, c, st); break;
+    default:
+      hipLaunchKernelGGL(yapd::attn_window_tile_kernel, dim3(static_cast<unsigned>(c.slots * P.parts * P.H)), dim3(256),
+                         yapd::kStages * yapd::kStage, st, P);
   }
   YAPD_LAUNCH_CHECK("attn_window_kernel launch");
   if (c.parts > 1) {
