@@ -353,14 +353,10 @@ __global__ __launch_bounds__(64 * KS * HPW) void attn_window_kernel(const Window
 // pages of 64 x 32 bytes, the halves swapped where hd & 8: the 16 lanes of a
 // phase of a fragment read fill 16 distinct slots.
 constexpr int kTileQ = 128, kTileChunk = 64, kStages = 3;
+constexpr float kSlack = 8.f;
 constexpr int kStage = 2 * kTileChunk * kHeadDim * 2;  // bytes
 
-template <int LATER>
-__device__ __forceinline__ void chunk_wait() {  // this wave's loads but the last LATER, and its LDS reads; then everyone's
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
-}
-
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_window_tile_kernel(const WindowParams P) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void attn_window_tile_kernel(const WindowParams P) {
   // dynamic: only the direct loads write it, which the compiler does not see as writes of a static array
   extern __shared__ __attribute__((aligned(16))) char ring[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -409,7 +405,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   f32x16_t o[2];
 #pragma unroll
   for (int mt = 0; mt < 2; ++mt) o[mt] = f32x16_t{};
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, mref = 0.f, l = 0.f;
+  const float slack = kSlack / P.scale_log2;
+  const bf16x2_t one2 = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
+  float inf = INFINITY;
+  asm("" : "+s"(inf));  // opaque: the compiler turns v_med3 with a known +inf back into v_max
   // row n of an S^T tile: key 16 (n / 16) + 8 (n / 4 & 1) + 4 (n / 8 & 1) + n % 4 of its 32
   const int key_n = 16 * (n >> 4) + 8 * (n >> 2 & 1) + 4 * (n >> 3 & 1) + (n & 3);
   const int k_row = key_n * 128, k_sw = key_n >> 1 & 7;
@@ -426,16 +426,34 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   if (c0 + 1 < c1) issue(c0 + 1, 1);
   int st = 0;
   for (int c = c0; c < c1; ++c) {
-    // chunk c has landed, and every wave has read chunk c - 1: its stage takes chunk c + 2
-    if (c + 1 < c1)
-      chunk_wait<4>();
-    else
-      chunk_wait<0>();
-    if (c + 2 < c1) issue(c + 2, st == 0 ? 2 : st - 1);
-    const char* kb = ring + st * kStage;
-    const char* vb = kb + kStage / 2;
-    st = st == 2 ? 0 : st + 1;
     const int k0 = cl.chunk(c) * kTileChunk;
+    char* const kb = ring + st * kStage;
+    char* const vb = kb + kStage / 2;
+    // this wave's page of chunk c has landed
+    if (c + 1 < c1)
+      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (k0 + kTileChunk > cl.hi || (k0 < cl.lo && k0 + kTileChunk > P.sinks)) {
+      // V of keys that no query of the tile sees is cleared, so 0 * V is never NaN: lane = head dim of the wave's page
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        u32x4_t* v = reinterpret_cast<u32x4_t*>(vb + wave * 2048 + lane * 32 + 16 * (half ^ (lane >> 3 & 1)));
+        u32x4_t x = *v;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int key = k0 + 16 * wave + 8 * half + 2 * w;
+          const bool see0 = key < cl.hi && (key >= cl.lo || key < P.sinks);
+          const bool see1 = key + 1 < cl.hi && (key + 1 >= cl.lo || key + 1 < P.sinks);
+          x[w] &= (see0 ? 0x0000ffffu : 0u) | (see1 ? 0xffff0000u : 0u);
+        }
+        *v = x;
+      }
+    }
+    // and everyone's, and every wave has read chunk c - 1: its stage takes chunk c + 2
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (c + 2 < c1) issue(c + 2, st == 0 ? 2 : st - 1);
+    st = st == 2 ? 0 : st + 1;
     if (!w_any || k0 >= any_hi || (k0 + kTileChunk <= any_lo && k0 >= P.sinks)) continue;  // no query of this wave sees it
     f32x16_t s[2];
 #pragma unroll
@@ -448,8 +466,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
             0, 0, 0);
     }
     // s[i][e] = S[q][key 32i + 16 (e / 8) + 8g + e % 8]
-    const bool mask = k0 + kTileChunk > all_hi || (k0 < all_lo && k0 + kTileChunk > P.sinks);
-    if (mask) {  // uniform
+    if (k0 + kTileChunk > all_hi || (k0 < all_lo && k0 + kTileChunk > P.sinks)) {  // uniform
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -459,52 +476,48 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
         }
       }
     }
-    float cm = fmaxf(s[0][0], s[1][0]);
+    // v_med3 with +inf is a maximum that does not quiet its operands first, as v_max would have to
+    float cm[8];
 #pragma unroll
-    for (int e = 1; e < 16; ++e) cm = fmaxf(cm, fmaxf(s[0][e], s[1][e]));
-    const float2 both = swap32(cm);
-    const float mn = fmaxf(m, fmaxf(both.x, both.y));
-    // no key seen yet: exponents against 0 give alpha = 0 and p = 0 instead of NaN
-    const float mref = mn == -INFINITY ? 0.f : mn * P.scale_log2;
-    const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, P.scale_log2, -mref));
-    float ps = 0.f;
+    for (int e = 0; e < 8; ++e)
+      cm[e] = fmaxf(__builtin_amdgcn_fmed3f(s[0][e], s[0][e + 8], inf), __builtin_amdgcn_fmed3f(s[1][e], s[1][e + 8], inf));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int e = 1; e < 8; ++e) cm[0] = fmaxf(cm[0], cm[e]);
+    const float2 both = swap32(cm[0]);
+    const float mn = fmaxf(both.x, both.y);
+    // The exponents are taken against m, which follows the maximum only when one of
+    // the wave's queries has left it by more than 2^kSlack: weights up to that are as exact.
+    if (__builtin_expect(__any(mn > m + slack), 0)) {
+      const float to = fmaxf(m, mn);
+      // no key seen yet: exponents against 0 give alpha = 0 and p = 0 instead of NaN
+      mref = to == -INFINITY ? 0.f : to * P.scale_log2;
+      const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, P.scale_log2, -mref));
+      m = to;
+      l *= alpha;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], P.scale_log2, -mref));
-        ps += s[i][e];
+        o[0][e] *= alpha;
+        o[1][e] *= alpha;
       }
+      // keeps the accumulators in their registers: without it every chunk pays 32 copies
+      asm volatile("" : "+v"(o[0]), "+v"(o[1]));
     }
-    l = l * alpha + ps;
-    m = mn;
-    o[0] *= alpha;
-    o[1] *= alpha;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {  // 16 keys: a page
       u32x4_t pw;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) pw[w] = pack_bf16x2(s[kk >> 1][8 * (kk & 1) + 2 * w], s[kk >> 1][8 * (kk & 1) + 2 * w + 1]);
-      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-      if (mask) {
-        // V of keys that no query of the tile sees: cleared, so 0 * V is never NaN
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int key = k0 + 16 * kk + 8 * g + 2 * w;
-          const bool see0 = key < cl.hi && (key >= cl.lo || key < P.sinks);
-          const bool see1 = key + 1 < cl.hi && (key + 1 >= cl.lo || key + 1 < P.sinks);
-          keep[w] = (see0 ? 0x0000ffffu : 0u) | (see1 ? 0xffff0000u : 0u);
-        }
+      for (int w = 0; w < 4; ++w) {
+        const int e = 8 * (kk & 1) + 2 * w;
+        const uint32_t two = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[kk >> 1][e], P.scale_log2, -mref)),
+                                         __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk >> 1][e + 1], P.scale_log2, -mref)));
+        pw[w] = two;
+        // the sum of the weights as the product with V has them
+        l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two), one2, l, false);
       }
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        u32x4_t vf = *reinterpret_cast<const u32x4_t*>(vb + kk * 2048 + mt * 1024 + v_row);
-        if (mask) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) vf[w] &= keep[w];
-        }
-        o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(vf), as_bf16x8(pw), o[mt], 0, 0, 0);
-      }
+      for (int mt = 0; mt < 2; ++mt)
+        o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            as_bf16x8(*reinterpret_cast<const u32x4_t*>(vb + kk * 2048 + mt * 1024 + v_row)), as_bf16x8(pw), o[mt], 0, 0, 0);
     }
   }
   const float2 lb = swap32(l);
