@@ -424,84 +424,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
 
   if (c0 < c1) issue(c0, 0);
   if (c0 + 1 < c1) issue(c0 + 1, 1);
-  int st = 0;
-  for (int c = c0; c < c1; ++c) {
-    const int k0 = cl.chunk(c) * kTileChunk;
-    char* const kb = ring + st * kStage;
-    char* const vb = kb + kStage / 2;
-    // this wave's page of chunk c has landed
-    if (c + 1 < c1)
-      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (k0 + kTileChunk > cl.hi || (k0 < cl.lo && k0 + kTileChunk > P.sinks)) {
-      // V of keys that no query of the tile sees is cleared, so 0 * V is never NaN: lane = head dim of the wave's page
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        u32x4_t* v = reinterpret_cast<u32x4_t*>(vb + wave * 2048 + lane * 32 + 16 * (half ^ (lane >> 3 & 1)));
-        u32x4_t x = *v;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int key = k0 + 16 * wave + 8 * half + 2 * w;
-          const bool see0 = key < cl.hi && (key >= cl.lo || key < P.sinks);
-          const bool see1 = key + 1 < cl.hi && (key + 1 >= cl.lo || key + 1 < P.sinks);
-          x[w] &= (see0 ? 0x0000ffffu : 0u) | (see1 ? 0xffff0000u : 0u);
-        }
-        *v = x;
-      }
-    }
-    // and everyone's, and every wave has read chunk c - 1: its stage takes chunk c + 2
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (c + 2 < c1) issue(c + 2, st == 0 ? 2 : st - 1);
-    st = st == 2 ? 0 : st + 1;
-    if (!w_any || k0 >= any_hi || (k0 + kTileChunk <= any_lo && k0 >= P.sinks)) continue;  // no query of this wave sees it
-    f32x16_t s[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      s[i] = f32x16_t{};
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-        s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            as_bf16x8(*reinterpret_cast<const u32x4_t*>(kb + i * 4096 + k_row + 16 * ((2 * ks + g) ^ k_sw))), qf[ks], s[i],
-            0, 0, 0);
-    }
-    // s[i][e] = S[q][key 32i + 16 (e / 8) + 8g + e % 8]
-    if (k0 + kTileChunk > all_hi || (k0 < all_lo && k0 + kTileChunk > P.sinks)) {  // uniform
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int key = k0 + 32 * i + 16 * (e >> 3) + 8 * g + (e & 7);
-          s[i][e] = key < q_hi && (key >= q_lo || key < P.sinks) ? s[i][e] : -INFINITY;
-        }
-      }
-    }
-    // v_med3 with +inf is a maximum that does not quiet its operands first, as v_max would have to
-    float cm[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      cm[e] = fmaxf(__builtin_amdgcn_fmed3f(s[0][e], s[0][e + 8], inf), __builtin_amdgcn_fmed3f(s[1][e], s[1][e + 8], inf));
-#pragma unroll
-    for (int e = 1; e < 8; ++e) cm[0] = fmaxf(cm[0], cm[e]);
-    const float2 both = swap32(cm[0]);
-    const float mn = fmaxf(both.x, both.y);
-    // The exponents are taken against m, which follows the maximum only when one of
-    // the wave's queries has left it by more than 2^kSlack: weights up to that are as exact.
-    if (__builtin_expect(__any(mn > m + slack), 0)) {
-      const float to = fmaxf(m, mn);
-      // no key seen yet: exponents against 0 give alpha = 0 and p = 0 instead of NaN
-      mref = to == -INFINITY ? 0.f : to * P.scale_log2;
-      const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, P.scale_log2, -mref));
-      m = to;
-      l *= alpha;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        o[0][e] *= alpha;
-        o[1][e] *= alpha;
-      }
-      // keeps the accumulators in their registers: without it every chunk pays 32 copies
-      asm volatile("" : "+v"(o[0]), "+v"(o[1]));
-    }
+  f32x16_t s[2];
+  // O^T += V^T P^T and the sum of the weights, for the scores in s and the V^T pages at vb
+  auto add_chunk = [&](const char* vb) {
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {  // 16 keys: a page
       u32x4_t pw;
@@ -519,6 +444,89 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
         o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
             as_bf16x8(*reinterpret_cast<const u32x4_t*>(vb + kk * 2048 + mt * 1024 + v_row)), as_bf16x8(pw), o[mt], 0, 0, 0);
     }
+  };
+  int st = 0;
+  for (int c = c0;; ++c) {
+    // The exponents are taken against m, which follows the maximum only when one of
+    // the wave's queries has left it by more than 2^kSlack: weights up to that are as
+    // exact.  The inner loop runs while none has, and keeps the accumulators in place
+    // (with the rescaling as a branch inside it, every chunk paid 80 register copies).
+    float mn = -INFINITY;
+    char* vb = ring;
+    bool moved = false;
+    for (; c < c1; ++c) {
+      const int k0 = cl.chunk(c) * kTileChunk;
+      char* const kb = ring + st * kStage;
+      vb = kb + kStage / 2;
+      // this wave's page of chunk c has landed
+      if (c + 1 < c1)
+        asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (k0 + kTileChunk > cl.hi || (k0 < cl.lo && k0 + kTileChunk > P.sinks)) {
+        // V of keys that no query of the tile sees is cleared, so 0 * V is never NaN: lane = head dim of the wave's page
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          u32x4_t* v = reinterpret_cast<u32x4_t*>(vb + wave * 2048 + lane * 32 + 16 * (half ^ (lane >> 3 & 1)));
+          u32x4_t x = *v;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int key = k0 + 16 * wave + 8 * half + 2 * w;
+            const bool see0 = key < cl.hi && (key >= cl.lo || key < P.sinks);
+            const bool see1 = key + 1 < cl.hi && (key + 1 >= cl.lo || key + 1 < P.sinks);
+            x[w] &= (see0 ? 0x0000ffffu : 0u) | (see1 ? 0xffff0000u : 0u);
+          }
+          *v = x;
+        }
+      }
+      // and everyone's, and every wave has read chunk c - 1: its stage takes chunk c + 2
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (c + 2 < c1) issue(c + 2, st == 0 ? 2 : st - 1);
+      st = st == 2 ? 0 : st + 1;
+      if (!w_any || k0 >= any_hi || (k0 + kTileChunk <= any_lo && k0 >= P.sinks)) continue;  // no query of the wave sees it
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s[i] = f32x16_t{};
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+          s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              as_bf16x8(*reinterpret_cast<const u32x4_t*>(kb + i * 4096 + k_row + 16 * ((2 * ks + g) ^ k_sw))), qf[ks],
+              s[i], 0, 0, 0);
+      }
+      // s[i][e] = S[q][key 32i + 16 (e / 8) + 8g + e % 8]
+      if (k0 + kTileChunk > all_hi || (k0 < all_lo && k0 + kTileChunk > P.sinks)) {  // uniform
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int key = k0 + 32 * i + 16 * (e >> 3) + 8 * g + (e & 7);
+            s[i][e] = key < q_hi && (key >= q_lo || key < P.sinks) ? s[i][e] : -INFINITY;
+          }
+        }
+      }
+      // v_med3 with +inf is a maximum that does not quiet its operands first, as v_max would have to
+      float cm[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        cm[e] = fmaxf(__builtin_amdgcn_fmed3f(s[0][e], s[0][e + 8], inf), __builtin_amdgcn_fmed3f(s[1][e], s[1][e + 8], inf));
+#pragma unroll
+      for (int e = 1; e < 8; ++e) cm[0] = fmaxf(cm[0], cm[e]);
+      const float2 both = swap32(cm[0]);
+      mn = fmaxf(both.x, both.y);
+      moved = __any(mn > m + slack);
+      if (moved) break;
+      add_chunk(vb);
+    }
+    if (!moved) break;  // the last chunk is done
+    mn = fmaxf(m, mn);
+    // no key seen yet: exponents against 0 give alpha = 0 and p = 0 instead of NaN
+    mref = mn == -INFINITY ? 0.f : mn * P.scale_log2;
+    const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, P.scale_log2, -mref));
+    m = mn;
+    l *= alpha;
+    o[0] *= alpha;
+    o[1] *= alpha;
+    add_chunk(vb);
   }
   const float2 lb = swap32(l);
   const float L = lb.x + lb.y;
