@@ -425,8 +425,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
   if (c0 < c1) issue(c0, 0);
   if (c0 + 1 < c1) issue(c0 + 1, 1);
   f32x16_t s[2];
-  // O^T += V^T P^T and the sum of the weights, for the scores in s and the V^T pages at vb
-  auto add_chunk = [&](const char* vb) {
+  u32x4_t vf[4][2];
+  // O^T += V^T P^T and the sum of the weights, for the scores in s and the V^T fragments in vf
+  auto add_chunk = [&] {
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {  // 16 keys: a page
       u32x4_t pw;
@@ -441,8 +442,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
       }
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
-        o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            as_bf16x8(*reinterpret_cast<const u32x4_t*>(vb + kk * 2048 + mt * 1024 + v_row)), as_bf16x8(pw), o[mt], 0, 0, 0);
+        o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(vf[kk][mt]), as_bf16x8(pw), o[mt], 0, 0, 0);
     }
   };
   int st = 0;
@@ -452,12 +452,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
     // exact.  The inner loop runs while none has, and keeps the accumulators in place
     // (with the rescaling as a branch inside it, every chunk paid 80 register copies).
     float mn = -INFINITY;
-    char* vb = ring;
     bool moved = false;
     for (; c < c1; ++c) {
       const int k0 = cl.chunk(c) * kTileChunk;
       char* const kb = ring + st * kStage;
-      vb = kb + kStage / 2;
+      char* const vb = kb + kStage / 2;
       // this wave's page of chunk c has landed
       if (c + 1 < c1)
         asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
@@ -484,15 +483,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
       if (c + 2 < c1) issue(c + 2, st == 0 ? 2 : st - 1);
       st = st == 2 ? 0 : st + 1;
       if (!w_any || k0 >= any_hi || (k0 + kTileChunk <= any_lo && k0 >= P.sinks)) continue;  // no query of the wave sees it
+      // all of a chunk's fragments are requested before the first is used
+      u32x4_t kf[4][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        s[i] = f32x16_t{};
+      for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-          s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              as_bf16x8(*reinterpret_cast<const u32x4_t*>(kb + i * 4096 + k_row + 16 * ((2 * ks + g) ^ k_sw))), qf[ks],
-              s[i], 0, 0, 0);
-      }
+        for (int i = 0; i < 2; ++i)
+          kf[ks][i] = *reinterpret_cast<const u32x4_t*>(kb + i * 4096 + k_row + 16 * ((2 * ks + g) ^ k_sw));
+      __builtin_amdgcn_sched_barrier(0);
+      s[0] = f32x16_t{};
+      s[1] = f32x16_t{};
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(kf[ks][i]), qf[ks], s[i], 0, 0, 0);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+          vf[kk][mt] = *reinterpret_cast<const u32x4_t*>(vb + kk * 2048 + mt * 1024 + v_row);
+      __builtin_amdgcn_sched_barrier(0);
       // s[i][e] = S[q][key 32i + 16 (e / 8) + 8g + e % 8]
       if (k0 + kTileChunk > all_hi || (k0 < all_lo && k0 + kTileChunk > P.sinks)) {  // uniform
 #pragma unroll
@@ -515,7 +526,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
       mn = fmaxf(both.x, both.y);
       moved = __any(mn > m + slack);
       if (moved) break;
-      add_chunk(vb);
+      add_chunk();
     }
     if (!moved) break;  // the last chunk is done
     mn = fmaxf(m, mn);
@@ -526,7 +537,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
     l *= alpha;
     o[0] *= alpha;
     o[1] *= alpha;
-    add_chunk(vb);
+    add_chunk();
   }
   const float2 lb = swap32(l);
   const float L = lb.x + lb.y;
