@@ -352,11 +352,11 @@ __global__ __launch_bounds__(64 * KS * HPW) void attn_window_kernel(const Window
 // LDS: K rows of 128 bytes, 16-byte piece c of key j in slot c ^ (j / 2 & 7); V^T
 // pages of 64 x 32 bytes, the halves swapped where hd & 8: the 16 lanes of a
 // phase of a fragment read fill 16 distinct slots.
-constexpr int kTileQ = 128, kTileChunk = 64, kStages = 3;
+constexpr int kTileQ = 128, kTileChunk = 64, kStages = 2;
 constexpr float kSlack = 8.f;
 constexpr int kStage = 2 * kTileChunk * kHeadDim * 2;  // bytes
 
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void attn_window_tile_kernel(const WindowParams P) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void attn_window_tile_kernel(const WindowParams P) {
   // dynamic: only the direct loads write it, which the compiler does not see as writes of a static array
   extern __shared__ __attribute__((aligned(16))) char ring[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -372,17 +372,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
   const int c0 = static_cast<int>(static_cast<int64_t>(cl.n) * part / P.parts);
   const int c1 = static_cast<int>(static_cast<int64_t>(cl.n) * (part + 1) / P.parts);
   const int q = wave * 32 + n;  // this lane's query of the tile
-
-  // Q^T fragments (B operand): lane holds Q[q][hd = 16s + 8g .. +7]
-  bf16x8_t qf[4];
-#pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    u32x4_t v = {0u, 0u, 0u, 0u};
-    if (q < t.qc) v = load16(P.q + (t.qs + q) * P.q_stride + h * kHeadDim + s * 16 + 8 * g);
-    qf[s] = as_bf16x8(v);
-  }
-#pragma unroll
-  for (int s = 0; s < 4; ++s) asm volatile("" ::"v"(qf[s]));  // complete before the counted waits begin
 
   Pages page_of(P, t, cl.chunk(c0) * (kTileChunk / kPageSize), lane);
   // Wave w brings page w of a chunk: 2 KB of K and 2 KB of V^T, 1 KB an instruction.
@@ -401,6 +390,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
 #pragma unroll
     for (int j = 0; j < 2; ++j) load_lds16(rs, v_ofs, v_plane + j * 1024, to + kStage / 2 + j * 1024);
   };
+
+  if (c0 < c1) issue(c0, 0);
+
+  // Q^T fragments (B operand): lane holds Q[q][hd = 16s + 8g .. +7]
+  bf16x8_t qf[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    u32x4_t v = {0u, 0u, 0u, 0u};
+    if (q < t.qc) v = load16(P.q + (t.qs + q) * P.q_stride + h * kHeadDim + s * 16 + 8 * g);
+    qf[s] = as_bf16x8(v);
+  }
+#pragma unroll
+  for (int s = 0; s < 4; ++s) asm volatile("" ::"v"(qf[s]));  // complete before the loop, whose waits are its own
 
   f32x16_t o[2];
 #pragma unroll
@@ -421,13 +423,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
   const bool w_any = wave * 32 < t.qc;
   const int all_hi = P.causal ? min(t.kvl, w_first + 1) : t.kvl, all_lo = w_last - P.window + 1;
   const int any_hi = P.causal ? min(t.kvl, w_last + 1) : t.kvl, any_lo = w_first - P.window + 1;
+  // list entries whose keys are all seen by all of this wave's queries: nothing to skip, mask or clear
+  const int clean_lo = max(cl.skip > 0 ? cl.n_sink : 0, (max(all_lo, 0) + kTileChunk - 1) / kTileChunk - cl.skip);
+  const int clean_hi = w_any ? max(all_hi, 0) / kTileChunk - cl.skip : 0;
 
-  if (c0 < c1) issue(c0, 0);
-  if (c0 + 1 < c1) issue(c0 + 1, 1);
   f32x16_t s[2];
-  u32x4_t vf[4][2];
+  u32x4_t vf[2][2];
   // O^T += V^T P^T and the sum of the weights, for the scores in s and the V^T fragments in vf
-  auto add_chunk = [&] {
+  auto add_chunk = [&](const char* vb) {
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {  // 16 keys: a page
       u32x4_t pw;
@@ -437,12 +440,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
         const uint32_t two = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[kk >> 1][e], P.scale_log2, -mref)),
                                          __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk >> 1][e + 1], P.scale_log2, -mref)));
         pw[w] = two;
+
         // the sum of the weights as the product with V has them
         l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two), one2, l, false);
       }
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-        o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(vf[kk][mt]), as_bf16x8(pw), o[mt], 0, 0, 0);
+      for (int mt = 0; mt < 2; ++mt) {
+        o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(vf[kk & 1][mt]), as_bf16x8(pw), o[mt], 0, 0, 0);
+        if (kk < 2) vf[kk & 1][mt] = *reinterpret_cast<const u32x4_t*>(vb + (kk + 2) * 2048 + mt * 1024 + v_row);
+      }
     }
   };
   int st = 0;
@@ -452,17 +458,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
     // exact.  The inner loop runs while none has, and keeps the accumulators in place
     // (with the rescaling as a branch inside it, every chunk paid 80 register copies).
     float mn = -INFINITY;
+    char* vb = ring;
     bool moved = false;
     for (; c < c1; ++c) {
+      const bool edge = c < clean_lo || c >= clean_hi;
       const int k0 = cl.chunk(c) * kTileChunk;
       char* const kb = ring + st * kStage;
-      char* const vb = kb + kStage / 2;
+      vb = kb + kStage / 2;
       // this wave's page of chunk c has landed
-      if (c + 1 < c1)
-        asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-      else
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (k0 + kTileChunk > cl.hi || (k0 < cl.lo && k0 + kTileChunk > P.sinks)) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (edge && (k0 + kTileChunk > cl.hi || (k0 < cl.lo && k0 + kTileChunk > P.sinks))) {
         // V of keys that no query of the tile sees is cleared, so 0 * V is never NaN: lane = head dim of the wave's page
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -478,11 +483,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
           *v = x;
         }
       }
-      // and everyone's, and every wave has read chunk c - 1: its stage takes chunk c + 2
+      // and everyone's, and every wave has read chunk c - 1: its stage takes chunk c + 1
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (c + 2 < c1) issue(c + 2, st == 0 ? 2 : st - 1);
-      st = st == 2 ? 0 : st + 1;
-      if (!w_any || k0 >= any_hi || (k0 + kTileChunk <= any_lo && k0 >= P.sinks)) continue;  // no query of the wave sees it
+      st ^= 1;
+      if (c + 1 < c1) issue(c + 1, st);
+      if (edge && (!w_any || k0 >= any_hi || (k0 + kTileChunk <= any_lo && k0 >= P.sinks))) continue;  // no query of the wave sees it
       // all of a chunk's fragments are requested before the first is used
       u32x4_t kf[4][2];
 #pragma unroll
@@ -499,13 +504,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
         for (int i = 0; i < 2; ++i)
           s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(kf[ks][i]), qf[ks], s[i], 0, 0, 0);
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
+      for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
           vf[kk][mt] = *reinterpret_cast<const u32x4_t*>(vb + kk * 2048 + mt * 1024 + v_row);
       __builtin_amdgcn_sched_barrier(0);
       // s[i][e] = S[q][key 32i + 16 (e / 8) + 8g + e % 8]
-      if (k0 + kTileChunk > all_hi || (k0 < all_lo && k0 + kTileChunk > P.sinks)) {  // uniform
+      if (edge) {  // uniform
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -526,7 +531,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
       mn = fmaxf(both.x, both.y);
       moved = __any(mn > m + slack);
       if (moved) break;
-      add_chunk();
+      add_chunk(vb);
     }
     if (!moved) break;  // the last chunk is done
     mn = fmaxf(m, mn);
@@ -537,7 +542,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void a
     l *= alpha;
     o[0] *= alpha;
     o[1] *= alpha;
-    add_chunk();
+    add_chunk(vb);
   }
   const float2 lb = swap32(l);
   const float L = lb.x + lb.y;
