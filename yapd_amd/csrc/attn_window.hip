@@ -510,14 +510,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void a
           vf[kk][mt] = *reinterpret_cast<const u32x4_t*>(vb + kk * 2048 + mt * 1024 + v_row);
       __builtin_amdgcn_sched_barrier(0);
       // s[i][e] = S[q][key 32i + 16 (e / 8) + 8g + e % 8]
-      if (edge) {  // uniform
+      if (edge) {  // uniform, as are the two below; element (i, e) of s is key kg + 32i + 16 (e / 8) + e % 8
+        const int kg = k0 + 8 * g;
+        if (k0 + kTileChunk > all_hi) {
+          const int end = q_hi - kg;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = k0 + 32 * i + 16 * (e >> 3) + 8 * g + (e & 7);
-            s[i][e] = key < q_hi && (key >= q_lo || key < P.sinks) ? s[i][e] : -INFINITY;
-          }
+            for (int e = 0; e < 16; ++e) s[i][e] = 32 * i + 16 * (e >> 3) + (e & 7) < end ? s[i][e] : -INFINITY;
+        }
+        if (k0 < all_lo && k0 + kTileChunk > P.sinks) {
+          const int begin = q_lo - kg, sink_end = P.sinks - kg;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int j = 32 * i + 16 * (e >> 3) + (e & 7);
+              s[i][e] = j >= begin || j < sink_end ? s[i][e] : -INFINITY;
+            }
         }
       }
       // v_med3 with +inf is a maximum that does not quiet its operands first, as v_max would have to
@@ -531,7 +541,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void a
       mn = fmaxf(both.x, both.y);
       moved = __any(mn > m + slack);
       if (moved) break;
+      __builtin_amdgcn_s_setprio(1);  // waves of a SIMD drift apart: one's products run beside another's exponentials
       add_chunk(vb);
+      __builtin_amdgcn_s_setprio(0);
     }
     if (!moved) break;  // the last chunk is done
     mn = fmaxf(m, mn);
