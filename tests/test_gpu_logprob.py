@@ -89,7 +89,12 @@ def special(V, dtype):
     block = torch.full((V,), -9.0)
     block[V // 2:V // 2 + 50] = torch.linspace(1, 2, min(50, V - V // 2))  # the best next to each other
     out["best in one place"] = block
-    return list(out), torch.stack([r.to(dtype) for r in out.values()])
+    out["best before a signalling NaN"] = base.float().clone()
+    out["best before a signalling NaN"][:64] = 50.0 + torch.arange(64) / 4
+    x = torch.stack([r.to(dtype) for r in out.values()])
+    bits, snan = (torch.int16, 0x7f81) if dtype == torch.bfloat16 else (torch.int32, 0x7f800001)
+    x[-1].view(bits)[1::2] = snan  # not by value: a conversion would quiet it
+    return list(out), x
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -105,6 +110,25 @@ def test_special_rows(dev, V, k, dtype):
             check(x[i:i + 1], t[i:i + 1], k, one)
         except AssertionError as e:
             raise AssertionError(f"{name}: {e}") from e
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [1400, 4001, 8194, 20500])
+@pytest.mark.parametrize("k", [0, 4, 32])
+def test_special_rows_among_many(dev, V, k, dtype):
+    """1024 rows or more: one wave each."""
+    names, x = special(V, dtype)
+    t = torch.full((len(names),), V // 2)
+    times = 1024 // len(names) + 1
+    res = scoring.token_logprobs(x.to(dev).repeat(times, 1), t.to(dev).repeat(times), k)
+    for first in (0, len(names), (times - 1) * len(names)):  # rows of other alignments where V is odd
+        for i, name in enumerate(names):
+            at = slice(first + i, first + i + 1)
+            one = scoring.TokenLogprobs(*(None if v is None else v[at] for v in vars(res).values()))
+            try:
+                check(x[i:i + 1], t[i:i + 1], k, one)
+            except AssertionError as e:
+                raise AssertionError(f"{name} at row {first + i}: {e}") from e
 
 
 def test_tokens_outside_the_vocabulary(dev):

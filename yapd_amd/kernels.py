@@ -247,17 +247,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Te
     if logits.is_cuda and dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):  # the launch goes to the current device
             return token_logprobs(logits, tokens, logprob, entropy, top_logprob, top_token)
-    wide = logits.dtype == torch.float32
-    require_cuda(logits, "logits", torch.float32 if wide else torch.bfloat16, dev, contiguous=False)
-    shape = logits.shape
-    require(len(shape) in (2, 3) and (shape[-1] <= 1 or logits.stride(-1) == 1),
-            "logits must be [n, V] or [rows, bl, V] with unit last stride")
-    lead = shape[:-1]
-    require_cuda(tokens, "tokens", torch.int64, dev)
+    check_token_logprobs(logits, tokens)
+    lead = logits.shape[:-1]
     require_cuda(logprob, "logprob", torch.float32, dev)
     require_cuda(entropy, "entropy", torch.float32, dev)
-    require(tokens.shape == lead and logprob.shape == lead and entropy.shape == lead,
-            "tokens, logprob and entropy must have the logits' leading shape")
+    require(logprob.shape == lead and entropy.shape == lead, "logprob and entropy must have the logits' leading shape")
     k = 0
     if top_logprob is not None or top_token is not None:
         require(top_logprob is not None and top_token is not None, "top_logprob and top_token come together")
@@ -266,10 +260,29 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Te
         k = top_token.shape[-1]
         require(top_logprob.shape == top_token.shape and top_token.shape[:-1] == lead,
                 "top_logprob and top_token must be [..., k] on the logits' leading shape")
-    seq, pos, rows, bl = (logits.stride(0), 0, shape[0], 1) if len(lead) == 1 else (*logits.stride()[:2], *lead)
+    launch_token_logprobs(logits, tokens, k, logprob, entropy, top_logprob, top_token)
+
+
+def check_token_logprobs(logits: torch.Tensor, tokens: torch.Tensor) -> None:
+    dev, shape = logits.device, logits.shape
+    require_cuda(logits, "logits", torch.float32 if logits.dtype == torch.float32 else torch.bfloat16, dev,
+                 contiguous=False)
+    require(len(shape) in (2, 3) and (shape[-1] <= 1 or logits.stride(-1) == 1),
+            "logits must be [n, V] or [rows, bl, V] with unit last stride")
+    require_cuda(tokens, "tokens", torch.int64, dev)
+    require(tokens.shape == shape[:-1], "tokens must have the logits' leading shape")
+
+
+def launch_token_logprobs(logits, tokens, k: int, logprob, entropy, top_logprob, top_token) -> None:
+    """:func:`token_logprobs` on tensors that are known to fit."""
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) == 2:
+        seq, pos, rows, bl = stride[0], 0, shape[0], 1
+    else:
+        (seq, pos, _), (rows, bl, _) = stride, shape
     check(load_library().yapd_token_logprobs(
-        logits.data_ptr(), wide, seq, pos, rows, bl, shape[-1], tokens.data_ptr(), k, logprob.data_ptr(),
-        entropy.data_ptr(), ptr(top_logprob), ptr(top_token), stream_ptr(dev)))
+        logits.data_ptr(), logits.dtype == torch.float32, seq, pos, rows, bl, shape[-1], tokens.data_ptr(), k,
+        logprob.data_ptr(), entropy.data_ptr(), ptr(top_logprob), ptr(top_token), stream_ptr(logits.device)))
 
 
 # --------------------------------------------------------------------------- #
@@ -461,13 +474,15 @@ def pool_pointers(pools):
     """The device addresses of every layer's pool as the array :func:`kv_copy_pages` hands on, and the
     pools' common shape and device, checked."""
     require(len(pools) >= 1, "no pools")
-    shape, dev = pools[0].shape, pools[0].device
-    require(len(shape) == 4 and shape[0] >= 1 and shape[1] == 2 and shape[3] == 1024, "pools must be [pages, 2, H, 16*64]")
+    shape, dev, bf16 = pools[0].shape, pools[0].device, torch.bfloat16
+    ptrs = []
     for p in pools:
-        require_cuda(p, "pool", torch.bfloat16, dev)
-        if p.shape != shape:
+        if p.dtype is not bf16 or p.shape != shape or p.device != dev or not p.is_cuda or not p.is_contiguous():
+            require_cuda(p, "pool", bf16, dev)
             raise ValueError("every layer's pool must have the same shape")
-    return (c_void * len(pools))(*[p.data_ptr() for p in pools]), shape, dev
+        ptrs.append(p.data_ptr())
+    require(len(shape) == 4 and shape[0] >= 1 and shape[1] == 2 and shape[3] == 1024, "pools must be [pages, 2, H, 16*64]")
+    return (c_void * len(ptrs))(*ptrs), shape, dev
 
 
 def page_ids(ids, name: str):
@@ -477,7 +492,7 @@ def page_ids(ids, name: str):
         require(not ids.is_cuda, f"{name} must be host integers, not a GPU tensor")
         ids = ids.numpy()
     a = np.asarray(ids)
-    if a.dtype != np.int32:
+    if a.dtype != np.int32:  # the library checks the range of those that are
         require(a.size == 0 or (a.dtype.kind in "iu" and bool((a >= 0).all()) and bool((a < 2**31).all())),
                 f"{name} must be page ids (integers of [0, 2^31))")
         a = a.astype(np.int32)

@@ -73,6 +73,7 @@ class PagedKV:
                         device=self.device)
             for _ in range(self.n_layers)
         ]
+        self._addresses, self._checked = [], None  # of the pools, and what was checked of them
 
     @property
     def bytes_per_layer(self) -> int:
@@ -92,7 +93,10 @@ class PagedKV:
         """``pool[dst[i]] = pool[src[i]]`` in every layer's pool for host page ids (see
         :func:`kernels.kv_copy_pages`), on the current stream; torch's index operations on the CPU."""
         if self.device.type == "cuda":
-            kernels.kv_copy_pages(self.pools, src, dst)
+            addresses = [p.data_ptr() for p in self.pools]
+            if addresses != self._addresses:  # the first call, or a pool was replaced
+                self._checked, self._addresses = kernels.pool_pointers(self.pools), addresses
+            kernels.kv_copy_pages_at(*self._checked, src, dst)
             return
         src, dst = (torch.as_tensor(np.asarray(x, dtype=np.int64)) for x in (src, dst))
         for pool in self.pools:
@@ -139,8 +143,6 @@ class SharedPagedKV(PagedKV):
         self.device = torch.device(device)
         self.n_pages = int(n_pages)
         self._make_pools()
-        if self.device.type == "cuda":
-            self._handle = kernels.pool_pointers(self.pools)
         self.table_host = np.zeros((self.n_rows, self.pages_per_row), dtype=np.int32)
         self.table = torch.zeros(self.n_rows, self.pages_per_row, dtype=torch.int32, device=self.device)
         self._refs = np.zeros(self.n_pages, dtype=np.int32)
@@ -155,12 +157,6 @@ class SharedPagedKV(PagedKV):
     def refcount(self, page: int) -> int:
         """Rows that map ``page``."""
         return int(self._refs[page])
-
-    def copy_pages(self, src, dst) -> None:
-        if self.device.type == "cuda":
-            kernels.kv_copy_pages_at(*self._handle, src, dst)
-        else:
-            super().copy_pages(src, dst)
 
     # ------------------------------------------------------------------ #
 

@@ -80,15 +80,19 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
     ``logits`` is bf16 or fp32, ``[n, V]`` or ``[rows, bl, V]`` with a unit last stride; ``tokens`` int64
     of its leading shape (below 0: a position without a token, e.g. padding).  Logits of -inf have
     probability 0.  Summed over its tokens, a candidate's log probability ranks it among others."""
-    lead = tuple(logits.shape[:-1])
     dev = logits.device
-    logprob, entropy = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
+    if logits.is_cuda and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):  # the launch goes to the current device
+            return token_logprobs(logits, tokens, top_k)
+    kernels.check_token_logprobs(logits, tokens)
+    logprob = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty_like(logprob)
     top_logprob = top_token = None
     if top_k:
         kernels.require(1 <= top_k <= kernels.TOP_MAX, f"top_k must be in [0, {kernels.TOP_MAX}]")
-        top_logprob = torch.empty(*lead, top_k, dtype=torch.float32, device=dev)
-        top_token = torch.empty(*lead, top_k, dtype=torch.int64, device=dev)
-    kernels.token_logprobs(logits, tokens, logprob, entropy, top_logprob, top_token)
+        top_logprob = torch.empty(*tokens.shape, top_k, dtype=torch.float32, device=dev)
+        top_token = torch.empty_like(top_logprob, dtype=torch.int64)
+    kernels.launch_token_logprobs(logits, tokens, top_k, logprob, entropy, top_logprob, top_token)
     return TokenLogprobs(logprob, entropy, top_logprob, top_token)
 
 
