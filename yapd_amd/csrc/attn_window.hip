@@ -133,8 +133,11 @@ struct Pages {
 
 constexpr int kWaveFloats = 4 * 64 * 4;  // a wave's O^T tile in LDS: fragment mt of lane l at (mt * 64 + l) * 4
 
+// Chunk c + 1 is on its way while chunk c is multiplied (two or three ahead measured the same: what bounds
+// few workgroups is what one CU can fetch, about 40 GB/s).
 template <int NQT, int KS, int HPW>
-__global__ __launch_bounds__(64 * KS * HPW) void attn_window_kernel(const WindowParams P) {
+__global__ __launch_bounds__(64 * KS * HPW) __attribute__((amdgpu_waves_per_eu(NQT > 2 ? 2 : NQT == 2 ? 3 : 4))) void
+attn_window_kernel(const WindowParams P) {
   constexpr int TQ = 16 * NQT;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -198,11 +201,10 @@ __global__ __launch_bounds__(64 * KS * HPW) void attn_window_kernel(const Window
     const int all_lo = last - P.window + 1;                 // keys from here on are in every query's window
     const int all_hi = P.causal ? min(t.kvl, t.p0 + 1) : t.kvl;  // keys below are before every query's end
 
-    u32x4_t kf[2][2], vf[4], kn[2][2], vn[4];
-    load_chunk(cl.chunk(c0) * kChunk, kf, vf);
-    for (int c = c0; c < c1; ++c) {
+    u32x4_t ka[2][2], va[4], kn[2][2], vn[4];
+    load_chunk(cl.chunk(c0) * kChunk, ka, va);
+    auto step = [&](int c, u32x4_t (&kf)[2][2], u32x4_t (&vf)[4]) {
       const int k0 = cl.chunk(c) * kChunk;
-      if (c + 1 < c1) load_chunk(cl.chunk(c + 1) * kChunk, kn, vn);
       const bool mask = k0 + kChunk > all_hi || (k0 < all_lo && k0 + kChunk > P.sinks);
       if (mask) {
         // V of keys that no query of the tile sees (behind the window, past the
@@ -265,13 +267,13 @@ __global__ __launch_bounds__(64 * KS * HPW) void attn_window_kernel(const Window
           o[qt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(vf[mt]), as_bf16x8(pw), o[qt][mt], 0, 0, 0);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        kf[i][0] = kn[i][0];
-        kf[i][1] = kn[i][1];
-      }
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) vf[mt] = vn[mt];
+    };
+    for (int c = c0; c < c1; c += 2) {
+      if (c + 1 < c1) load_chunk(cl.chunk(c + 1) * kChunk, kn, vn);
+      step(c, ka, va);
+      if (c + 1 >= c1) break;
+      if (c + 2 < c1) load_chunk(cl.chunk(c + 2) * kChunk, ka, va);
+      step(c + 1, kn, vn);
     }
   }
 
@@ -608,10 +610,12 @@ __global__ __launch_bounds__(256) void attn_window_join_kernel(const WindowParam
   const int64_t step = static_cast<int64_t>(P.n_q) * P.H;
   const int64_t at = static_cast<int64_t>(qs + i) * P.H + h;
   float M = -INFINITY;
+#pragma unroll 8
   for (int s = 0; s < P.parts; ++s) M = fmaxf(M, P.part_ml[(s * step + at) * 2]);
   const float mref = M == -INFINITY ? 0.f : M;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
   float L = 0.f;
+#pragma unroll 8
   for (int s = 0; s < P.parts; ++s) {
     const float w = __builtin_amdgcn_exp2f(P.part_ml[(s * step + at) * 2] - mref);
     L += w * P.part_ml[(s * step + at) * 2 + 1];
@@ -631,7 +635,22 @@ struct Cut {
   int64_t slots;
 };
 
-constexpr int64_t kWavesWanted = 2048;  // two a SIMD
+// Waves to a head's chunks, by how many (tile, head) pairs there are; us a call with 1, 2 and 4 of them, 16 heads.
+// One token, 804 of 1201 keys: one row 27.2, 16.0, 8.4; 32 rows (512 pairs) 31.0, 21.0, 20.9; 64 rows 36.6, 38.3, 38.3;
+// 256 rows 140.6, 142.9, 142.9.  Blocks of 32: 32 rows 39.0, 24.4, 24.3; 64 rows 41.7, 42.1, 42.4; 128 rows 79.0, 81.7,
+// 87.0, but 130 ragged rows of 100 to 2000 keys 64.7, 59.6, 56.0.  Blocks of 64: 64 rows 54.8, 48.5, 57.8.  One token
+// on 61 keys, 300 rows: 16.7, 17.9, 22.5.  Eight waves: 8.7 at one row, 14.9 against 13.6 for 16 blocks of 32.
+constexpr int64_t kFour = 512, kTwo = 2560;
+
+// Parts: while there are fewer workgroups than CUs, for at least kPartChunks chunks each, where the second launch
+// (3 us) is won back.  One token, 16 heads, 2000 keys: 16.7 us in one part, 11.1 as cut here; 4000 keys 28.7 and 13.0;
+// 30000 keys 205 and 29.0; eight rows of 4000 keys 34.7 and 25.9; but 804 keys 7.9 in one part and 8.4 in four.
+constexpr int64_t kCUs = 256, kPartChunks = 16;
+
+int parts_of(int64_t workgroups, int64_t chunks) {
+  if (chunks < 3 * kPartChunks) return 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min(kCUs / workgroups, chunks / kPartChunks)));
+}
 
 Cut cut_of(int rows, int max_q, int n_q, bool packed, int n_heads, int window, int sinks, int max_kv) {
   Cut c;
@@ -641,28 +660,19 @@ Cut cut_of(int rows, int max_q, int n_q, bool packed, int n_heads, int window, i
   const int64_t tiles = std::min<int64_t>(c.slots, (n_q + tq - 1) / tq + rows);
   const int64_t keys = std::min<int64_t>(max_kv, static_cast<int64_t>(window) + sinks + tq);
   const int64_t chunks = (keys + kChunk - 1) / kChunk + 1;
-  if (tq == kTileQ) {
-    // parts of at least 16 chunks of 64 keys while there are fewer workgroups than CUs
-    c.ks = 1;
-    const int64_t want = (256 + tiles * n_heads - 1) / (tiles * n_heads);
-    c.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, chunks / 32)));
-    return c;
-  }
-  const int64_t waves = tiles * n_heads;
-  c.ks = waves * 4 <= kWavesWanted && chunks >= 8 ? 8 : waves <= kWavesWanted && chunks >= 4 ? 4 : 1;
-  // more parts only where eight waves are not enough, each with eight chunks a wave
-  const int64_t want = (kWavesWanted + waves * c.ks - 1) / (waves * c.ks);
-  c.parts = c.ks < 8 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, chunks / (8 * c.ks))));
+  const int64_t pairs = tiles * n_heads;
+  c.ks = tq == kTileQ ? 1 : pairs <= kFour && chunks >= 4 ? 4 : pairs <= kTwo && chunks >= 2 ? 2 : 1;
+  c.parts = tq == kTileQ ? parts_of(pairs, chunks / 2) : c.ks == 4 ? parts_of(pairs, chunks) : 1;
   return c;
 }
 
 template <int NQT>
 void launch_tiles(const WindowParams& P, const Cut& c, hipStream_t st) {
   const int64_t items = c.slots * P.parts;
-  if (c.ks == 8)
-    hipLaunchKernelGGL((attn_window_kernel<NQT, 8, 1>), dim3(items * P.H), dim3(512), 0, st, P);
-  else if (c.ks == 4)
+  if (c.ks == 4)
     hipLaunchKernelGGL((attn_window_kernel<NQT, 4, 1>), dim3(items * P.H), dim3(256), 0, st, P);
+  else if (c.ks == 2)
+    hipLaunchKernelGGL((attn_window_kernel<NQT, 2, 2>), dim3(items * (P.H / 2)), dim3(256), 0, st, P);
   else
     hipLaunchKernelGGL((attn_window_kernel<NQT, 1, 4>), dim3(items * (P.H / 4)), dim3(256), 0, st, P);
 }
