@@ -6,6 +6,14 @@
 // destination (the host checks), so the copies may run in any order, all layers in one launch.
 // The pairs and the pool addresses travel as kernel arguments: no upload, no
 // device list to keep alive, and a captured launch holds its own copy.
+//
+// Bound by memory.  30 layers of 16 heads: 301 pages 217 us, 5.45 TB/s read and
+// written (a copy of 1 GiB reaches 5.18); a prefix of 19 pages to seven rows
+// 48.6 us; one page 2.8 us.  The stores are non-temporal, so they do not push
+// out what is still to be read: with plain ones the prefix, whose reads the
+// caches can serve six times of seven, takes 79.6 us and the 301 pages 225.9.
+// One workgroup that reads a source's segment once and writes all its copies
+// was slower (54.3 us), having fewer loads in flight.
 #include <new>
 #include <vector>
 
@@ -39,7 +47,8 @@ __global__ __launch_bounds__(256) void kv_copy_pages_kernel(const CopyParams P) 
     if (w0 + 256 * i < P.words) v[i] = load16(src + (w0 + 256 * i) * 8);
 #pragma unroll
   for (int i = 0; i < kWords / 256; ++i)
-    if (w0 + 256 * i < P.words) *reinterpret_cast<u32x4_t*>(dst + (w0 + 256 * i) * 8) = v[i];
+    if (w0 + 256 * i < P.words)
+      __builtin_nontemporal_store(v[i], reinterpret_cast<u32x4_t*>(dst + (w0 + 256 * i) * 8));
 }
 
 // Whether the pairs may be copied in any order: ids inside the pool, every

@@ -477,10 +477,11 @@ def pool_pointers(pools):
     shape, dev, bf16 = pools[0].shape, pools[0].device, torch.bfloat16
     ptrs = []
     for p in pools:
-        if p.dtype is not bf16 or p.shape != shape or p.device != dev or not p.is_cuda or not p.is_contiguous():
+        if p.dtype is not bf16 or p.shape != shape or p.device != dev or not p.is_contiguous():
             require_cuda(p, "pool", bf16, dev)
             raise ValueError("every layer's pool must have the same shape")
         ptrs.append(p.data_ptr())
+    require_cuda(pools[0], "pool", bf16, dev)
     require(len(shape) == 4 and shape[0] >= 1 and shape[1] == 2 and shape[3] == 1024, "pools must be [pages, 2, H, 16*64]")
     return (c_void * len(ptrs))(*ptrs), shape, dev
 
