@@ -98,6 +98,14 @@ def test_static_rows_copy_as_before(dev):
         assert same(p, w)
 
 
+def test_a_replaced_pool_is_checked_again(dev):
+    kv = PagedKV(n_layers=2, n_rows=2, pages_per_row=4, n_heads=4, device=dev)
+    kv.copy_row_pages(0, 1, 20)
+    kv.pools[0] = kv.pools[0][:6]  # the same address, fewer pages
+    with pytest.raises(ValueError, match="same shape"):
+        kv.copy_row_pages(0, 1, 20)
+
+
 def test_long_use_keeps_to_its_window_of_pages(dev):
     """One row written and released behind its window: the pool never holds more than the window needs."""
     kv = SharedPagedKV(n_layers=1, n_rows=1, pages_per_row=40, n_heads=4, device=dev, n_pages=8)

@@ -374,6 +374,7 @@ def attn_window(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len
 
     Lengths are read on the device: no plan, and a captured call follows them.  ``max_q`` and
     ``max_kv`` are the host's upper bounds (default: all queries, all positions the table maps).
+    ``scale`` is positive, and scores have to stay below 2^30 in magnitude.
     Few queries over many keys need a float32 ``workspace``
     (``yapd_attn_window_workspace``), allocated here unless given.
     """
@@ -471,8 +472,7 @@ def kv_gather(pool: torch.Tensor, table_row: torch.Tensor, kv_len: int):
 
 
 def pool_pointers(pools):
-    """The device addresses of every layer's pool as the array :func:`kv_copy_pages` hands on, and the
-    pools' common shape and device, checked."""
+    """The device addresses of every layer's pool, and the pools' common shape and device, checked."""
     require(len(pools) >= 1, "no pools")
     shape, dev, bf16 = pools[0].shape, pools[0].device, torch.bfloat16
     ptrs = []
@@ -508,14 +508,10 @@ def kv_copy_pages(pools, src, dst) -> None:
     ``src`` and ``dst`` are host page ids.  A source may repeat (a fork); a page that is the
     destination of two pairs, or a source and a destination, is refused, so the result does not
     depend on the order of the copies."""
-    kv_copy_pages_at(*pool_pointers(pools), src, dst)
-
-
-def kv_copy_pages_at(ptrs, shape, dev: torch.device, src, dst) -> None:
-    """:func:`kv_copy_pages` on what :func:`pool_pointers` gave for pools that are still alive."""
+    ptrs, shape, dev = pool_pointers(pools)
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):  # the launch goes to the current device
-            return kv_copy_pages_at(ptrs, shape, dev, src, dst)
+            return kv_copy_pages(pools, src, dst)
     src, dst = page_ids(src, "src"), page_ids(dst, "dst")
     require(src.size == dst.size, "src and dst must have the same length")
     check(load_library().yapd_kv_copy_pages(ptrs, len(ptrs), shape[0], shape[2], src.ctypes.data, dst.ctypes.data,

@@ -73,7 +73,6 @@ class PagedKV:
                         device=self.device)
             for _ in range(self.n_layers)
         ]
-        self._addresses, self._checked = [], None  # of the pools, and what was checked of them
 
     @property
     def bytes_per_layer(self) -> int:
@@ -93,10 +92,7 @@ class PagedKV:
         """``pool[dst[i]] = pool[src[i]]`` in every layer's pool for host page ids (see
         :func:`kernels.kv_copy_pages`), on the current stream; torch's index operations on the CPU."""
         if self.device.type == "cuda":
-            addresses = [p.data_ptr() for p in self.pools]
-            if addresses != self._addresses:  # the first call, or a pool was replaced
-                self._checked, self._addresses = kernels.pool_pointers(self.pools), addresses
-            kernels.kv_copy_pages_at(*self._checked, src, dst)
+            kernels.kv_copy_pages(self.pools, src, dst)
             return
         src, dst = (torch.as_tensor(np.asarray(x, dtype=np.int64)) for x in (src, dst))
         for pool in self.pools:
