@@ -195,7 +195,8 @@ int yapd_attn_paged_block_noalloc(const void* q, const void* kv_pool, int64_t n_
  * sizes.  With few queries over many keys the keys are cut into parts joined
  * by a second launch: workspace then holds yapd_attn_window_workspace() floats
  * (0: not needed, may be NULL), 16-byte aligned, not shared by calls that may
- * overlap.  window >= 1, sinks >= 0, H a multiple of 4, scale > 0. */
+ * overlap.  window >= 1, sinks >= 0, H a multiple of 4, 1e-30 <= scale <= 1e30
+ * and scores (scale q.k) below 2^30 in magnitude. */
 int yapd_attn_window(const void* q, int64_t q_tok_stride, const void* kv_pool, int64_t n_pages,
                      const int32_t* page_table, int table_stride, int table_cols, const int32_t* kv_len,
                      const int32_t* q_start, int rows, int max_q, int n_q, int n_heads, int window, int sinks,

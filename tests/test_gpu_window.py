@@ -192,6 +192,23 @@ def test_full_window_agrees_with_the_paged_block_attention(dev):
     c.check(other)
 
 
+@pytest.mark.parametrize("rows,H,bl,kv", [(2, 4, 1, 700), (1, 4, 1, 20000), (2, 4, 40, 300), (2, 4, 150, 400),
+                                          (1, 4, 150, 9000)])
+def test_scales_at_the_ends_of_the_range(dev, rows, H, bl, kv):
+    """A power of two moved between the queries and the scale changes nothing, bit for bit; with the
+    smallest scale every visible key weighs the same."""
+    c = Case(q_lens=[bl] * rows, kv_lens=[kv] * rows, H=H, window=kv, sinks=0, causal=True)
+    t = c.device(dev)
+
+    def run(q, scale):
+        out = torch.empty_like(q)
+        kernels.attn_window(q, t["pool"], t["table"], t["kv_len"], out, scale, window=kv)
+        return out.view(torch.int16)
+
+    assert bool((run(t["q"], 0.125) == run(t["q"] * 2.0**-100, 0.125 * 2.0**100)).all())
+    assert bool((run(t["q"], 1e-30) == run(torch.zeros_like(t["q"]), 0.125)).all())
+
+
 def test_no_queries_or_rows_is_no_launch(dev):
     pool = torch.zeros(2, 2, 4, 1024, dtype=torch.bfloat16, device=dev)
     i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731

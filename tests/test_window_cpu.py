@@ -40,6 +40,7 @@ GOOD = dict(q=P, q_stride=1024, pool=P, n_pages=64, table=P, table_stride=8, tab
     (dict(out=P + 2), b"16-byte aligned"), (dict(q_stride=1000), b"q_tok_stride"), (dict(q_stride=1028), b"q_tok_stride"),
     (dict(n_pages=0), b"empty pool"), (dict(table_cols=9), b"empty pool or table"), (dict(n_q=9), b"rows * max_q"),
     (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"), (dict(scale=float("inf")), b"scale"),
+    (dict(scale=1e-31), b"scale"), (dict(scale=1e31), b"scale"), (dict(scale=float("nan")), b"scale"),
     (dict(table_cols=2**27, table_stride=2**27), b"table_cols"),
     (dict(rows=1, max_q=1, n_q=1, n_heads=4, window=20000, max_kv=20000), b"workspace must be"),
     (dict(rows=1, max_q=1, n_q=1, n_heads=4, window=20000, max_kv=20000, ws=P, ws_floats=100), b"workspace must be"),

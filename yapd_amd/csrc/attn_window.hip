@@ -15,7 +15,6 @@
 // launch.  Chunk arithmetic is that of the paged block attention: S^T = K Q^T
 // and O^T += V^T P^T on v_mfma_f32_16x16x32_bf16, every lane owning one query.
 #include <algorithm>
-#include <cmath>
 
 #include "attn_tile.h"
 #include "common.h"
@@ -714,7 +713,8 @@ extern "C" int yapd_attn_window(const void* q, int64_t q_tok_stride, const void*
   YAPD_REQUIRE(table_cols <= yapd::kCap / yapd::kPageSize, "attn_window: table_cols must be at most 2^26");
   YAPD_REQUIRE(q_start != nullptr || n_q == static_cast<int64_t>(rows) * max_q,
                "attn_window: without q_start n_q must be rows * max_q");
-  YAPD_REQUIRE(std::isfinite(scale) && scale > 0.f, "attn_window: scale must be finite and > 0");
+  // 8 / scale and scale * log2(e) * a score stay in range
+  YAPD_REQUIRE(scale >= 1e-30f && scale <= 1e30f, "attn_window: scale must be in [1e-30, 1e30]");
   const yapd::Cut c = yapd::cut_of(rows, max_q, n_q, q_start != nullptr, n_heads, window, sinks, max_kv);
   YAPD_REQUIRE(c.slots * c.parts * n_heads < (int64_t{1} << 22), "attn_window: too many tiles for one launch");
   const int64_t tokens = static_cast<int64_t>(c.parts) * n_q * n_heads;

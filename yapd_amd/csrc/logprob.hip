@@ -500,8 +500,8 @@ extern "C" int yapd_token_logprobs(const void* logits, int wide, int64_t seq_str
   YAPD_REQUIRE(logits && tokens && logprob && entropy && (top_k == 0 || (top_logprob && top_token)),
                "token_logprobs: NULL pointer");
   YAPD_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (wide ? 3u : 1u)) == 0, "token_logprobs: misaligned logits");
-  yapd::LogprobParams P{logits, seq_stride, pos_stride, static_cast<uint32_t>(items), static_cast<uint32_t>(bl), vocab, top_k, tokens, logprob, entropy,
-                          top_logprob, top_token};
+  const yapd::LogprobParams P{logits, seq_stride, pos_stride, static_cast<uint32_t>(items), static_cast<uint32_t>(bl),
+                              vocab, top_k, tokens, logprob, entropy, top_logprob, top_token};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (wide)
     yapd::launch_rows<true>(P, st);
