@@ -161,6 +161,15 @@ def test_same_bits_twice_and_under_capture(dev):
             assert all(torch.equal(a, b) for a, b in zip(vars(res).values(), vars(first).values()))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_past_32_bits_of_elements(dev, dtype):
+    x, _ = rows(3, 1000, dtype, 5)
+    far = torch.empty(2**31 + 4096, dtype=dtype, device=dev).as_strided((3, 1000), (2**30 + 1024, 1))
+    far.copy_(x)
+    tokens = torch.tensor([0, 999, 500], device=dev)
+    check(far, tokens, 8, scoring.token_logprobs(far, tokens, top_k=8))
+
+
 def test_empty(dev):
     res = scoring.token_logprobs(torch.empty(0, 50, dtype=torch.bfloat16, device=dev),
                                  torch.empty(0, dtype=torch.int64, device=dev), 3)

@@ -39,6 +39,17 @@ def test_copies(dev, layers, heads, pages, n, shared):
     assert all(same(p, w) for p, w in zip(pools, want))
 
 
+def test_pages_past_32_bits_of_elements(dev):
+    n = 2**31 // (2 * 4 * 1024) + 5
+    pool = torch.empty(n, 2, 4, 1024, dtype=torch.bfloat16, device=dev)
+    pool[:4].normal_()
+    pool[-3:].normal_()
+    want = pool[0].clone(), pool[-1].clone()
+    kernels.kv_copy_pages([pool], [0, n - 1], [n - 2, 2])
+    assert same(pool[n - 2], want[0]) and same(pool[2], want[1])
+    assert same(pool[0], want[0]) and same(pool[-1], want[1])
+
+
 def test_no_pairs(dev):
     pools = pools_of(dev, 1, 3, 4)
     want = pools[0].clone()

@@ -192,6 +192,23 @@ def test_full_window_agrees_with_the_paged_block_attention(dev):
     c.check(other)
 
 
+@pytest.mark.parametrize("q", [1, 30, 150])
+def test_pages_past_32_bits_of_elements(dev, q):
+    """The same rows on the first and on the last pages of a pool of 2^31 + 2^19 elements: the same bits."""
+    c = Case(q_lens=[q] * 2, kv_lens=[200, 333], H=4, window=100, sinks=7, causal=True)
+    t = c.device(dev)
+    n_pages, first = 2**31 // (2 * 4 * 1024) + 64, c.pool.shape[0]
+    pool = torch.empty(n_pages, 2, 4, 1024, dtype=torch.bfloat16, device=dev)
+    pool[:first], pool[-first:] = t["pool"], t["pool"]
+    outs = []
+    for shift in (0, n_pages - first):
+        out = torch.full_like(t["q"], 77.0)
+        kernels.attn_window(t["q"], pool, (t["table"] + shift).contiguous(), t["kv_len"], out, 0.125, window=100, sinks=7)
+        outs.append(out)
+    c.check(outs[0])
+    assert bool((outs[0].view(torch.int16) == outs[1].view(torch.int16)).all())
+
+
 @pytest.mark.parametrize("rows,H,bl,kv", [(2, 4, 1, 700), (1, 4, 1, 20000), (2, 4, 40, 300), (2, 4, 150, 400),
                                           (1, 4, 150, 9000)])
 def test_scales_at_the_ends_of_the_range(dev, rows, H, bl, kv):
