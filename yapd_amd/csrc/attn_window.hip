@@ -591,14 +591,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void a
   }
 }
 
-// Joins the parts of every query: thread (query, head, 4 head-dim values).
+// Joins the parts of every query: thread (query, head, 4 head-dim values).  Eight parts' values are requested
+// before the first is used, so up to eight parts cost one memory latency: what bounds it.
 __global__ __launch_bounds__(256) void attn_window_join_kernel(const WindowParams P) {
+  constexpr int kAtOnce = 8;
   const int lane = threadIdx.x & 63;
-  const int per = 256 / 16;  // (query, head) pairs of a workgroup
-  const int64_t pair = static_cast<int64_t>(blockIdx.x) * per + (threadIdx.x >> 4);
-  const int64_t row_q = pair / P.H;
+  // there are parts only where (query, head) pairs are few: they fit 32 bits
+  const uint32_t pair = blockIdx.x * 16 + (threadIdx.x >> 4);
+  const uint32_t row_q = pair / static_cast<uint32_t>(P.H);
   const int h = static_cast<int>(pair - row_q * P.H);
-  const int r = static_cast<int>(row_q / P.max_q), i = static_cast<int>(row_q - static_cast<int64_t>(r) * P.max_q);
+  const int r = static_cast<int>(row_q / P.max_q), i = static_cast<int>(row_q - static_cast<uint32_t>(r) * P.max_q);
   if (r >= P.rows) return;
   int qs = r * P.max_q, qc = P.max_q;
   if (P.q_start != nullptr) {
@@ -608,17 +610,32 @@ __global__ __launch_bounds__(256) void attn_window_join_kernel(const WindowParam
   if (i >= qc) return;
   const int64_t step = static_cast<int64_t>(P.n_q) * P.H;
   const int64_t at = static_cast<int64_t>(qs + i) * P.H + h;
-  float M = -INFINITY;
-#pragma unroll 8
-  for (int s = 0; s < P.parts; ++s) M = fmaxf(M, P.part_ml[(s * step + at) * 2]);
-  const float mref = M == -INFINITY ? 0.f : M;
+  float M = -INFINITY, L = 0.f;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-  float L = 0.f;
-#pragma unroll 8
-  for (int s = 0; s < P.parts; ++s) {
-    const float w = __builtin_amdgcn_exp2f(P.part_ml[(s * step + at) * 2] - mref);
-    L += w * P.part_ml[(s * step + at) * 2 + 1];
-    acc += w * *reinterpret_cast<const f32x4_t*>(P.part_o + (s * step + at) * kHeadDim + (lane & 15) * 4);
+  for (int s0 = 0; s0 < P.parts; s0 += kAtOnce) {
+    float2 ml[kAtOnce];
+    f32x4_t po[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int64_t from = min(s0 + j, P.parts - 1) * step + at;
+      ml[j] = *reinterpret_cast<const float2*>(P.part_ml + from * 2);
+      po[j] = *reinterpret_cast<const f32x4_t*>(P.part_o + from * kHeadDim + (lane & 15) * 4);
+    }
+    float mn = M;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) mn = fmaxf(mn, ml[j].x);  // the last part's again past the end
+    const float mref = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(M - mref);
+    M = mn;
+    L *= alpha;
+    acc *= alpha;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (s0 + j >= P.parts) break;
+      const float w = __builtin_amdgcn_exp2f(ml[j].x - mref);
+      L += w * ml[j].y;
+      acc += w * po[j];
+    }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   u32x2_t w2;
@@ -641,13 +658,14 @@ struct Cut {
 // on 61 keys, 300 rows: 16.7, 17.9, 22.5.  Eight waves: 8.7 at one row, 14.9 against 13.6 for 16 blocks of 32.
 constexpr int64_t kFour = 512, kTwo = 2560;
 
-// Parts: while there are fewer workgroups than CUs, for at least kPartChunks chunks each, where the second launch
-// (3 us) is won back.  One token, 16 heads, 2000 keys: 16.7 us in one part, 11.1 as cut here; 4000 keys 28.7 and 13.0;
-// 30000 keys 205 and 29.0; eight rows of 4000 keys 34.7 and 25.9; but 804 keys 7.9 in one part and 8.4 in four.
-constexpr int64_t kCUs = 256, kPartChunks = 16;
+// Parts: while there are fewer workgroups than CUs, for at least kPartChunks chunks each.  us with one part and as cut
+// here, one token, 16 heads: 1400 keys 10.2, 8.5; 2000 keys 16.7, 8.7; 4000 keys 28.7, 11.8; 30000 keys 205, 27.5; four
+// rows of 1400 keys 13.5, 10.2; eight rows of 4000 keys 34.7, 25.5.  Below five parts' chunks the second launch costs
+// the host (2 us) more than it saves: 1028 keys 8.8 in one part, 8.2 in four; 804 keys 7.6 and 8.0.
+constexpr int64_t kCUs = 256, kPartChunks = 8;
 
 int parts_of(int64_t workgroups, int64_t chunks) {
-  if (chunks < 3 * kPartChunks) return 1;
+  if (chunks < 5 * kPartChunks) return 1;
   return static_cast<int>(std::max<int64_t>(1, std::min(kCUs / workgroups, chunks / kPartChunks)));
 }
 
