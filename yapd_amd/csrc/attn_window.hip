@@ -658,15 +658,17 @@ struct Cut {
 // on 61 keys, 300 rows: 16.7, 17.9, 22.5.  Eight waves: 8.7 at one row, 14.9 against 13.6 for 16 blocks of 32.
 constexpr int64_t kFour = 512, kTwo = 2560;
 
-// Parts: while there are fewer workgroups than CUs, for at least kPartChunks chunks each.  us with one part and as cut
-// here, one token, 16 heads: 1400 keys 10.2, 8.5; 2000 keys 16.7, 8.7; 4000 keys 28.7, 11.8; 30000 keys 205, 27.5; four
-// rows of 1400 keys 13.5, 10.2; eight rows of 4000 keys 34.7, 25.5.  Below five parts' chunks the second launch costs
-// the host (2 us) more than it saves: 1028 keys 8.8 in one part, 8.2 in four; 804 keys 7.6 and 8.0.
-constexpr int64_t kCUs = 256, kPartChunks = 8;
+// Parts: as many as bring the workgroups to `wanted`, of at least `least` chunks each.  us in one part and as cut here.
+// Waves on short tiles, up to the number of CUs and 8 chunks; one token, 16 heads: 1400 keys 10.2, 8.5; 2000 keys 16.7,
+// 8.7; 4000 keys 28.7, 11.8; 30000 keys 205, 27.5; four rows of 1400 keys 13.5, 10.2; eight of 4000 keys 34.7, 25.5.
+// Below kCutChunks the second launch costs the host (2 us) more than it saves: 1028 keys 8.8, 8.2 in four parts; 804
+// keys 7.6, 8.0.  The tile kernel, which gains until a CU holds three workgroups, and 16 chunks; 200 queries, 16 heads:
+// 1400 keys 24, 17.9; 4200 keys 64, 21.3 (parts of 8 chunks 24.4); 1300 on 9300 keys 132, 76 (to two a CU 91).
+constexpr int64_t kCutChunks = 40;
 
-int parts_of(int64_t workgroups, int64_t chunks) {
-  if (chunks < 5 * kPartChunks) return 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min(kCUs / workgroups, chunks / kPartChunks)));
+int parts_of(int64_t workgroups, int64_t wanted, int64_t chunks, int64_t least) {
+  if (chunks < kCutChunks) return 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min(wanted / workgroups, chunks / least)));
 }
 
 Cut cut_of(int rows, int max_q, int n_q, bool packed, int n_heads, int window, int sinks, int max_kv) {
@@ -679,7 +681,7 @@ Cut cut_of(int rows, int max_q, int n_q, bool packed, int n_heads, int window, i
   const int64_t chunks = (keys + kChunk - 1) / kChunk + 1;
   const int64_t pairs = tiles * n_heads;
   c.ks = tq == kTileQ ? 1 : pairs <= kFour && chunks >= 4 ? 4 : pairs <= kTwo && chunks >= 2 ? 2 : 1;
-  c.parts = tq == kTileQ ? parts_of(pairs, chunks / 2) : c.ks == 4 ? parts_of(pairs, chunks) : 1;
+  c.parts = tq == kTileQ ? parts_of(pairs, 768, chunks, 16) : c.ks == 4 ? parts_of(pairs, 256, chunks, 8) : 1;
   return c;
 }
 
