@@ -14,6 +14,12 @@
 // runs (waves); runs join in LDS, parts through a workspace and a second
 // launch.  Chunk arithmetic is that of the paged block attention: S^T = K Q^T
 // and O^T += V^T P^T on v_mfma_f32_16x16x32_bf16, every lane owning one query.
+//
+// Short tiles are bound by memory: 256 ragged rows of one token on up to 1088 keys
+// x 16 heads 169 us, 5.9 TB/s; three rows on 16384 keys 37.0 us, 5.5 TB/s; 130
+// blocks of 32 on up to 565 keys 61 us, 4.8 TB/s.  One row on 1028 keys takes 8.8 us:
+// length, page ids and keys are loads that wait for each other, and one CU fetches
+// about 50 GB/s.
 #include <algorithm>
 
 #include "attn_tile.h"
@@ -344,11 +350,21 @@ attn_window_kernel(const WindowParams P) {
 }
 
 // Long runs of queries: a workgroup takes 128 queries of one head, 32 a wave,
-// and brings 64-key chunks through LDS, where the four waves share them; three
-// chunks are in flight, one barrier a chunk.  v_mfma_f32_32x32x16_bf16: S^T = K Q^T
+// and brings 64-key chunks through a ring of two LDS stages, where the four
+// waves share them, one barrier a chunk.  v_mfma_f32_32x32x16_bf16: S^T = K Q^T
 // (M = keys, N = queries) leaves a lane one query and half of a tile's keys;
 // K rows are permuted so that those are 8 consecutive keys per 16, the operand
 // of O^T += V^T P^T, and 8 consecutive bf16 of a V^T row of a page.
+//
+// Bound by issue: a wave's 32 x 64 scores are 123 vector instructions (64 of
+// them the exponentials and their arguments) beside 16 products that hold the
+// vector unit for part of their 32 cycles each; four workgroups a CU run at
+// 1.9 GHz, where the card holds its power.  8000 queries x 16 heads on a window
+// of 2048: 91 us, 0.74 PF/s; without the products 61, without the exponentials
+// 79.  A third or fourth stage gains 2 to 4 % where workgroups are few and costs
+// a workgroup of a CU where they are many (100 us); one workgroup a CU takes 1 us
+// a chunk.  From 65 queries on: 16 rows of 80 x 16 heads 27.4 us, in tiles of 64
+// on single waves 38.9; 64 rows of 64 there 48.4, here 54.0.
 //
 // LDS: K rows of 128 bytes, 16-byte piece c of key j in slot c ^ (j / 2 & 7); V^T
 // pages of 64 x 32 bytes, the halves swapped where hd & 8: the 16 lanes of a
