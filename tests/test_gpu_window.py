@@ -60,6 +60,23 @@ def test_packed_rows(dev, q, kv, H, window, sinks, causal):
     c.check(c.run(dev, kernels, max_q=max(q), max_kv=max(kv)))
 
 
+@pytest.mark.parametrize("rows,H", [(2, 4), (63, 4), (64, 4), (65, 4), (64, 16), (44, 64)])
+@pytest.mark.parametrize("window,causal", [(1, True), (200, True), (200, False), (100000, True)])
+def test_packed_prompts_among_short_rows(dev, rows, H, window, causal):
+    """Rows of 0 to 3 tiles of 128 queries behind 0 to 3 tiles of earlier keys, some of them empty; of few and of many
+    workgroups."""
+    g = torch.Generator().manual_seed(rows + H)
+    q = [int(x) for x in torch.tensor([0, 1, 2, 70, 127, 128, 129, 300])[torch.randint(0, 8, (rows,), generator=g)]]
+    q[-1] = 131
+    past = [int(x) for x in torch.randint(0, 400, (rows,), generator=g)]
+    past[0] = 0
+    if rows > 40:  # the oracle's time
+        q = [min(x, 131) for x in q]
+    c = Case(q_lens=q, kv_lens=[a + b for a, b in zip(q, past)], H=H, window=window, sinks=3, causal=causal, packed=True,
+             tail_q=3)
+    c.check(c.run(dev, kernels))
+
+
 def test_packed_many_rows(dev):
     """More rows than 64 * 64: three steps of the row search."""
     n = 4500

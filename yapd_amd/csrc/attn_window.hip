@@ -373,6 +373,68 @@ constexpr int kTileQ = 128, kTileChunk = 64, kStages = 2;
 constexpr float kSlack = 8.f;
 constexpr int kStage = 2 * kTileChunk * kHeadDim * 2;  // bytes
 
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) {
+  return __builtin_amdgcn_mov_dpp(v, CTRL, 0xF, 0xF, true);  // no lane is out of range
+}
+// A wave's sum or maximum, uniform: quad permutes, half-row and row mirrors, then the four rows.
+template <class Op>
+__device__ __forceinline__ int wave_reduce(int v, Op op) {
+  v = op(v, dpp<0xB1>(v));
+  v = op(v, dpp<0x4E>(v));
+  v = op(v, dpp<0x141>(v));
+  v = op(v, dpp<0x140>(v));
+  return op(op(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+            op(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+
+// find_tile for packed rows that a wave holds one a lane: slot i is the i-th tile by weight, the heaviest first (the
+// weight: keys before the tile, in tiles, up to the window).  All workgroups of a launch that fits the chip start at
+// once, a CU has every 256th of them, and tiles of a row's begin weigh little: in the order of the rows some CUs have
+// half as much again as the mean.  us by weight / in row order, 16 heads, prompts of 70 to 1500 tokens: 9 on a window
+// of 512 27.2 / 33.0, of 4000 33.1 / 40.5; 20 (2300 workgroups) 51.0 / 55.4 and 58.4 / 68.1; but 40 (4600) 110.6 / 108.1,
+// where the light tiles' start is no longer hidden behind heavy ones.
+constexpr unsigned kWeighed = 2560;  // workgroups
+
+__device__ __forceinline__ bool find_weighed_tile(const WindowParams& P, int slot, int lane, Tile& t) {
+  const int r = min(lane, P.rows - 1);
+  const int qs = first_query(P, r), qe = first_query(P, r + 1);
+  const int len = min(max(P.kv_len[r], 0), P.table_cols * kPageSize);
+  const int n = lane < P.rows ? min(max(qe - qs, 0), P.max_q) : 0;
+  const int tiles = (n + kTileQ - 1) / kTileQ, before = max(len - n, 0) / kTileQ;
+  const auto add = [](int a, int b) { return a + b; };
+  const auto larger = [](int a, int b) { return max(a, b); };
+  const int top = wave_reduce(tiles > 0 ? min(tiles - 1 + before, (P.window + kTileQ - 1) / kTileQ) : 0, larger);
+  const auto first_of = [&](int w) { return w > top ? tiles : min(max(w - before, 0), tiles); };  // tile of weight >= w
+  if (slot >= wave_reduce(tiles, add)) return false;
+  int lo = 0, hi = top + 1, above = 0;  // weights >= lo hold more than `slot` tiles, weights >= hi hold `above`, no more
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1, count = wave_reduce(tiles - first_of(mid), add);
+    if (count > slot) {
+      lo = mid;
+    } else {
+      hi = mid;
+      above = count;
+    }
+  }
+  const int k0 = first_of(lo), m = first_of(hi) - k0;  // this row's tiles of weight lo
+  int sum = m;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int left = __shfl_up(sum, d);
+    if (lane >= d) sum += left;
+  }
+  const int at = __ffsll(static_cast<unsigned long long>(__ballot(sum > slot - above))) - 1;
+  const int first = __builtin_amdgcn_readlane(k0 + m - sum, at) + slot - above;
+  t.row = at;
+  t.kvl = __builtin_amdgcn_readlane(len, at);
+  const int qc = __builtin_amdgcn_readlane(n, at);
+  t.p0 = t.kvl - qc + first * kTileQ;
+  t.qs = __builtin_amdgcn_readlane(qs, at) + first * kTileQ;
+  t.qc = min(kTileQ, qc - first * kTileQ);
+  return true;
+}
+
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void attn_window_tile_kernel(const WindowParams P) {
   // dynamic: only the direct loads write it, which the compiler does not see as writes of a static array
   extern __shared__ __attribute__((aligned(16))) char ring[];
@@ -382,7 +444,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void a
   const int h = static_cast<int>(blockIdx.x) - item * P.H;
   const int slot = item / P.parts, part = item - slot * P.parts;
   Tile t;
-  if (!find_tile<kTileQ>(P, slot, lane, t)) return;  // the whole workgroup
+  if (P.q_start != nullptr && P.rows > 1 && P.rows <= 64 && gridDim.x <= kWeighed) {
+    if (!find_weighed_tile(P, slot, lane, t)) return;  // the whole workgroup
+  } else if (!find_tile<kTileQ>(P, slot, lane, t)) {
+    return;
+  }
   const int g = lane >> 5, n = lane & 31;
   const int H = P.H;
   const ChunkList cl(P, t, kTileChunk);
