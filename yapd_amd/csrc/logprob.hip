@@ -134,14 +134,17 @@ __global__ __launch_bounds__(64 * NW * ROWS) void token_logprob_kernel(const Log
   constexpr int TH = 64 * NW;
   constexpr int LE = RD * GE;        // elements of a lane's tile
   constexpr int W = NW * ROWS;
-  constexpr int kTiles = 8;          // maxima of a lane in LDS; each is of as many tiles as it takes
+  constexpr int SUB = NW == 1 ? RD : 3;  // granules of a lane to a maximum that is kept
+  constexpr int kKept = 24;          // maxima of a lane in LDS; each is of as many SUB granules as it takes
+  static_assert(RD % SUB == 0);
   constexpr int kBatch = 8;          // lanes of a wave that have their granules in LDS at a time
   __shared__ float s_stat[NW][3];
   __shared__ uint32_t s_bound[NW][2];
   __shared__ int s_count;
   __shared__ uint64_t s_list[ROWS][kList];
-  // several waves a row: the maxima of (lane, tile) pairs, and those pairs that are read again
-  __shared__ float s_max[NW == 1 ? 1 : W][kTiles][64];
+  // several waves a row: the maxima of (lane, SUB granules) pairs, their orders' upper halves, and those pairs that are
+  // read again
+  __shared__ uint16_t s_max[NW == 1 ? 1 : W][kKept][64];
   __shared__ uint16_t s_pair[NW == 1 ? 1 : W][kPairs];
   // one wave a row: the granules of lanes with candidates
   __shared__ u32x4_t s_gran[NW == 1 ? W : 1][kBatch][RD];
@@ -165,8 +168,9 @@ __global__ __launch_bounds__(64 * NW * ROWS) void token_logprob_kernel(const Log
   float m = -INFINITY, s = 0.f, t = 0.f;  // of this lane: maximum, sum 2^d, sum d 2^d, d = (x - m) log2(e)
   uint32_t best_bound = kNone;            // order of T
   int n_list = 0;                         // candidates; past kList they are only counted
-  int g0 = wave * 64, tile = 0;
-  const int fold = (n_gran + RD * TH * kTiles - 1) / (RD * TH * kTiles);  // tiles to a maximum in LDS
+  int g0 = wave * 64;
+  const int fold = (n_gran + SUB * TH * kKept - 1) / (SUB * TH * kKept);  // times SUB granules to a maximum in LDS
+  int kept = 0, folds = 0;                                                // maxima there, and how often the last one was raised
   float folded = -INFINITY;
   // Order of the wave's n-th largest lane maximum (below kNone if it has fewer lanes).
   auto nth_maximum = [&](int n) {
@@ -225,10 +229,24 @@ __global__ __launch_bounds__(64 * NW * ROWS) void token_logprob_kernel(const Log
     }
     float tm = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < RD; ++j) {
-      if (j < rounds) {
+    for (int j0 = 0; j0 < RD; j0 += SUB) {
+      float sm = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < GE; e += 2) tm = max3(tm, value(j, e), value(j, e + 1));
+      for (int j = j0; j < j0 + SUB; ++j) {
+        if (j < rounds) {
+#pragma unroll
+          for (int e = 0; e < GE; e += 2) sm = max3(sm, value(j, e), value(j, e + 1));
+        }
+      }
+      tm = fmaxf(tm, sm);
+      if (NW > 1 && k > 0 && j0 < rounds) {
+        folded = fmaxf(folded, sm);
+        s_max[wg_wave][kept][lane] = static_cast<uint16_t>(order_of(folded) >> 16);
+        if (++folds == fold) {
+          folded = -INFINITY;
+          folds = 0;
+          ++kept;
+        }
       }
     }
     const float mn = fmaxf(m, tm);
@@ -265,12 +283,8 @@ __global__ __launch_bounds__(64 * NW * ROWS) void token_logprob_kernel(const Log
         }
       }
     }
-    if (k > 0) {
-      if constexpr (NW > 1) {
-        folded = fmaxf(folded, tm);
-        s_max[wg_wave][tile / fold][lane] = folded;
-        if (++tile % fold == 0) folded = -INFINITY;
-      } else {
+    if constexpr (NW == 1) {
+      if (k > 0) {
         best_bound = max(nth_maximum(k), kNone);
         const float limit = value_of(best_bound);
         uint64_t lanes = __ballot(tm >= limit && tm > -INFINITY);
@@ -309,9 +323,9 @@ __global__ __launch_bounds__(64 * NW * ROWS) void token_logprob_kernel(const Log
   [[maybe_unused]] auto collect = [&](float limit) {
     int n_pair = 0;
     wave_fence();
-    for (int i = 0; i * fold < tile; ++i) {
-      const float x = s_max[wg_wave][i][lane];
-      const bool take = x >= limit && x > -INFINITY;
+    for (int i = 0; i < kept + (folds > 0); ++i) {
+      const uint32_t o = s_max[wg_wave][i][lane];
+      const bool take = o >= best_bound >> 16 && o > kNone >> 16;
       const uint64_t taken = __ballot(take);
       const int to = n_pair + below(taken);
       if (take && to < kPairs) s_pair[wg_wave][to] = static_cast<uint16_t>(i * 64 + lane);
@@ -322,7 +336,7 @@ __global__ __launch_bounds__(64 * NW * ROWS) void token_logprob_kernel(const Log
       if (lane == 0) atomicAdd(count, kList + 1);
       return;
     }
-    const int per = LE * fold, n = n_pair * per;  // element f of the pairs: e = f % per of pair f / per
+    const int per = SUB * GE * fold, n = n_pair * per;  // element f of the pairs: e = f % per of pair f / per
     constexpr int kAhead = 4;
     for (int f0 = 0; f0 < n; f0 += 64 * kAhead) {
       float x[kAhead];
@@ -330,9 +344,9 @@ __global__ __launch_bounds__(64 * NW * ROWS) void token_logprob_kernel(const Log
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
         const int f = min(f0 + 64 * a + lane, n);
-        const int pair = min(f, n - 1) / (fold == 1 ? LE : per), e = f - pair * per;
+        const int pair = min(f, n - 1) / (fold == 1 ? SUB * GE : per), e = f - pair * per;
         const int id = s_pair[wg_wave][pair];
-        const int granule = wave * 64 + (id & 63) + (id / 64 * fold * RD + e / GE) * TH;
+        const int granule = wave * 64 + (id & 63) + (id / 64 * fold * SUB + e / GE) * TH;
         index[a] = granule * GE + e % GE - head;
         x[a] = -INFINITY;
         if (f < n && index[a] >= 0 && index[a] < V) x[a] = element<kWide>(row, index[a]);
