@@ -116,10 +116,10 @@ def test_special_rows(dev, V, k, dtype):
 @pytest.mark.parametrize("V", [1400, 4001, 8194, 20500])
 @pytest.mark.parametrize("k", [0, 4, 32])
 def test_special_rows_among_many(dev, V, k, dtype):
-    """1024 rows or more: one wave each."""
+    """2048 rows or more: one wave each."""
     names, x = special(V, dtype)
     t = torch.full((len(names),), V // 2)
-    times = 1024 // len(names) + 1
+    times = 2048 // len(names) + 1
     res = scoring.token_logprobs(x.to(dev).repeat(times, 1), t.to(dev).repeat(times), k)
     for first in (0, len(names), (times - 1) * len(names)):  # rows of other alignments where V is odd
         for i, name in enumerate(names):
@@ -159,6 +159,15 @@ def test_same_bits_twice_and_under_capture(dev):
         check(y, u, 8, res)
         if seed == 3:
             assert all(torch.equal(a, b) for a, b in zip(vars(res).values(), vars(first).values()))
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.float32, 147457), (torch.float32, 500009), (torch.bfloat16, 294913),
+                                     (torch.bfloat16, 1000003)])
+def test_vocabularies_whose_maxima_are_of_more_than_three_granules(dev, dtype, V):
+    x, tokens = rows(3, V, dtype, V)
+    x[1] = -math.inf
+    x[1, 5::1000] = 1.0
+    check(x.to(dev), tokens.to(dev), 32, scoring.token_logprobs(x.to(dev), tokens.to(dev), top_k=32))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

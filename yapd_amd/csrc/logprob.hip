@@ -7,17 +7,18 @@
 // One pass over a row by one wave or eight: every lane keeps the running maximum and the two
 // sums over its 16-byte granules, a tile of them in registers at a time, rescaled when
 // the maximum grows; they are joined across lanes on DPP and across waves in LDS.
-// What bounds many rows is HBM: 16384 rows of 8194 bf16 with four alternatives 55 us, 4.9 TB/s
+// What bounds many rows is HBM: 16384 rows of 8194 bf16 with four alternatives 53.5 us, 5.0 TB/s
 // (one wave a row: with four, 71, bound by the instructions that every wave runs once);
-// 900 of 100003 fp32 with twenty 76 us, 4.7 TB/s.  64 rows of 8194 take 7.1 us: one
-// wave's chain of load, sums, search for T, second read and ranks.
+// 900 of 100003 fp32 with twenty 73.6 us, 4.9 TB/s (65.3 without alternatives: what a row does once, and
+// the second read).  64 rows of 8194 take 7.0 us: one wave's chain of load, sums, search
+// for T, second read and ranks.
 //
 // The best k: with T the k-th largest lane maximum (found bit by bit with ballots; of
 // several waves' rows a bound below it), at least k elements reach T, and few more.  They sit in
 // the lanes whose maximum reaches T.  A row of one wave has them put their granules into LDS, tile
 // by tile, where the wave looks at one lane's elements at a time.  A row of several waves
-// keeps the maxima of (lane, tile) pairs in LDS, and once T is known those that reach
-// it are read again (they are still in a cache).  What reaches T goes to a list with its
+// keeps the maxima of (lane, three granules) pairs in LDS, and once T is known those that
+// reach it are read again.  What reaches T goes to a list with its
 // index, and each candidate counts the keys above its own: that is its rank.  Rows of many equal
 // logits (a mask's -inf or lowest value among the best k) overflow the list;
 // there one wave walks the row for what lies above T and the first k that equal it.
@@ -31,7 +32,7 @@ namespace {
 
 constexpr int kMaxTop = 32;
 constexpr int kList = 256;    // candidates of a row; (kMaxTop - 1) lanes' granules of 8 and one more fit
-constexpr int kPairs = 256;   // (lane, tile) pairs of a wave that hold them
+constexpr int kPairs = 256;   // (lane, granules) pairs of a wave that hold them
 constexpr uint32_t kNone = 0x007fffffu;  // order_of(-inf)
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
 constexpr float kGone = -200.f;  // 2^kGone is 0 in fp32: a bound for d where d 2^d is 0, also at d = -inf
@@ -164,6 +165,7 @@ __global__ __launch_bounds__(64 * NW * ROWS) void token_logprob_kernel(const Log
   const char* base = row - head * (kWide ? 4 : 2);
   const int n_gran = static_cast<int>((static_cast<int64_t>(V) + head + GE - 1) / GE);
   const int64_t token = P.tokens[item];
+  const float x_token = element<kWide>(row, min(max(token, int64_t{0}), int64_t{V - 1}));  // asked for before the row is
 
   float m = -INFINITY, s = 0.f, t = 0.f;  // of this lane: maximum, sum 2^d, sum d 2^d, d = (x - m) log2(e)
   uint32_t best_bound = kNone;            // order of T
@@ -407,7 +409,7 @@ __global__ __launch_bounds__(64 * NW * ROWS) void token_logprob_kernel(const Log
   const float log_s = (log2_s - left_of(M)) * kLn2;
   if (lane == 0) {
     P.entropy[item] = (log2_s - T / S) * kLn2;
-    P.logprob[item] = token < 0 ? 0.f : token >= V ? NAN : (element<kWide>(row, token) - M) - log_s;
+    P.logprob[item] = token < 0 ? 0.f : token >= V ? NAN : (x_token - M) - log_s;
   }
   if (k == 0) return;
 
@@ -438,7 +440,7 @@ __global__ __launch_bounds__(64 * NW * ROWS) void token_logprob_kernel(const Log
   int64_t* top_token = P.top_token + static_cast<int64_t>(item) * k;
   auto store = [&](int rank, uint64_t key) {
     const int index = static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
-    top_logprob[rank] = (element<kWide>(row, index) - M) - log_s;
+    top_logprob[rank] = (value_of(static_cast<uint32_t>(key >> 32)) - M) - log_s;  // a NaN's is -inf, but then log_s is NaN
     top_token[rank] = index;
   };
   if (n <= kList) {
@@ -474,19 +476,20 @@ void launch(const LogprobParams& P, hipStream_t st) {
                      0, st, P);
 }
 
-// One wave a row where there are rows enough to fill the chip so (four a CU), or
+// One wave a row where there are rows enough to fill the chip so (six a CU), or
 // where a row is little work: what a wave does once (the search for T, the joins) is
 // most of a short tile's work, and no workgroup waits.  Else eight waves a row.
 // Tiles are as long as the row needs, up to 17 granules a lane (five waves a SIMD).
-// us a call, one wave / eight: 64 rows of 8194 bf16 10.2 / 7.1, 512 10.7 / 9.1, 1024 11.2 / 12.9, 2048 15.6 /
-// 21.3; 1024 of 20000 22.2 / 22.8; 512 of 300 4.6 / 6.3.  Rows of more than four such tiles
-// (900 of 100003 fp32: 104 / 76) keep eight waves at any number.
+// us a call, one wave / eight, eight alternatives: 64 rows of 8194 bf16 10.2 / 7.0, 512 10.8 / 8.8, 1024 12.4 / 12.7,
+// 2048 15.6 / 21.1, 16384 57 / 148; 1024 of 20000 22.0 / 18.5, 2048 25.8 / 30.8; 1024 of 16000 fp32 22.8 / 19.7, 4000
+// 53.6 / 58.2; 512 of 300 4.6 / 6.3.  Rows of more than four such tiles keep eight waves at any number: 1024 of 60000
+// 41.1 / 29.7, 3000 75.6 / 75.0.
 template <bool kWide>
 void launch_rows(const LogprobParams& P, hipStream_t st) {
   const int64_t granules = (static_cast<int64_t>(P.vocab) + (kWide ? 3 : 7)) / (kWide ? 4 : 8) + 1;
   if (granules <= 3 * 64) {
     launch<kWide, 1, 4, 3>(P, st);
-  } else if (P.items >= 1024 && granules <= 4 * 17 * 64) {
+  } else if (P.items >= 1536 && granules <= 4 * 17 * 64) {
     if (granules <= 9 * 64)
       launch<kWide, 1, 4, 9>(P, st);
     else
