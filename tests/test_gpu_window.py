@@ -155,6 +155,36 @@ def test_captured_call_follows_the_device_lengths(dev):
         assert torch.equal(out, ref)
 
 
+def test_captured_packed_call_follows_the_device_rows(dev):
+    """One graph of packed prompts, replayed over other partitions of its queries: rows come, go and empty."""
+    H, n_q = 4, 450
+    c = Case(q_lens=[n_q, 0, 0, 0], kv_lens=[700, 700, 700, 700], H=H, window=5000, sinks=0, causal=True, packed=True)
+    t = c.device(dev)
+    pool = torch.randn(t["pool"].shape, generator=torch.Generator().manual_seed(1)).bfloat16().to(dev)
+    table = torch.arange(4 * t["table"].shape[1], dtype=torch.int32, device=dev).view(4, -1) % pool.shape[0]
+    q_start, kv_len = t["q_start"], t["kv_len"]
+    call = lambda o: kernels.attn_window(t["q"], pool, table, kv_len, o, 0.125, window=90, sinks=3,  # noqa: E731
+                                         q_start=q_start)
+    out = torch.empty_like(t["q"])
+    call(out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(out)
+    for starts, lens in (([0, 450, 450, 450, 450], [700, 0, 0, 0]), ([0, 1, 130, 400, 450], [1, 300, 270, 690]),
+                         ([0, 0, 0, 0, 3], [0, 0, 5, 3]), ([7, 140, 140, 140, 440], [133, 9, 9, 301])):
+        q_start.copy_(torch.tensor(starts, dtype=torch.int32))
+        kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(77.0)
+        g.replay()
+        ref = torch.full_like(out, 77.0)
+        call(ref)
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref)
+        assert bool((out[:starts[0]] == 77.0).all()) and bool((out[starts[-1]:] == 77.0).all())
+        assert bool(out[starts[0]:starts[-1]].isfinite().all())
+
+
 def test_two_graphs_with_parts_do_not_share_a_workspace(dev):
     """Captured calls that split over the keys, replayed on two streams at once."""
     cases = [Case(q_lens=[1], kv_lens=[9000 + i], H=4, window=8000, sinks=4, causal=True, seed=i) for i in range(2)]
