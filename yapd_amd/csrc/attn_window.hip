@@ -17,7 +17,7 @@
 //
 // Short tiles are bound by memory: 256 ragged rows of one token on up to 1088 keys
 // x 16 heads 169 us, 5.9 TB/s; three rows on 16384 keys 37.0 us, 5.5 TB/s; 130
-// blocks of 32 on up to 565 keys 61 us, 4.8 TB/s.  One row on 1028 keys takes 8.8 us:
+// blocks of 32 on up to 565 keys 61 us, 4.8 TB/s.  One row on 1028 keys takes 8.2 us:
 // length, page ids and keys are loads that wait for each other, and one CU fetches
 // about 50 GB/s.
 #include <algorithm>
@@ -753,17 +753,17 @@ struct Cut {
 };
 
 // Waves to a head's chunks, by how many (tile, head) pairs there are; us a call with 1, 2 and 4 of them, 16 heads.
-// One token, 804 of 1201 keys: one row 27.2, 16.0, 8.4; 32 rows (512 pairs) 31.0, 21.0, 20.9; 64 rows 36.6, 38.3, 38.3;
-// 256 rows 140.6, 142.9, 142.9.  Blocks of 32: 32 rows 39.0, 24.4, 24.3; 64 rows 41.7, 42.1, 42.4; 128 rows 79.0, 81.7,
-// 87.0, but 130 ragged rows of 100 to 2000 keys 64.7, 59.6, 56.0.  Blocks of 64: 64 rows 54.8, 48.5, 57.8.  One token
-// on 61 keys, 300 rows: 16.7, 17.9, 22.5.  Eight waves: 8.7 at one row, 14.9 against 13.6 for 16 blocks of 32.
+// One token, 804 of 1201 keys: one row 19.3, 11.7, 7.2; 32 rows (512 pairs) 30.5, 20.6, 20.3; 64 rows 37.0, 37.5, 38.0;
+// 256 rows 139.5, 141.7, 144.1.  Blocks of 32: 32 rows 36.1, 22.8, 23.8; 64 rows 39.8, 41.5, 42.4; 128 rows 78.6, 83.0,
+// 87.8, but 130 ragged rows of 100 to 2000 keys 65.7, 58.7, 60.3.  Blocks of 64: 64 rows 55.1, 48.7, 58.1.  One token
+// on 61 keys, 300 rows: 16.5, 19.1, 22.1.
 constexpr int64_t kFour = 512, kTwo = 2560;
 
 // Parts: as many as bring the workgroups to `wanted`, of at least `least` chunks each.  us in one part and as cut here.
-// Waves on short tiles, up to the number of CUs and 8 chunks; one token, 16 heads: 1400 keys 10.2, 8.5; 2000 keys 16.7,
-// 8.7; 4000 keys 28.7, 11.8; 30000 keys 205, 27.5; four rows of 1400 keys 13.5, 10.2; eight of 4000 keys 34.7, 25.5.
-// Below kCutChunks the second launch costs the host (2 us) more than it saves: 1028 keys 8.8, 8.2 in four parts; 804
-// keys 7.6, 8.0.  The tile kernel, which gains until a CU holds three workgroups, and 16 chunks; 200 queries, 16 heads:
+// Waves on short tiles, up to the number of CUs and 8 chunks; one token, 16 heads: 1400 keys 11.5, 8.4; 2000 keys 15.3,
+// 8.9; 4000 keys 27.2, 11.3; 30000 keys 207, 27.6; four rows of 1400 keys 13.1, 9.8; eight of 4000 keys 35.0, 25.4.
+// Below kCutChunks the second launch costs the host (2 us) more than it saves: 1028 keys 9.0, 8.2 in four parts; 804
+// keys 7.6, 7.6.  The tile kernel, which gains until a CU holds three workgroups, and 16 chunks; 200 queries, 16 heads:
 // 1400 keys 24, 17.9; 4200 keys 64, 21.3 (parts of 8 chunks 24.4); 1300 on 9300 keys 132, 76 (to two a CU 91).
 constexpr int64_t kCutChunks = 40;
 
