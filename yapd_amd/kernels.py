@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from array import array
 from pathlib import Path
 from typing import Optional
 
@@ -383,14 +384,17 @@ def attn_window(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len
         with torch.cuda.device(dev):  # the launch goes to the current device
             return attn_window(q, pool, table, kv_len, out, scale, window=window, sinks=sinks, causal=causal,
                                q_start=q_start, max_q=max_q, max_kv=max_kv, workspace=workspace)
-    require_cuda(q, "q", torch.bfloat16, dev, contiguous=False)
+    bf16, i32 = torch.bfloat16, torch.int32
+    require_cuda(q, "q", bf16, dev, contiguous=False)
+    # sizes and strides are asked for once: a single token's call is host time
     shape, stride = q.shape, q.stride()
+    dims = len(shape)
+    require((dims >= 2 and stride[-1] == 1 and stride[-2] == 64) or q.numel() == 0, "q's heads must be packed")
     packed = q_start is not None
-    require(q.numel() == 0 or (stride[-1] == 1 and len(shape) >= 2 and stride[-2] == 64), "q's heads must be packed")
     if packed:
-        require(len(shape) == 3 and shape[2] == 64, "packed q must be [n_q, H, 64]")
+        require(dims == 3 and shape[2] == 64, "packed q must be [n_q, H, 64]")
         n_q, H, _ = shape
-        require_cuda(q_start, "q_start", torch.int32, dev)
+        require_cuda(q_start, "q_start", i32, dev)
         rows = q_start.numel() - 1
         require(rows >= 0, "q_start must be [rows + 1]")
         if max_q is None:
@@ -398,28 +402,30 @@ def attn_window(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len
         require(n_q == 0 or rows == 0 or max_q >= 1, "max_q must be >= 1")
         tok = stride[0] if n_q > 1 else H * 64
     else:
-        require(len(shape) == 4 and shape[3] == 64, "q must be [rows, bl, H, 64] (or [n_q, H, 64] with q_start)")
+        require(dims == 4 and shape[3] == 64, "q must be [rows, bl, H, 64] (or [n_q, H, 64] with q_start)")
         rows, bl, H, _ = shape
         n_q = rows * bl
         require(max_q is None or max_q == bl, "max_q is given by q's shape unless q is packed")
         max_q = bl
         tok = stride[1] if bl > 1 else stride[0] if rows > 1 else H * 64
-        require(rows <= 1 or stride[0] == bl * tok, "q's rows must follow each other")
-    require_cuda(pool, "pool", torch.bfloat16, dev)
-    if not (pool.dim() == 4 and pool.shape[1] == 2 and pool.shape[2] == H and pool.shape[3] == 1024):
+        require(rows <= 1 or stride[0] == bl * tok or n_q == 0, "q's rows must follow each other")
+    require_cuda(pool, "pool", bf16, dev)
+    pool_shape = pool.shape
+    if pool_shape[1:] != (2, H, 1024):
         raise ValueError("pool must be [pages, 2, H, 16*64]")
-    require_cuda(table, "table", torch.int32, dev, contiguous=False)
-    require(table.dim() == 2 and table.shape[0] >= rows and (table.shape[1] == 1 or table.stride(1) == 1),
+    require_cuda(table, "table", i32, dev, contiguous=False)
+    table_shape, table_stride = table.shape, table.stride()
+    require(len(table_shape) == 2 and table_shape[0] >= rows and (table_shape[1] == 1 or table_stride[1] == 1),
             "table must be [>= rows, max_pages] with unit column stride")
-    require(rows <= 1 or table.stride(0) >= table.shape[1], "table rows must not overlap")
-    require_cuda(kv_len, "kv_len", torch.int32, dev)
+    cols, pitch = table_shape[1], table_stride[0]
+    require(rows <= 1 or pitch >= cols, "table rows must not overlap")
+    require_cuda(kv_len, "kv_len", i32, dev)
     require(kv_len.numel() >= rows, "kv_len must have rows entries")
-    require_cuda(out, "out", torch.bfloat16, dev)
+    require_cuda(out, "out", bf16, dev)
     require(out.shape == shape, "out must match q")
     require(window >= 1 and sinks >= 0, "need window >= 1 and sinks >= 0")
     if n_q == 0 or rows == 0:
         return
-    cols = table.shape[1]
     require(cols >= 1, "the table maps no page")
     window, sinks = min(int(window), WINDOW_CAP), min(int(sinks), WINDOW_CAP)
     kv_max = cols * 16 if max_kv is None else min(int(max_kv), cols * 16)
@@ -432,7 +438,7 @@ def attn_window(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len
     if workspace is not None:
         require_cuda(workspace, "workspace", torch.float32, dev)
     check(lib.yapd_attn_window(
-        q.data_ptr(), tok, pool.data_ptr(), pool.shape[0], table.data_ptr(), max(table.stride(0), cols), cols,
+        q.data_ptr(), tok, pool.data_ptr(), pool_shape[0], table.data_ptr(), max(pitch, cols), cols,
         kv_len.data_ptr(), ptr(q_start), rows, max_q, n_q, H, window, sinks, causal, kv_max, scale, ptr(workspace),
         0 if workspace is None else workspace.numel(), out.data_ptr(), stream_ptr(dev)))
 
@@ -475,15 +481,16 @@ def pool_pointers(pools):
     """The device addresses of every layer's pool, and the pools' common shape and device, checked."""
     require(len(pools) >= 1, "no pools")
     shape, dev, bf16 = pools[0].shape, pools[0].device, torch.bfloat16
+    index = pools[0].get_device()
     ptrs = []
     for p in pools:
-        if p.dtype is not bf16 or p.shape != shape or p.device != dev or not p.is_contiguous():
+        if p.dtype is not bf16 or p.shape != shape or p.get_device() != index or not p.is_contiguous():
             require_cuda(p, "pool", bf16, dev)
             raise ValueError("every layer's pool must have the same shape")
         ptrs.append(p.data_ptr())
     require_cuda(pools[0], "pool", bf16, dev)
     require(len(shape) == 4 and shape[0] >= 1 and shape[1] == 2 and shape[3] == 1024, "pools must be [pages, 2, H, 16*64]")
-    return (c_void * len(ptrs))(*ptrs), shape, dev
+    return array("Q", ptrs), shape, dev
 
 
 def page_ids(ids, name: str):
@@ -514,8 +521,8 @@ def kv_copy_pages(pools, src, dst) -> None:
             return kv_copy_pages(pools, src, dst)
     src, dst = page_ids(src, "src"), page_ids(dst, "dst")
     require(src.size == dst.size, "src and dst must have the same length")
-    check(load_library().yapd_kv_copy_pages(ptrs, len(ptrs), shape[0], shape[2], src.ctypes.data, dst.ctypes.data,
-                                            src.size, stream_ptr(dev)))
+    check(load_library().yapd_kv_copy_pages(ptrs.buffer_info()[0], len(ptrs), shape[0], shape[2], src.ctypes.data,
+                                            dst.ctypes.data, src.size, stream_ptr(dev)))
 
 
 # --------------------------------------------------------------------------- #

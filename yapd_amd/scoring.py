@@ -85,7 +85,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
         with torch.cuda.device(dev):  # the launch goes to the current device
             return token_logprobs(logits, tokens, top_k)
     kernels.check_token_logprobs(logits, tokens)
-    logprob = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    logprob = torch.empty_like(tokens, dtype=torch.float32)
     entropy = torch.empty_like(logprob)
     top_logprob = top_token = None
     if top_k:
