@@ -1,0 +1,72 @@
+"""GPU: windowed attention where every weight is known exactly: large scores beside rising ones."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import window as OW
+from yapd_amd import kernels
+
+pytestmark = pytest.mark.gpu
+H = 4
+LOG2E = np.float32(1.4426950408889634)
+
+
+def paged(K, V):
+    """Dense ``K, V [rows, kv, H, 64]`` (kv a multiple of 16) as a pool and its table."""
+    rows, kv = K.shape[:2]
+    n = rows * kv // 16
+    pool = torch.empty(n, 2, H, 1024, dtype=torch.bfloat16, device=K.device)
+    pool[:, 0] = K.reshape(n, 16, H, 64).permute(0, 2, 1, 3).reshape(n, H, 1024)
+    pool[:, 1] = V.reshape(n, 16, H, 64).permute(0, 2, 3, 1).reshape(n, H, 1024)
+    return pool, torch.arange(n, dtype=torch.int32, device=K.device).view(rows, kv // 16)
+
+
+def attend(q, K, V, kv, **kw):
+    pool, table = paged(K, V)
+    out = torch.full_like(q, 77.0)
+    kv_len = torch.tensor(kv, dtype=torch.int32, device=q.device)
+    kernels.attn_window(q, pool, table, kv_len, out, 0.125, **kw)
+    torch.cuda.synchronize()
+    return out
+
+
+def worst_residual(near, scale=0.125):
+    """The bf16 value within a factor of two above ``near`` whose product with scale * log2(e) is rounded the most."""
+    e = np.float32(2.0 ** np.floor(np.log2(near)))
+    a = e * (1 + np.arange(128, dtype=np.float32) / 128)
+    c = np.float32(scale) * LOG2E
+    off = np.abs(np.float64(a * c) - np.float64(a) * np.float64(c))
+    return float(a[off.argmax()])
+
+
+@pytest.mark.parametrize("parts", [1, 2])
+@pytest.mark.parametrize("q_n", [40, 100])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("score", [100, 1000, 2**13, 10**5, 2**20, 2**29])
+def test_equal_scores_beside_rising_ones(dev, score, sign, q_n, parts):
+    """Query 0's scores are all ``score``; the others' rise by 8 with every 64 keys, so their maxima keep moving.
+    V names its keys' 64: query 0 gives 1/64 for each.  In tiles of 128 that is exact: its weights are one bf16 number w,
+    their sum 4096 w and each product's 64 w need at most 20 bits, and what remains, 1 / (4096 w) times 64 w, is off by a
+    few 2^-24, far below half a step of the result's bf16.  Up to 64 queries the sum is of the weights before their
+    rounding to bf16: half a step of theirs, and half a step of the result."""
+    kv = 64 * 64
+    q = torch.zeros(1, q_n, H, 64)
+    q[0, 0, :, 0] = sign * worst_residual(score / 0.125)
+    q[0, 1:, :, 1] = 64.0
+    K, V = torch.zeros(1, kv, H, 64), torch.zeros(1, kv, H, 64)
+    chunk = torch.arange(kv) // 64
+    K[..., 0] = 1.0
+    K[0, :, :, 1] = chunk[:, None].float()
+    V[0, torch.arange(kv), :, chunk] = 1.0
+    q, K, V = (x.bfloat16().to(dev) for x in (q, K, V))
+    lib = kernels.load_library()
+    # the host's bound of the length only decides how the work is cut
+    max_kv = 1 if parts == 1 else kv
+    assert (lib.yapd_attn_window_workspace(1, q_n, q_n, 0, H, 2 * kv, 0, max_kv) > 0) == (parts > 1)
+    out = attend(q, K, V, [kv], window=2 * kv, causal=False, max_kv=max_kv).cpu()
+    off = (out[0, 0].double() * 64 - 1).abs().max().item()
+    assert off <= (0.0 if q_n > 64 else 2 * 2.0 ** -8 + 1e-4), off
+    # the rising ones: half a step of the result's bf16 and of the weights', whose scores of up to 727 are off by 2^-24 of that
+    want, a = OW.attend(q[0, 1:2].cpu(), K[0].cpu(), V[0].cpu(), 2 * kv, 0, False, 0.125)
+    assert bool(((out[0, 1:].double() - want).abs() <= (2 * 2.0 ** -8 + 1e-4) * a + 1e-6).all())

@@ -454,6 +454,12 @@ __device__ __forceinline__ bool find_weighed_tile(const WindowParams& P, int slo
   return true;
 }
 
+// A product that is rounded wherever it is used: never fused into a sum.
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void attn_window_tile_kernel(const WindowParams P) {
   // dynamic: only the direct loads write it, which the compiler does not see as writes of a static array
   extern __shared__ __attribute__((aligned(16))) char ring[];
@@ -648,11 +654,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void a
       __builtin_amdgcn_s_setprio(0);
     }
     if (!moved) break;  // the last chunk is done
-    mn = fmaxf(m, mn);
-    // no key seen yet: exponents against 0 give alpha = 0 and p = 0 instead of NaN
-    mref = mn == -INFINITY ? 0.f : mn * P.scale_log2;
-    const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, P.scale_log2, -mref));
-    m = mn;
+    // The factor is taken between the references as the exponents had them: exactly 1 for a query whose maximum stays,
+    // however often others move.  A first maximum's is of sums that are 0: held to 1, it cannot be infinite.
+    const bool mine = mn > m;
+    const float to = mine ? rounded_product(mn, P.scale_log2) : mref;
+    const float alpha = __builtin_amdgcn_exp2f(fminf(mref - to, 0.f));
+    m = mine ? mn : m;
+    mref = to;
     l *= alpha;
     o[0] *= alpha;
     o[1] *= alpha;
