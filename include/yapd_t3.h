@@ -192,7 +192,7 @@ int yapd_attn_paged_block_noalloc(const void* q, const void* kv_pool, int64_t n_
  * The work is cut by sizes the host knows and the device lengths alone, so
  * a captured launch follows kv_len and q_start from replay to replay.  How
  * it is cut (and with it the order of a query's sums) depends on the call's
- * sizes.  With few queries over many keys the keys are cut into parts joined
+ * sizes and its rows' lengths, never on the other queries' values.  With few queries over many keys the keys are cut into parts joined
  * by a second launch: workspace then holds yapd_attn_window_workspace() floats
  * (0: not needed, may be NULL), 16-byte aligned, not shared by calls that may
  * overlap.  window >= 1, sinks >= 0, H a multiple of 4, 1e-30 <= scale <= 1e30

@@ -1,4 +1,5 @@
-"""GPU: windowed attention where every weight is known exactly: large scores beside rising ones."""
+"""GPU: windowed attention where every weight is known exactly: large scores beside rising ones, and
+outputs that do not depend on other queries' values."""
 
 import numpy as np
 import pytest
@@ -70,3 +71,19 @@ def test_equal_scores_beside_rising_ones(dev, score, sign, q_n, parts):
     # the rising ones: half a step of the result's bf16 and of the weights', whose scores of up to 727 are off by 2^-24 of that
     want, a = OW.attend(q[0, 1:2].cpu(), K[0].cpu(), V[0].cpu(), 2 * kv, 0, False, 0.125)
     assert bool(((out[0, 1:].double() - want).abs() <= (2 * 2.0 ** -8 + 1e-4) * a + 1e-6).all())
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("q_n,kv,window", [(30, 320, 100), (64, 640, 1000), (198, 1008, 1000), (198, 1008, 300), (700, 1504, 2000)])
+def test_a_query_does_not_depend_on_the_others_values(dev, q_n, kv, window, causal):
+    """Half of a row's queries get other values, far larger ones: the bits of the rest stay."""
+    g = torch.Generator().manual_seed(q_n)
+    K, V = (torch.randn(2, kv, H, 64, generator=g).bfloat16().to(dev) for _ in range(2))
+    q = 2 * torch.randn(2, q_n, H, 64, generator=g)
+    kw = dict(window=window, sinks=5, causal=causal)
+    first = attend(q.bfloat16().to(dev), K, V, [kv, kv - 9], **kw)
+    for factor in (0.0, 4.0, 20.0):
+        other = q.clone()
+        other[:, 1::2] = factor * torch.randn(2, q_n // 2, H, 64, generator=g)
+        out = attend(other.bfloat16().to(dev), K, V, [kv, kv - 9], **kw)
+        assert torch.equal(out[:, ::2], first[:, ::2])

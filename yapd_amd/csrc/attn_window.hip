@@ -654,9 +654,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void a
       __builtin_amdgcn_s_setprio(0);
     }
     if (!moved) break;  // the last chunk is done
-    // The factor is taken between the references as the exponents had them: exactly 1 for a query whose maximum stays,
-    // however often others move.  A first maximum's is of sums that are 0: held to 1, it cannot be infinite.
-    const bool mine = mn > m;
+    // Of the wave's queries those move that have left their own maximum that far, so a query's sums depend on its own
+    // scores alone.  The factor is taken between the references as the exponents had them: exactly 1 for a query that
+    // stays, however often others move.  A first maximum's is of sums that are 0: held to 1, it cannot be infinite.
+    const bool mine = mn > m + slack;
     const float to = mine ? rounded_product(mn, P.scale_log2) : mref;
     const float alpha = __builtin_amdgcn_exp2f(fminf(mref - to, 0.f));
     m = mine ? mn : m;
