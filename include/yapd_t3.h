@@ -181,8 +181,9 @@ int yapd_attn_paged_block_noalloc(const void* q, const void* kv_pool, int64_t n_
  *   64], which must not overlap q or the pool.  q_start NULL: row r's queries
  *   are tokens r * max_q .. (n_q = rows * max_q).  q_start (device int32
  *   [rows + 1], not decreasing): row r's are tokens [q_start[r],
- *   q_start[r+1]), at most max_q of them (further ones are left out); a row may
- *   have none; output rows of no row's are not written.
+ *   q_start[r+1]) (held to [0, n_q]).  At most max_q of them have an output:
+ *   further ones keep their positions, but their output rows are not written, as
+ *   output rows of no row's are not.  A row may have none.
  *   kv_len (device int32 [rows]) counts the row's keys, its queries' own
  *   included; it is clamped to 16 * table_cols.  Pages wholly outside the keys
  *   seen are never read into a result: their table entries may be anything.

@@ -1,6 +1,6 @@
 // Paged-KV attention with a sliding window and sink tokens.
 //
-// Query i of row r stands at position p = kv_len[r] - n_q(r) + i and sees key
+// Query i of row r stands at position p = kv_len[r] - n(r) + i and sees key
 // j iff  j < hi  and  (j < sinks  or  j > p - window),  hi = p + 1 (causal) or
 // kv_len[r] (block: the later positions of its own block too):
 //   out = sum_j softmax_j(scale q . k_j) v_j   over the visible j.
@@ -66,31 +66,32 @@ __device__ __forceinline__ int first_query(const WindowParams& P, int r) {
 // is found by a 64-way search.  false: the slot holds no query.
 template <int TQ>
 __device__ __forceinline__ bool find_tile(const WindowParams& P, int slot, int lane, Tile& t) {
-  int first;
+  int first, n;  // n: the row's queries, also those past max_q, which have positions but no tile
   if (P.q_start == nullptr) {
     const int per = (P.max_q + TQ - 1) / TQ;
     t.row = slot / per;
     t.qs = t.row * P.max_q;
-    t.qc = P.max_q;
+    n = P.max_q;
     first = (slot - t.row * per) * TQ;
   } else {
-    int base = 0, n = P.rows;
-    while (n > 1) {
-      const int step = (n + 63) / 64;
+    int base = 0, left = P.rows;
+    while (left > 1) {
+      const int step = (left + 63) / 64;
       const int i = lane * step;
-      const bool le = i < n && first_query(P, base + min(i, n - 1)) / TQ + base + i <= slot;
+      const bool le = i < left && first_query(P, base + min(i, left - 1)) / TQ + base + i <= slot;
       const int at = (max(__popcll(__ballot(le)), 1) - 1) * step;
       base += at;
-      n = min(step, n - at);
+      left = min(step, left - at);
     }
     t.row = base;
     t.qs = first_query(P, base);
-    t.qc = min(max(first_query(P, base + 1) - t.qs, 0), P.max_q);
+    n = max(first_query(P, base + 1) - t.qs, 0);
     first = (slot - t.qs / TQ - base) * TQ;
   }
+  t.qc = min(n, P.max_q);
   if (first < 0 || first >= t.qc) return false;
   t.kvl = min(max(P.kv_len[t.row], 0), P.table_cols * kPageSize);
-  t.p0 = t.kvl - t.qc + first;
+  t.p0 = t.kvl - n + first;
   t.qs += first;
   t.qc = min(TQ, t.qc - first);
   return true;
@@ -419,8 +420,9 @@ __device__ __forceinline__ bool find_weighed_tile(const WindowParams& P, int slo
   const int r = min(lane, P.rows - 1);
   const int qs = first_query(P, r), qe = first_query(P, r + 1);
   const int len = min(max(P.kv_len[r], 0), P.table_cols * kPageSize);
-  const int n = lane < P.rows ? min(max(qe - qs, 0), P.max_q) : 0;
-  const int tiles = (n + kTileQ - 1) / kTileQ, before = max(len - n, 0) / kTileQ;
+  const int n = lane < P.rows ? max(qe - qs, 0) : 0;  // also those past max_q, which have positions but no tile
+  const int n_tiled = min(n, P.max_q);
+  const int tiles = (n_tiled + kTileQ - 1) / kTileQ, before = max(len - n, 0) / kTileQ;
   const auto add = [](int a, int b) { return a + b; };
   const auto larger = [](int a, int b) { return max(a, b); };
   const int top = wave_reduce(tiles > 0 ? min(tiles - 1 + before, (P.window + kTileQ - 1) / kTileQ) : 0, larger);
@@ -447,10 +449,9 @@ __device__ __forceinline__ bool find_weighed_tile(const WindowParams& P, int slo
   const int first = __builtin_amdgcn_readlane(k0 + m - sum, at) + slot - above;
   t.row = at;
   t.kvl = __builtin_amdgcn_readlane(len, at);
-  const int qc = __builtin_amdgcn_readlane(n, at);
-  t.p0 = t.kvl - qc + first * kTileQ;
+  t.p0 = t.kvl - __builtin_amdgcn_readlane(n, at) + first * kTileQ;
   t.qs = __builtin_amdgcn_readlane(qs, at) + first * kTileQ;
-  t.qc = min(kTileQ, qc - first * kTileQ);
+  t.qc = min(kTileQ, __builtin_amdgcn_readlane(n_tiled, at) - first * kTileQ);
   return true;
 }
 

@@ -369,8 +369,8 @@ def attn_window(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len
     ``j`` iff ``j < hi`` and (``j < sinks`` or ``j > p - window``), with ``hi = p + 1`` (``causal``) or
     ``kv_len`` (a block step).  Queries are ``[rows, bl, H, 64]``, or packed ``[n_q, H, 64]`` with the
     device ``q_start [rows + 1]`` (int32, not decreasing): row ``r`` has rows ``q_start[r]`` up to
-    ``q_start[r + 1]`` of ``q`` and ``out``, at most ``max_q`` of them; rows of ``out`` that belong to no
-    row are left as they were.  ``q`` may be a view with packed heads and any token stride (a slice of
+    ``q_start[r + 1]`` of ``q`` and ``out``; of more than ``max_q`` the first ``max_q`` are computed, at the positions
+    that the whole row gives them.  Rows of ``out`` that are not computed or belong to no row are left as they were.  ``q`` may be a view with packed heads and any token stride (a slice of
     a fused QKV buffer); ``out`` is contiguous and must not overlap ``q``.
 
     Lengths are read on the device: no plan, and a captured call follows them.  ``max_q`` and
