@@ -84,7 +84,12 @@ __device__ __forceinline__ uint64_t key_of(float x, int index) {
 // what the rounding left out.  That is small while |m| is; beyond kHuge (far from
 // any model's logits, but a mask may hold the type's lowest value) the exponent
 // is (x - m) L.  0 where nothing is above -inf yet: sums of 0, not NaN.
-__device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.f : __fmul_rn(m, kLog2e); }
+// The shift is never fused into a sum (as __fmul_rn may be): the sums of an unchanged maximum
+// would be scaled by what its rounding leaves out, tile by tile.
+__device__ __forceinline__ float shift_of(float m) {
+#pragma clang fp contract(off)
+  return m == -INFINITY ? 0.f : m * kLog2e;
+}
 __device__ __forceinline__ float left_of(float m) {
   return fabsf(m) > kHuge ? 0.f : __builtin_fmaf(m, kLog2e, -shift_of(m));
 }
