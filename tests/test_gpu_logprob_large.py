@@ -44,3 +44,19 @@ def test_equal_logits(dev, n, V, dtype, near, sign):
             off = (got.cpu().double() - want).abs().max().item()
             assert off <= (bound + 2.0 ** -24 * want.abs().max()).item(), (i, off, bound.item())
         assert torch.equal(res.top_token[i].cpu(), top[0])
+
+
+@pytest.mark.parametrize("n", [2, 1600])
+def test_terms_lost_beside_a_large_one(dev, n):
+    """Terms just below half a step of 1: a lane that holds the 1 first adds none of its other V / 64 terms."""
+    V = 34800  # 4350 granules: one wave a row from 1536 rows on
+    x = torch.full((1, V), -16.75, dtype=torch.bfloat16)
+    x[0, 0] = 0.0
+    t = torch.tensor([0])
+    res = scoring.token_logprobs(x.repeat(n, 1).to(dev), t.repeat(n).to(dev), 1)
+    lp, ent, top_lp, top = OL.token_logprobs(x, t, 1)
+    tol, tol_e = OL.tolerances(x, ent)
+    off = (res.logprob.cpu().double() - lp).abs().max().item()
+    print(f"off by {off * 2 ** 24:.0f} of {tol.item() * 2 ** 24:.0f} half steps")
+    assert off <= tol.item() and (res.entropy.cpu().double() - ent).abs().max().item() <= tol_e.item()
+    assert (res.top_logprob.cpu().double() - top_lp).abs().max().item() <= tol.item() and bool((res.top_token == 0).all())
