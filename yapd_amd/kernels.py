@@ -508,6 +508,16 @@ def page_ids(ids, name: str):
     return np.ascontiguousarray(a)
 
 
+def check_page_pairs(src, dst, n_pages: int) -> None:
+    """What ``yapd_kv_copy_pages`` refuses of page ids, for pools on the CPU."""
+    import numpy as np
+    require(src.size == dst.size, "src and dst must have the same length")
+    both = np.concatenate([src, dst])
+    require(not both.size or (both.min() >= 0 and both.max() < n_pages), f"pairs outside the pool's {n_pages} pages")
+    require(np.unique(dst).size == dst.size, "a page is the destination of two pairs")
+    require(not np.intersect1d(src, dst).size, "a page is a source and a destination")
+
+
 def kv_copy_pages(pools, src, dst) -> None:
     """``pool[dst[i]] = pool[src[i]]`` for every pair ``i`` in every layer's pool of ``pools``, in one
     launch (per 64 layers and 384 pairs).

@@ -90,13 +90,17 @@ class PagedKV:
 
     def copy_pages(self, src, dst) -> None:
         """``pool[dst[i]] = pool[src[i]]`` in every layer's pool for host page ids (see
-        :func:`kernels.kv_copy_pages`), on the current stream; torch's index operations on the CPU."""
+        :func:`kernels.kv_copy_pages`), on the current stream; torch's index operations, with the same
+        refusals, on the CPU."""
         if self.device.type == "cuda":
             kernels.kv_copy_pages(self.pools, src, dst)
             return
-        src, dst = (torch.as_tensor(np.asarray(x, dtype=np.int64)) for x in (src, dst))
+        src, dst = kernels.page_ids(src, "src"), kernels.page_ids(dst, "dst")
         for pool in self.pools:
-            pool.index_copy_(0, dst, pool.index_select(0, src))
+            kernels.check_page_pairs(src, dst, pool.shape[0])
+        src_t, dst_t = (torch.from_numpy(x.astype(np.int64)) for x in (src, dst))
+        for pool in self.pools:
+            pool.index_copy_(0, dst_t, pool.index_select(0, src_t))
 
     def copy_row_pages(self, src_row: int, dst_row: int, n_positions: int) -> None:
         """Copy the pages holding positions ``[0, n_positions)`` of one row to another, every layer."""
