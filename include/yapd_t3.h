@@ -178,7 +178,7 @@ int yapd_attn_paged_block_noalloc(const void* q, const void* kv_pool, int64_t n_
  * later positions too).  out = softmax(q K^T * scale) V over the keys seen; a
  * query that sees none gets zeros.  It has no counterpart in the reference.
  *   q: bf16, token t's head h at t * q_tok_stride + h * 64; out: bf16 [n_q, H,
- *   64], which must not overlap q or the pool.  q_start NULL: row r's queries
+ *   64]; one that shares memory with q's heads or the pool is refused.  q_start NULL: row r's queries
  *   are tokens r * max_q .. (n_q = rows * max_q).  q_start (device int32
  *   [rows + 1], not decreasing): row r's are tokens [q_start[r],
  *   q_start[r+1]) (held to [0, n_q]).  At most max_q of them have an output:

@@ -809,6 +809,13 @@ void launch_tiles(const WindowParams& P, const Cut& c, hipStream_t st) {
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether any of n blocks of `bytes`, `pitch` >= bytes apart from a on, shares a byte with [b, b + b_bytes).
+bool overlap(const void* a, int64_t n, int64_t pitch, int64_t bytes, const void* b, int64_t b_bytes) {
+  const int64_t from = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b)) - static_cast<int64_t>(reinterpret_cast<uintptr_t>(a));
+  const int64_t first = from < bytes ? 0 : (from - bytes) / pitch + 1;  // the first block that ends behind b
+  return first < n && first * pitch < from + b_bytes;
+}
+
 int window_checks(int rows, int max_q, int n_q, int n_heads, int window, int sinks, int max_kv) {
   YAPD_REQUIRE(rows >= 1 && max_q >= 1 && n_q >= 1, "attn_window: need rows, max_q and n_q >= 1 (got %d, %d, %d)", rows,
                max_q, n_q);
@@ -853,6 +860,10 @@ extern "C" int yapd_attn_window(const void* q, int64_t q_tok_stride, const void*
                                 workspace_floats >= tokens * (yapd::kHeadDim + 2)),
                "attn_window: the workspace must be 16-byte aligned and hold %lld floats",
                static_cast<long long>(tokens * (yapd::kHeadDim + 2)));
+  const int64_t out_bytes = static_cast<int64_t>(n_q) * n_heads * yapd::kHeadDim * 2;
+  YAPD_REQUIRE(!yapd::overlap(q, n_q, q_tok_stride * 2, out_bytes / n_q, out, out_bytes), "attn_window: out overlaps q");
+  const int64_t pool_bytes = n_pages * 2 * n_heads * yapd::kHeadTile * 2;
+  YAPD_REQUIRE(!yapd::overlap(kv_pool, 1, pool_bytes, pool_bytes, out, out_bytes), "attn_window: out overlaps the pool");
   yapd::WindowParams P;
   P.q = static_cast<const uint16_t*>(q);
   P.q_stride = q_tok_stride;

@@ -371,7 +371,7 @@ def attn_window(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len
     device ``q_start [rows + 1]`` (int32, not decreasing): row ``r`` has rows ``q_start[r]`` up to
     ``q_start[r + 1]`` of ``q`` and ``out``; of more than ``max_q`` the first ``max_q`` are computed, at the positions
     that the whole row gives them.  Rows of ``out`` that are not computed or belong to no row are left as they were.  ``q`` may be a view with packed heads and any token stride (a slice of
-    a fused QKV buffer); ``out`` is contiguous and must not overlap ``q``.
+    a fused QKV buffer); ``out`` is contiguous; one that shares memory with ``q`` or the pool is refused.
 
     Lengths are read on the device: no plan, and a captured call follows them.  ``max_q`` and
     ``max_kv`` are the host's upper bounds (default: all queries, all positions the table maps).
