@@ -1,5 +1,5 @@
-"""GPU: windowed attention where every weight is known exactly: large scores beside rising ones, and
-outputs that do not depend on other queries' values."""
+"""GPU: windowed attention where every weight is known exactly: large scores beside rising ones, every key of a wide
+window counted; and outputs that do not depend on other queries' values."""
 
 import numpy as np
 import pytest
@@ -87,3 +87,35 @@ def test_a_query_does_not_depend_on_the_others_values(dev, q_n, kv, window, caus
         other[:, 1::2] = factor * torch.randn(2, q_n // 2, H, 64, generator=g)
         out = attend(other.bfloat16().to(dev), K, V, [kv, kv - 9], **kw)
         assert torch.equal(out[:, ::2], first[:, ::2])
+
+
+# (q per row, kv lengths, window, sinks, max_kv): short tiles on four, two and one wave, with parts, tiles of 128 with and without
+WIDE = [
+    (1, [4000, 1001], 3000, 33, None), (1, [2000] * 250, 1100, 7, None), (1, [1600] * 700, 1500, 0, None),
+    (1, [8000], 7000, 64, 8000), (16, [3000, 500], 2500, 4, 1), (33, [2000] * 3, 900, 17, None), (64, [1500] * 20, 1333, 0, None),
+    (64, [6000], 5000, 16, 6000), (100, [3000, 777], 2900, 40, 1), (128, [2049, 128], 1999, 100, 1), (300, [6400], 6000, 9, 6400),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("q_n,kv,window,sinks,max_kv", WIDE)
+def test_every_key_of_a_wide_window_counts_once(dev, q_n, kv, window, sinks, max_kv, causal):
+    """Queries of 0: every visible key weighs the same, exactly 1 before the division.  V names its key's number modulo 64, or its
+    64, so an output is a count over N: whole numbers below 2^24, a division off by a few 2^-24 and one rounding to bf16,
+    2^-8 of it.  A count is 129 at most here: a key lost or twice there is more."""
+    rows, cap = len(kv), (max(kv) + 15) // 16 * 16
+    q = torch.zeros(rows, q_n, H, 64, dtype=torch.bfloat16, device=dev)
+    j = torch.arange(cap)
+    K = torch.randn(1, cap, 1, 64, generator=torch.Generator().manual_seed(0)).bfloat16()
+    for name in (j % 64, j // 64 % 64):
+        V = torch.nn.functional.one_hot(name, 64).to(torch.bfloat16).view(1, cap, 1, 64)
+        Kd, Vd = (x.to(dev).expand(rows, cap, H, 64) for x in (K, V))
+        out = attend(q, Kd, Vd, kv, window=window, sinks=sinks, causal=causal, max_kv=max_kv).cpu().double()
+        for r in {kv[i]: i for i in range(rows)}.values():  # one of each length
+            see = OW.visible(kv[r], q_n, window, sinks, causal).double()
+            count = see @ V[0, :kv[r], 0].double()
+            assert count.max() <= 129
+            want = (count / see.sum(1, keepdim=True))[:, None, :].expand(q_n, H, 64)
+            assert bool(((out[r] - want).abs() <= want * (2.0 ** -8 + 1e-6)).all()), (r, name[1].item())
+        for r in range(rows):
+            assert torch.equal(out[r], out[kv.index(kv[r])])
