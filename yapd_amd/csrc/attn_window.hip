@@ -376,15 +376,17 @@ attn_window_kernel(const WindowParams P) {
 // K rows are permuted so that those are 8 consecutive keys per 16, the operand
 // of O^T += V^T P^T, and 8 consecutive bf16 of a V^T row of a page.
 //
-// Bound by issue: a wave's 32 x 64 scores are 123 vector instructions (64 of
-// them the exponentials and their arguments) beside 16 products that hold the
-// vector unit for part of their 32 cycles each; four workgroups a CU run at
-// 1.9 GHz, where the card holds its power.  8000 queries x 16 heads on a window
-// of 2048: 91 us, 0.74 PF/s; without the products 61, without the exponentials
-// 79.  A third or fourth stage gains 2 to 4 % where workgroups are few and costs
-// a workgroup of a CU where they are many (100 us); one workgroup a CU takes 1 us
-// a chunk.  From 65 queries on: 16 rows of 80 x 16 heads 27.4 us, in tiles of 64
-// on single waves 38.9; 64 rows of 64 there 48.4, here 54.0.
+// Bound by neither unit alone but by how little of the two overlaps: a wave's
+// 32 x 64 scores are 123 vector instructions (64 of them the exponentials and
+// their arguments) and 16 products, and within a wave the products with K, the
+// softmax and the products with V follow each other; only waves that drift apart
+// run one beside another.  8000 queries x 16 heads on a window of 2048: 92 us,
+// 0.73 PF/s, at 1.9 GHz; without the products 61, without the exponentials 79; the
+// vector unit issues in 44 % of the cycles, the matrix unit is busy in 28 %.  A
+// third or fourth stage gains 2 to 4 % where workgroups are few and costs a
+// workgroup of a CU where they are many (100 us); one workgroup a CU takes 1 us a
+// chunk, its waves' chain of these steps.  From 65 queries on: 16 rows of 80 x 16
+// heads 23.3 us, in tiles of 64 on single waves 38.9; 64 rows of 64 there 48.4, here 54.0.
 //
 // LDS: K rows of 128 bytes, 16-byte piece c of key j in slot c ^ (j / 2 & 7); V^T
 // pages of 64 x 32 bytes, the halves swapped where hd & 8: the 16 lanes of a
@@ -562,10 +564,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void a
   };
   int st = 0;
   for (int c = c0;; ++c) {
-    // The exponents are taken against m, which follows the maximum only when one of
-    // the wave's queries has left it by more than 2^kSlack: weights up to that are as
-    // exact.  The inner loop runs while none has, and keeps the accumulators in place
-    // (with the rescaling as a branch inside it, every chunk paid 80 register copies).
+    // The exponents are taken against m, which follows a query's maximum only when that
+    // has left it by more than 2^kSlack.  The inner loop runs while none of the wave's has,
+    // and keeps the accumulators in place (with the rescaling as a branch inside it, every
+    // chunk paid 80 register copies).  It costs precision: against the maximum itself the
+    // heaviest weight is 1, which bf16 holds, against one that lags it is rounded like the
+    // others.  Relative error of 8000 queries on a window of 2048, spread 2: 2.18e-3, with no
+    // slack 1.89e-3 in 102.4 us instead of 92.9 (the output's own rounding alone: 1.66e-3);
+    // nine packed prompts 1.96e-3 and 1.82e-3, 27.8 and 28.6; 16 rows of 80 23.3 and 24.1.
     float mn = -INFINITY;
     char* vb = ring;
     bool moved = false;

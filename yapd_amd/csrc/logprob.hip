@@ -489,6 +489,11 @@ void launch(const LogprobParams& P, hipStream_t st) {
 // 2048 15.6 / 21.1, 16384 57 / 148; 1024 of 20000 22.0 / 18.5, 2048 25.8 / 30.8; 1024 of 16000 fp32 22.8 / 19.7, 4000
 // 53.6 / 58.2; 512 of 300 4.6 / 6.3.  Rows of more than four such tiles keep eight waves at any number: 1024 of 60000
 // 41.1 / 29.7, 3000 75.6 / 75.0.
+// 17 granules are the speech vocabulary's row of 8194 bf16 (1025 granules, 16.02 a lane).  A row just longer takes a second
+// tile of as many loads, most of them the last granule again: 2048 rows of 8704 15.6 us, of 8800 17.0, of 10000 18.4; 16384 rows
+// 57.7, 63.1, 69.5, a step of 8 %.
+// Between 512 and some thousand rows neither form fills the chip: at 2048 rows of 8194 (15.7 us; the bytes alone 6.5) one wave a
+// row leaves a SIMD two waves, and what a row does once is exposed; two or four waves a row are not built there.
 template <bool kWide>
 void launch_rows(const LogprobParams& P, hipStream_t st) {
   const int64_t granules = (static_cast<int64_t>(P.vocab) + (kWide ? 3 : 7)) / (kWide ? 4 : 8) + 1;
