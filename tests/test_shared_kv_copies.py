@@ -73,6 +73,26 @@ def test_a_copied_row_does_not_follow_its_source():
     assert not m.kv.table_host[0, :2].any() and m.kv.table_host[0, 2:].all()
 
 
+def test_a_row_is_copied_again_in_a_full_pool():
+    """The pages that the destination gives back are enough for its copy."""
+    m = CopyModel(SharedPagedKV(n_layers=1, n_rows=3, pages_per_row=4, n_heads=4, device=CPU, n_pages=7))
+    m.write(0, 0, 48)
+    m.copy_row(0, 1, 48)
+    assert m.kv.free_pages == 0
+    m.write(0, 0, 20)
+    m.copy_row(0, 1, 48)
+    m.check()
+    m.kv.release(1)
+    m.rows[1] = [None] * 64
+    m.fork(0, [1], 48)     # shares all: nothing of its own to give back
+    m.write(2, 0, 16)
+    with pytest.raises(RuntimeError, match="3 needed, 2 free"):
+        m.copy_row(0, 1, 48)
+    m.check()
+    m.copy_row(0, 1, 32)
+    m.check()
+
+
 BAD = [
     ([1], [10], "outside the pool"), ([-1], [2], "page ids"), ([10], [2], "outside the pool"), ([1, 2], [3, 3], "two pairs"),
     ([1, 2], [2, 3], "source and a destination"), ([4], [4], "source and a destination"), ([1, 2], [3], "same length"),

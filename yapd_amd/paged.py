@@ -163,9 +163,13 @@ class SharedPagedKV(PagedKV):
     def _check_row(self, row: int) -> None:
         kernels.require(0 <= row < self.n_rows, f"row {row} outside [0, {self.n_rows})")
 
+    def _check_free(self, n: int, given_back: int = 0) -> None:
+        free = len(self._free) + given_back
+        if n > free:
+            raise RuntimeError(f"the pool is out of pages: {n} needed, {free} free")
+
     def _take(self, n: int) -> List[int]:
-        if n > len(self._free):
-            raise RuntimeError(f"the pool is out of pages: {n} needed, {len(self._free)} free")
+        self._check_free(n)
         return [self._free.pop() for _ in range(n)]
 
     def _drop(self, pages: np.ndarray) -> None:
@@ -266,7 +270,8 @@ class SharedPagedKV(PagedKV):
 
     def copy_row_pages(self, src_row: int, dst_row: int, n_positions: int) -> None:
         """Positions ``[0, n_positions)`` of ``src_row`` as pages of ``dst_row``'s own; what the destination
-        mapped there is given back.  Unmapped source pages stay unmapped."""
+        mapped there is given back first.  Unmapped source pages stay unmapped.  Raises ``RuntimeError``,
+        with nothing changed, if the pool has too few pages left."""
         self._check_row(src_row)
         self._check_row(dst_row)
         kernels.require(0 <= n_positions <= self.pages_per_row * PAGE_SIZE, "n_positions outside what a row maps")
@@ -275,14 +280,16 @@ class SharedPagedKV(PagedKV):
         cols = np.arange((n_positions + PAGE_SIZE - 1) // PAGE_SIZE)
         src = self.table_host[src_row, cols]
         mapped = src != 0
-        own = self._take(int(mapped.sum()))
         old = self.table_host[dst_row, cols]
+        old = old[old != 0]
+        self._check_free(int(mapped.sum()), int((self._refs[old] == 1).sum()))
+        self._drop(old)  # first, so that its own pages can be taken again; the source's are still mapped by it
+        own = self._take(int(mapped.sum()))
         new = np.zeros_like(src)
         new[mapped] = own
         self._refs[own] = 1
         self.copy_pages(src[mapped], own)
         self.table_host[dst_row, cols] = new
-        self._drop(old[old != 0])
         self._upload([dst_row])
 
 
