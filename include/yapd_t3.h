@@ -199,9 +199,9 @@ int yapd_attn_paged_block_noalloc(const void* q, const void* kv_pool, int64_t n_
  * overlap.  window >= 1, sinks >= 0, H a multiple of 4, 1e-30 <= scale <= 1e30
  * and scores (scale q.k) below 2^30 in magnitude.
  * Scores, sums and statistics are fp32.  The weights are rounded to bf16 for the
- * product with V, from 65 queries a row on relative to a maximum that may lag by
- * 2^8: a relative error of 1.9e-3 up to 64 queries and 2.2e-3 from there on,
- * 1.7e-3 of which is the output's own rounding (random inputs of spread 2). */
+ * product with V, for max_q > 64 relative to a maximum that may lag by 2^8: a
+ * relative error of 1.9e-3 for max_q <= 64 and 2.2e-3 beyond, against 1.7e-3 of
+ * the output's rounding alone (random inputs of spread 2). */
 int yapd_attn_window(const void* q, int64_t q_tok_stride, const void* kv_pool, int64_t n_pages,
                      const int32_t* page_table, int table_stride, int table_cols, const int32_t* kv_len,
                      const int32_t* q_start, int rows, int max_q, int n_q, int n_heads, int window, int sinks,
