@@ -194,7 +194,7 @@ def _prepare_store(case, seed):
     qkv = qkv.to(BF)
     return SimpleNamespace(op="store", k=qkv[:, 1], v=qkv[:, 2], pool8=_pool(g, n_pages, H, 8),
                            table=torch.from_numpy(table).to(DEV), pos0=_ints(past), kv_len=_ints(kv_len),
-                           q_start=_ints(_starts(n_new)), max_q=max(n_new), max_kv=max(kv_len),
+                           q_start=_ints(_starts(n_new)), max_kv=max(kv_len),
                            pool=torch.zeros(n_wide, 2, H, PAGE * HD, dtype=BF, device=DEV),
                            wide_table=torch.from_numpy(wide_table).to(DEV))
 
@@ -260,7 +260,7 @@ def _own_tree(s):
 
 def _own_store(s):
     from yapd_amd import kernels
-    kernels.kv8_write(s.k, s.v, s.pool8, s.table, s.pos0, q_start=s.q_start, max_q=s.max_q)
+    kernels.kv8_write(s.k, s.v, s.pool8, s.table, s.pos0, q_start=s.q_start)
     kernels.kv8_unpack(s.pool8, s.table, s.kv_len, s.pool, s.wide_table, max_kv=s.max_kv)
     return s.pool
 
