@@ -214,6 +214,78 @@ int64_t yapd_attn_window_workspace(int rows, int max_q, int n_q, int packed, int
                                    int max_kv);
 
 /* ------------------------------------------------------------------------ *
+ * Drafted tokens: an 8-bit KV cache, attention for trees of drafted tokens over
+ * a cache of either width, the accepted tokens moved together.  For hosts that
+ * decode token by token or verify drafts with a layer loop of their own; none
+ * has a counterpart in the reference.
+ *
+ * 8-bit pool (one per layer): [n_pages][2][H][16*64 + 16] bytes.  A head's plane
+ * holds its 16 tokens' codes in the bf16 pool's order (signed bytes in [-127,
+ * 127]), then a scale byte e for each token: value = code * 2^(e - 127).
+ * n_heads is a multiple of 4, at most 1024, in all of these.
+ * ------------------------------------------------------------------------ */
+
+/* As yapd_kv_copy_pages, for 8-bit pools. */
+int yapd_kv8_copy_pages(void* const* kv_pools, int n_layers, int64_t n_pages, int n_heads, const int32_t* src,
+                        const int32_t* dst, int n_pairs, void* stream);
+
+/* Quantise k, v (bf16 [n_tokens, H, 64] with token strides k_tok_stride,
+ * v_tok_stride) into the pages.  For the 64 values x of a token's head: e - 127 =
+ * max(floor(log2 max|x|) - 6, -126), code = x 2^(127 - e) rounded to the nearest
+ * (ties to even) and held to [-127, 127]: off by at most 2^(e - 128) <= max|x| / 128.
+ * NaN counts as 0, an infinity as the largest finite bf16.  Row r's tokens, n_tokens / rows
+ * each or (q_start, device int32 [rows + 1], not decreasing) tokens [q_start[r],
+ * q_start[r + 1]), go to positions pos0[r], pos0[r] + 1, ...; positions that the
+ * table does not map to a page in [0, n_pages) are left out, and no other
+ * byte of the pool is written.  Two tokens of one position: either's. */
+int yapd_kv8_write(const void* k, const void* v, int64_t k_tok_stride, int64_t v_tok_stride, void* kv_pool8,
+                   int64_t n_pages, const int32_t* page_table, int table_stride, int table_cols, const int32_t* pos0,
+                   const int32_t* q_start, int rows, int n_tokens, int n_heads, void* stream);
+
+/* Read an 8-bit cache back: for every row and column c with 16 c < min(kv_len[r],
+ * max_kv, what both tables map), page page_table[r][c] of kv_pool (bf16) becomes
+ * the values of page page_table8[r][c] of kv_pool8, all 16 slots as they
+ * stand.  Exact: code * 2^(e - 127) is a bf16 value.  Columns that either table does not map
+ * to a page of its pool are left out.  Rows that share a page on both
+ * sides write the same bytes.  kv_len: device int32 [rows]. */
+int yapd_kv8_unpack(const void* kv_pool8, int64_t n_pages8, const int32_t* page_table8, int table8_stride,
+                    int table8_cols, const int32_t* kv_len, int rows, int max_kv, int n_heads, void* kv_pool,
+                    int64_t n_pages, const int32_t* page_table, int table_stride, int table_cols, void* stream);
+
+/* Attention for trees of drafted tokens.  Row r's n(r) <= 64 nodes are the cache's
+ * positions ctx .. ctx + n - 1, ctx = kv_len[r] - n(r), their K and V already
+ * written.  Node i sees node j iff bit j of its mask is set (bits from n on are
+ * ignored), and key j < ctx iff j < sinks or j > ctx + depth - window, depth = the
+ * number of other bits set in its mask.  out = softmax(q K^T * scale) V over the
+ * keys seen; a node that sees none gets zeros.
+ *   q, out, page tables, kv_len, q_start, max_q, n_q, max_kv and workspace: as
+ *   yapd_attn_window; max_q <= 64 and window >= max_q.  mask: device int64 [n_q].
+ *   kv_pool: bits = 16 the bf16 pool, bits = 8 the 8-bit pool.  K and V have to be
+ *   finite where any node of the row sees them.
+ * Scores, sums and statistics are fp32; the weights (of an 8-bit pool times V's
+ * scales) are rounded to bf16 for the product with V. */
+int yapd_attn_tree(const void* q, int64_t q_tok_stride, const void* kv_pool, int bits, int64_t n_pages,
+                   const int32_t* page_table, int table_stride, int table_cols, const int32_t* kv_len,
+                   const int32_t* q_start, const int64_t* mask, int rows, int max_q, int n_q, int n_heads, int window,
+                   int sinks, int max_kv, float scale, float* workspace, int64_t workspace_floats, void* out,
+                   void* stream);
+
+/* Floats of workspace that yapd_attn_tree needs for a call of these sizes; 0 if
+ * none, -1 on a bad argument. */
+int64_t yapd_attn_tree_workspace(int rows, int max_q, int n_q, int n_heads, int window, int sinks, int max_kv, int bits);
+
+/* Accepted nodes moved together, in every layer: position base[r] + i of row r
+ * becomes what position base[r] + kept[r * kept_stride + i] was, i < min(n_kept[r],
+ * max_kept), K, V and (bits = 8) their scales.  A row's values are all read
+ * before the first is written.  base, kept, n_kept: device int32; kv_pools: a
+ * host array of pool addresses.  Entries whose source or destination the table
+ * does not map to a page in [0, n_pages) are left out.  The pages written must belong to
+ * one row alone.  max_kept <= 64, rows <= 65535. */
+int yapd_kv_keep(void* const* kv_pools, int n_layers, int bits, int64_t n_pages, int n_heads,
+                 const int32_t* page_table, int table_stride, int table_cols, const int32_t* base,
+                 const int32_t* kept, int kept_stride, int max_kept, const int32_t* n_kept, int rows, void* stream);
+
+/* ------------------------------------------------------------------------ *
  * (b) bf16 MFMA projections (nn.Linear layout: C = A W^T, fp32 accumulate).
  * K must be a multiple of 64; A, W 16-byte aligned with leading dims
  * multiples of 8.

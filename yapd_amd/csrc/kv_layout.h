@@ -29,4 +29,16 @@ __host__ __device__ __forceinline__ int64_t v_offset(int64_t page, int head, int
   return kv_plane_offset(page, 1, head, n_heads) + d * kPageSize + slot;
 }
 
+// The 8-bit pool is [pages][2][heads][kTile8] bytes: a head's plane holds the codes of its 16 tokens in the order
+// above (K token-major, V transposed), then the tokens' scale bytes e, one for each (token, head, plane):
+// value = code * 2^(e - 127), code a signed byte in [-127, 127].
+constexpr int kTile8 = kHeadTile + kPageSize;  // 1040 = 65 * 16: every plane starts on 16 bytes
+
+__host__ __device__ __forceinline__ int64_t kv8_plane_offset(int64_t page, int plane, int head, int n_heads) {
+  return ((page * 2 + plane) * n_heads + head) * static_cast<int64_t>(kTile8);
+}
+
+// 2^(byte - 127), 0 for byte 0: the scale bytes are fp32 exponents.
+__device__ __forceinline__ float kv8_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+
 }  // namespace yapd

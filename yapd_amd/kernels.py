@@ -50,6 +50,17 @@ _SIGNATURES = {
                               c_int, c_int, c_void]),
     "yapd_kv_gather": (c_int, [c_void, c_i64, c_void, c_int, c_int, c_int, c_void, c_void, c_void]),
     "yapd_kv_copy_pages": (c_int, [c_void, c_int, c_i64, c_int, c_void, c_void, c_int, c_void]),
+    "yapd_kv8_copy_pages": (c_int, [c_void, c_int, c_i64, c_int, c_void, c_void, c_int, c_void]),
+    "yapd_kv8_write": (c_int, [c_void, c_void, c_i64, c_i64, c_void, c_i64, c_void, c_int, c_int, c_void, c_void, c_int,
+                               c_int, c_int, c_void]),
+    "yapd_kv8_unpack": (c_int, [c_void, c_i64, c_void, c_int, c_int, c_void, c_int, c_int, c_int, c_void, c_i64, c_void,
+                                c_int, c_int, c_void]),
+    "yapd_kv_keep": (c_int, [c_void, c_int, c_int, c_i64, c_int, c_void, c_int, c_int, c_void, c_void, c_int, c_int,
+                             c_void, c_int, c_void]),
+    "yapd_attn_tree": (c_int, [
+        c_void, c_i64, c_void, c_int, c_i64, c_void, c_int, c_int, c_void, c_void, c_void, c_int, c_int, c_int, c_int,
+        c_int, c_int, c_int, c_float, c_void, c_i64, c_void, c_void]),
+    "yapd_attn_tree_workspace": (c_i64, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "yapd_gemm_bf16": (c_int, [c_void, c_i64, c_void, c_i64, c_int, c_int, c_int, c_void, c_i64, c_void]),
     "yapd_gemm_bf16_residual": (c_int, [c_void, c_i64, c_void, c_i64, c_int, c_int, c_int, c_void, c_i64, c_void]),
     "yapd_gemm_head_shift": (c_int, [c_void, c_void, c_int, c_int, c_int, c_void, c_i64, c_int, c_void, c_i64,
@@ -478,18 +489,22 @@ def kv_gather(pool: torch.Tensor, table_row: torch.Tensor, kv_len: int):
 
 
 def pool_pointers(pools):
-    """The device addresses of every layer's pool, and the pools' common shape and device, checked."""
+    """The device addresses of every layer's pool, and the pools' common shape and device, checked.
+
+    Pools are bf16, or uint8 for an 8-bit cache (``shape[3]`` tells which)."""
     require(len(pools) >= 1, "no pools")
-    shape, dev, bf16 = pools[0].shape, pools[0].device, torch.bfloat16
+    shape, dev = pools[0].shape, pools[0].device
+    dtype = torch.uint8 if pools[0].dtype is torch.uint8 else torch.bfloat16
     index = pools[0].get_device()
     ptrs = []
     for p in pools:
-        if p.dtype is not bf16 or p.shape != shape or p.get_device() != index or not p.is_contiguous():
-            require_cuda(p, "pool", bf16, dev)
+        if p.dtype is not dtype or p.shape != shape or p.get_device() != index or not p.is_contiguous():
+            require_cuda(p, "pool", dtype, dev)
             raise ValueError("every layer's pool must have the same shape")
         ptrs.append(p.data_ptr())
-    require_cuda(pools[0], "pool", bf16, dev)
-    require(len(shape) == 4 and shape[0] >= 1 and shape[1] == 2 and shape[3] == 1024, "pools must be [pages, 2, H, 16*64]")
+    require_cuda(pools[0], "pool", dtype, dev)
+    require(len(shape) == 4 and shape[0] >= 1 and shape[1] == 2 and shape[3] == (TILE8 if dtype is torch.uint8 else 1024),
+            "pools must be [pages, 2, H, 16*64] (uint8: [pages, 2, H, 16*64 + 16])")
     return array("Q", ptrs), shape, dev
 
 
@@ -531,8 +546,223 @@ def kv_copy_pages(pools, src, dst) -> None:
             return kv_copy_pages(pools, src, dst)
     src, dst = page_ids(src, "src"), page_ids(dst, "dst")
     require(src.size == dst.size, "src and dst must have the same length")
-    check(load_library().yapd_kv_copy_pages(ptrs.buffer_info()[0], len(ptrs), shape[0], shape[2], src.ctypes.data,
-                                            dst.ctypes.data, src.size, stream_ptr(dev)))
+    copy = load_library().yapd_kv_copy_pages if shape[3] == 1024 else load_library().yapd_kv8_copy_pages
+    check(copy(ptrs.buffer_info()[0], len(ptrs), shape[0], shape[2], src.ctypes.data, dst.ctypes.data, src.size,
+               stream_ptr(dev)))
+
+
+# --------------------------------------------------------------------------- #
+# drafted tokens: the 8-bit cache, attention for trees, the accepted tokens
+# --------------------------------------------------------------------------- #
+
+TILE8 = 16 * 64 + 16  # bytes of one head's plane on a page of an 8-bit pool: codes, then a scale byte a token
+MAX_NODES = 64        # nodes of a drafted tree: bits of a mask
+
+
+def kv_bits(pool: torch.Tensor) -> int:
+    """8 or 16: the width of a pool's values."""
+    return 8 if pool.dtype is torch.uint8 else 16
+
+
+def check_pool(pool: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device, heads: int) -> None:
+    require_cuda(pool, name, dtype, dev)
+    tile = TILE8 if dtype is torch.uint8 else 1024
+    if pool.shape[1:] != (2, heads, tile):
+        raise ValueError(f"{name} must be [pages, 2, {heads}, {'16*64 + 16' if tile == TILE8 else '16*64'}]")
+
+
+def check_table(table: torch.Tensor, name: str, dev: torch.device, rows: int):
+    """``(columns, row pitch)`` of an int32 page table of at least ``rows`` rows."""
+    require_cuda(table, name, torch.int32, dev, contiguous=False)
+    shape, stride = table.shape, table.stride()
+    require(len(shape) == 2 and shape[0] >= rows and shape[1] >= 1 and (shape[1] == 1 or stride[1] == 1),
+            f"{name} must be [>= rows, max_pages] with unit column stride")
+    require(rows <= 1 or stride[0] >= shape[1], f"{name}'s rows must not overlap")
+    return shape[1], max(stride[0], shape[1])
+
+
+def kv8_write(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, pos0: torch.Tensor, *,
+              q_start: Optional[torch.Tensor] = None) -> None:
+    """Quantise fresh ``k, v`` (bf16 ``[tokens, H, 64]`` with packed heads, any token stride) into the pages of an
+    8-bit pool (``yapd_kv8_write``): uint8 ``[pages, 2, H, 16*64 + 16]``, one power-of-two scale a (token, head, plane).
+
+    Row ``r``'s tokens go to positions ``pos0[r], pos0[r] + 1, ...``: ``tokens / rows`` of them each (``rows`` the entries
+    of ``pos0``), or packed ``[q_start[r], q_start[r + 1])`` (int32, not decreasing).  Positions that the table does not
+    map to a page of the pool are left out; every other byte of the pool stays.  NaN is written as 0, infinities as
+    the largest finite value."""
+    dev = k.device
+    if k.is_cuda and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):  # the launch goes to the current device
+            return kv8_write(k, v, pool, table, pos0, q_start=q_start)
+    for name, t in (("k", k), ("v", v)):
+        require_cuda(t, name, torch.bfloat16, dev, contiguous=False)
+        require(t.dim() == 3 and t.shape == k.shape and t.shape[2] == 64, "k and v must be [tokens, H, 64]")
+        require(t.numel() == 0 or (t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == 64)), f"{name}'s heads must be packed")
+    n, H, _ = k.shape
+    check_pool(pool, "pool", torch.uint8, dev, H)
+    require_cuda(pos0, "pos0", torch.int32, dev)
+    rows = pos0.numel()
+    cols, pitch = check_table(table, "table", dev, rows)
+    if q_start is None:
+        require(n % rows == 0 if rows else n == 0, "k and v must hold the same number of tokens for every row")
+    else:
+        require_cuda(q_start, "q_start", torch.int32, dev)
+        require(q_start.numel() == rows + 1, "q_start must be [rows + 1]")
+    if n == 0 or rows == 0:
+        return
+    tok = [t.stride(0) if n > 1 else H * 64 for t in (k, v)]
+    check(load_library().yapd_kv8_write(
+        k.data_ptr(), v.data_ptr(), tok[0], tok[1], pool.data_ptr(), pool.shape[0], table.data_ptr(), pitch, cols,
+        pos0.data_ptr(), ptr(q_start), rows, n, H, stream_ptr(dev)))
+
+
+def kv8_unpack(pool8: torch.Tensor, table8: torch.Tensor, kv_len: torch.Tensor, pool: torch.Tensor,
+               table: torch.Tensor, *, max_kv: Optional[int] = None) -> None:
+    """Read an 8-bit cache back: the pages that hold positions ``[0, kv_len[r])`` of every row, mapped by ``table8``
+    in ``pool8``, become the bf16 pages of ``pool`` that ``table`` maps there (``yapd_kv8_unpack``).  Exact: a code
+    times its scale is a bf16 value.  A page's slots past ``kv_len`` are converted as they stand.
+
+    ``kv_len`` is read on the device; ``max_kv`` is the host's upper bound (default: all that both tables map),
+    past which nothing is converted.  Columns that either table does not map to a page of its pool are left out."""
+    dev = pool8.device
+    if pool8.is_cuda and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):  # the launch goes to the current device
+            return kv8_unpack(pool8, table8, kv_len, pool, table, max_kv=max_kv)
+    require(pool8.dim() == 4, "pool8 must be [pages, 2, H, 16*64 + 16]")
+    H = pool8.shape[2]
+    check_pool(pool8, "pool8", torch.uint8, dev, H)
+    check_pool(pool, "pool", torch.bfloat16, dev, H)
+    require_cuda(kv_len, "kv_len", torch.int32, dev)
+    rows = kv_len.numel()
+    if rows == 0:
+        return
+    cols8, pitch8 = check_table(table8, "table8", dev, rows)
+    cols, pitch = check_table(table, "table", dev, rows)
+    most = min(cols8, cols) * 16
+    most = most if max_kv is None else min(int(max_kv), most)
+    require(most >= 1, "max_kv must be >= 1")
+    check(load_library().yapd_kv8_unpack(
+        pool8.data_ptr(), pool8.shape[0], table8.data_ptr(), pitch8, cols8, kv_len.data_ptr(), rows, most, H,
+        pool.data_ptr(), pool.shape[0], table.data_ptr(), pitch, cols, stream_ptr(dev)))
+
+
+def tree_masks(parents):
+    """The masks of one drafted tree for :func:`attn_tree`, as an int64 numpy array: node ``i`` sees itself and its
+    ancestors.  ``parents[i]`` is the node that ``i`` follows (an earlier one), or -1 for the row's last token."""
+    import numpy as np
+    parents = [int(p) for p in parents]
+    require(len(parents) <= MAX_NODES, f"a tree has at most {MAX_NODES} nodes")
+    masks = []
+    for i, p in enumerate(parents):
+        require(-1 <= p < i, "a node's parent must be an earlier node, or -1")
+        masks.append((masks[p] if p >= 0 else 0) | 1 << i)
+    return np.array(masks, dtype=np.uint64).view(np.int64)
+
+
+def attn_tree(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, mask: torch.Tensor,
+              out: torch.Tensor, scale: float, *, window: Optional[int] = None, sinks: int = 0,
+              q_start: Optional[torch.Tensor] = None, max_q: Optional[int] = None, max_kv: Optional[int] = None,
+              workspace: Optional[torch.Tensor] = None) -> None:
+    """``out = softmax(q K^T * scale) V`` for trees of at most 64 drafted tokens over each row's pages, bf16 or 8-bit.
+
+    A row's ``n`` nodes are its last positions, ``ctx = kv_len - n`` up to ``kv_len``, their keys already in the cache.
+    Node ``i`` sees node ``j`` iff bit ``j`` of its ``mask`` (int64) is set (:func:`tree_masks`), and key ``j < ctx`` iff
+    ``j < sinks`` or ``j > ctx + depth - window``, ``depth`` the number of other nodes in its mask.  With one node and
+    mask 1 that is the next token of an ordinary decode.  A node that sees nothing gets zeros.
+
+    Nodes are ``[rows, n, H, 64]`` (``mask [rows, n]``), or packed ``[n_q, H, 64]`` (``mask [n_q]``) with the device
+    ``q_start [rows + 1]`` (int32, not decreasing); of a row of more than ``max_q`` nodes the first ``max_q`` are computed, as
+    the row's first.  Rows of ``out`` that are not computed or belong to no row are left as they were.  ``q`` may be a
+    view with packed heads and any token stride; ``out`` is contiguous; one that shares memory with ``q`` or the pool is refused.
+
+    Lengths and masks are read on the device: a captured call follows them.  ``max_q`` (default: all, at most 64) and
+    ``max_kv`` (default: all positions the table maps) are the host's upper bounds; ``window`` (default: none) is at least
+    ``max_q``.  Scores have to stay below 2^30 in magnitude.  Few nodes over many keys need a float32 ``workspace``
+    (``yapd_attn_tree_workspace``), allocated here unless given."""
+    dev = q.device
+    if q.is_cuda and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):  # the launch goes to the current device
+            return attn_tree(q, pool, table, kv_len, mask, out, scale, window=window, sinks=sinks, q_start=q_start,
+                             max_q=max_q, max_kv=max_kv, workspace=workspace)
+    require_cuda(q, "q", torch.bfloat16, dev, contiguous=False)
+    shape, stride = q.shape, q.stride()
+    packed = q_start is not None
+    if packed:
+        require(len(shape) == 3 and shape[2] == 64, "packed q must be [n_q, H, 64]")
+        n_q, H, _ = shape
+        require_cuda(q_start, "q_start", torch.int32, dev)
+        rows = q_start.numel() - 1
+        require(rows >= 0, "q_start must be [rows + 1]")
+        max_q = min(n_q, MAX_NODES) if max_q is None else int(max_q)
+        require(n_q == 0 or rows == 0 or max_q >= 1, "max_q must be >= 1")
+        tok = stride[0] if n_q > 1 else H * 64
+    else:
+        require(len(shape) == 4 and shape[3] == 64, "q must be [rows, n, H, 64] (or [n_q, H, 64] with q_start)")
+        rows, bl, H, _ = shape
+        n_q = rows * bl
+        require(max_q is None or max_q == bl, "max_q is given by q's shape unless q is packed")
+        max_q = bl
+        tok = stride[1] if bl > 1 else stride[0] if rows > 1 else H * 64
+        require(rows <= 1 or stride[0] == bl * tok or n_q == 0, "q's rows must follow each other")
+    require(n_q * H == 0 or (stride[-1] == 1 and (H == 1 or stride[-2] == 64)), "q's heads must be packed")
+    require_cuda(mask, "mask", torch.int64, dev)
+    require(mask.shape == shape[:-2], "mask must be q's shape without heads")
+    bits = kv_bits(pool)
+    check_pool(pool, "pool", torch.uint8 if bits == 8 else torch.bfloat16, dev, H)
+    require_cuda(kv_len, "kv_len", torch.int32, dev)
+    require(kv_len.numel() >= rows, "kv_len must have rows entries")
+    require_cuda(out, "out", torch.bfloat16, dev)
+    require(out.shape == shape, "out must match q")
+    window = WINDOW_CAP if window is None else min(int(window), WINDOW_CAP)
+    sinks = min(int(sinks), WINDOW_CAP)
+    require(window >= 1 and sinks >= 0, "need window >= 1 and sinks >= 0")
+    if n_q == 0 or rows == 0:
+        return
+    cols, pitch = check_table(table, "table", dev, rows)
+    kv_max = cols * 16 if max_kv is None else min(int(max_kv), cols * 16)
+    require(kv_max >= 1, "max_kv must be >= 1")
+    max_q = min(max_q, n_q)
+    lib = load_library()
+    if workspace is None:
+        need = lib.yapd_attn_tree_workspace(rows, max_q, n_q, H, window, sinks, kv_max, bits)
+        if need > 0:
+            workspace = torch.empty(need, dtype=torch.float32, device=dev)
+    else:
+        require_cuda(workspace, "workspace", torch.float32, dev)
+    check(lib.yapd_attn_tree(
+        q.data_ptr(), tok, pool.data_ptr(), bits, pool.shape[0], table.data_ptr(), pitch, cols, kv_len.data_ptr(),
+        ptr(q_start), mask.data_ptr(), rows, max_q, n_q, H, window, sinks, kv_max, scale, ptr(workspace),
+        0 if workspace is None else workspace.numel(), out.data_ptr(), stream_ptr(dev)))
+
+
+def kv_keep(pools, table: torch.Tensor, base: torch.Tensor, kept: torch.Tensor, n_kept: torch.Tensor) -> None:
+    """Move the accepted nodes of drafted trees together, in every layer's pool of ``pools`` (bf16 or 8-bit):
+    position ``base[r] + i`` of row ``r`` becomes what position ``base[r] + kept[r, i]`` was, for ``i < n_kept[r]``, in one
+    launch per 64 layers (``yapd_kv_keep``).
+
+    ``base [rows]``, ``kept [rows, m]`` (``m <= 64``) and ``n_kept [rows]`` are device int32, so a verification on the
+    device needs no synchronisation.  A row's values are all read before the first is written: any nodes in any
+    order.  Positions that the table does not map to a page of the pool are left out.  The written pages
+    must belong to one row alone."""
+    ptrs, shape, dev = pool_pointers(pools)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):  # the launch goes to the current device
+            return kv_keep(pools, table, base, kept, n_kept)
+    i32 = torch.int32
+    require_cuda(base, "base", i32, dev)
+    require_cuda(kept, "kept", i32, dev, contiguous=False)
+    require_cuda(n_kept, "n_kept", i32, dev)
+    rows = base.numel()
+    require(kept.dim() == 2 and kept.shape[0] == rows and kept.shape[1] <= MAX_NODES
+            and (kept.shape[1] <= 1 or kept.stride(1) == 1) and (rows <= 1 or kept.stride(0) >= kept.shape[1]),
+            f"kept must be [rows, at most {MAX_NODES}] with unit column stride")
+    require(n_kept.numel() == rows, "n_kept must have rows entries")
+    cols, pitch = check_table(table, "table", dev, rows)
+    if rows == 0 or kept.shape[1] == 0:
+        return
+    check(load_library().yapd_kv_keep(
+        ptrs.buffer_info()[0], len(ptrs), 16 if shape[3] == 1024 else 8, shape[0], shape[2], table.data_ptr(), pitch, cols,
+        base.data_ptr(), kept.data_ptr(), max(kept.stride(0), kept.shape[1]), kept.shape[1], n_kept.data_ptr(), rows, stream_ptr(dev)))
 
 
 # --------------------------------------------------------------------------- #

@@ -47,11 +47,19 @@ def copy_from_host_async(dst: torch.Tensor, data) -> None:
     dst.copy_(t.pin_memory(), non_blocking=True)
 
 
+def _check_bits(kv_bits: int) -> int:
+    kernels.require(kv_bits in (8, 16), f"kv_bits must be 8 or 16, got {kv_bits}")
+    return int(kv_bits)
+
+
 class PagedKV:
     """Per-layer page pools plus a host-side page allocator and device page table."""
 
     def __init__(self, *, n_layers: int, n_rows: int, pages_per_row: int, n_heads: int,
-                 device: torch.device, n_pages: Optional[int] = None, shuffle_seed: Optional[int] = None):
+                 device: torch.device, n_pages: Optional[int] = None, shuffle_seed: Optional[int] = None,
+                 kv_bits: int = 16):
+        """``kv_bits`` 8: uint8 pools of codes and scales (``kernels.kv8_write``), half the bytes; 16: bf16."""
+        self.kv_bits = _check_bits(kv_bits)
         self.n_layers = int(n_layers)
         self.n_rows = int(n_rows)
         self.pages_per_row = int(pages_per_row)
@@ -68,15 +76,15 @@ class PagedKV:
         self.table = torch.from_numpy(self.table_host).to(self.device)
 
     def _make_pools(self) -> None:
+        tile, dtype = (kernels.TILE8, torch.uint8) if self.kv_bits == 8 else (PAGE_SIZE * HEAD_DIM, torch.bfloat16)
         self.pools: List[torch.Tensor] = [
-            torch.zeros(self.n_pages, 2, self.n_heads, PAGE_SIZE * HEAD_DIM, dtype=torch.bfloat16,
-                        device=self.device)
+            torch.zeros(self.n_pages, 2, self.n_heads, tile, dtype=dtype, device=self.device)
             for _ in range(self.n_layers)
         ]
 
     @property
     def bytes_per_layer(self) -> int:
-        return self.pools[0].numel() * 2
+        return self.pools[0].numel() * self.pools[0].element_size()
 
     def swap_rows(self, a: int, b: int) -> None:
         """Exchange page-table rows ``a`` and ``b`` (host mirror and device table): each row's KV
@@ -101,6 +109,11 @@ class PagedKV:
         src_t, dst_t = (torch.from_numpy(x.astype(np.int64)) for x in (src, dst))
         for pool in self.pools:
             pool.index_copy_(0, dst_t, pool.index_select(0, src_t))
+
+    def keep_nodes(self, base: torch.Tensor, kept: torch.Tensor, n_kept: torch.Tensor) -> None:
+        """Move the accepted nodes of every row's drafted tree to the positions from ``base`` on, in every layer (see
+        :func:`kernels.kv_keep`; entry ``r`` of the device tensors is the cache's row ``r``), on the current stream."""
+        kernels.kv_keep(self.pools, self.table, base, kept, n_kept)
 
     def copy_row_pages(self, src_row: int, dst_row: int, n_positions: int) -> None:
         """Copy the pages holding positions ``[0, n_positions)`` of one row to another, every layer."""
@@ -132,8 +145,10 @@ class SharedPagedKV(PagedKV):
     """
 
     def __init__(self, *, n_layers: int, n_rows: int, pages_per_row: int, n_heads: int, device: torch.device,
-                 n_pages: int):
-        """``n_pages`` counts the pool's pages, page 0 included; a row maps at most ``pages_per_row``."""
+                 n_pages: int, kv_bits: int = 16):
+        """``n_pages`` counts the pool's pages, page 0 included; a row maps at most ``pages_per_row``; ``kv_bits`` as
+        :class:`PagedKV` has it."""
+        self.kv_bits = _check_bits(kv_bits)
         kernels.require(n_layers >= 1 and n_rows >= 1 and pages_per_row >= 1 and n_heads >= 1 and n_pages >= 2,
                         "need at least one layer, row, page per row and head, and two pages")
         self.n_layers = int(n_layers)
