@@ -99,6 +99,28 @@ int yapd_token_logprobs(const void* logits, int wide, int64_t seq_stride, int64_
                         int vocab, const int64_t* tokens, int top_k, float* logprob, float* entropy,
                         float* top_logprob, int64_t* top_token, void* stream);
 
+/* A token drawn from every row of logits with a given random number (what a host
+ * that decodes token by token does next; the reference's step draws by its own
+ * scorer).  logits, wide, strides: as yapd_token_logprobs.  In the order of a
+ * row's tokens (larger logit first, of equal ones the lower index) with weights w_i =
+ * e^((x_i - max) / T), top-k keeps the first top_k (<= 0: all), top-p of those
+ * the fewest first ones whose weight is at least top_p times theirs (>= 1: all; at
+ * least one), min-p those of w_i >= min_p (<= 0: all; the largest always).
+ * token is the first of what all three keep whose weight, with that of the ones before
+ * it, exceeds uniform times the weight kept, and logprob = ln(w_token / the
+ * weight kept).  T = 0 (or not above 0), like top_k = 1: the first token, logprob
+ * 0.  uniform is held to [0, 1 - 2^-24].  Tokens of logit -inf are never drawn.
+ * A row that holds a NaN or +inf, or -inf alone: token -1, logprob NaN.
+ * uniform [rows * bl] fp32; temperature, top_p, min_p (fp32) and top_k (int32) are
+ * [rows * bl], or NULL: the number beside it holds for every row.  token int64, logprob fp32.
+ * Weights are rounded to 64-bit fixed point (2^-51, with more than 2^11 tokens
+ * 2^-62 times the next power of two), their sums are exact: the same call gives the same
+ * token.  vocab <= 2^24.  One launch, no workspace. */
+int yapd_sample_tokens(const void* logits, int wide, int64_t seq_stride, int64_t pos_stride, int rows, int bl,
+                       int vocab, const float* uniform, const float* temperature, float temperature_all,
+                       const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all, const float* min_p,
+                       float min_p_all, int64_t* token, float* logprob, void* stream);
+
 /* ------------------------------------------------------------------------ *
  * Paged KV pool (one per layer): bf16 [n_pages][2][H][16*64]; plane 0 holds
  * K (token-major inside a head), plane 1 holds V transposed inside a head.

@@ -1,0 +1,496 @@
+// Tokens drawn from logits with given random numbers: temperature, top-k, top-p and min-p.
+//
+// A row's tokens in order (larger logit first, of equal ones the lower index) have the weights
+//   w_i = e^((x_i - max) / T);  W(n) = the sum of the first n.
+// Each filter keeps a prefix of that order: top-k the first k; top-p the shortest whose weight is at least p W(k); min-p
+// the tokens of w_i >= min_p.  So all three together keep the shortest, whose weight is the least, Z = min(W(k), W_p,
+// W_m), and the token is the first whose inclusive sum exceeds u Z.  No token's membership is ever asked: three
+// sums are looked for, in the same order.
+//
+// The row is not sorted.  Its weights are added up in kBins bins of equal width in x (in fp32, which keeps the order),
+// the bins' prefix sums find the bin where a sum crosses a target, and that bin's elements, usually a few dozen, go to
+// a list where each adds up what precedes it.  A bin of more than kList elements (many equal or nearly equal
+// logits) is divided again, by the bits of (value, index), 10 a time.
+// Weights are fixed-point numbers of 64 bits, rounded from 64-bit exponentials: their sums are exact, so they do not
+// depend on the order of LDS atomics, and a border is off by V roundings of 2^-52 to 2^-39 at most.
+#include "attn_tile.h"
+#include "common.h"
+
+namespace yapd {
+namespace {
+
+constexpr int kBins = 1024;
+constexpr int kList = 256;
+constexpr double kLn2 = 0.69314718055994530942, kLog2e = 1.44269504088896340736;
+
+struct SampleParams {
+  const void* logits;
+  int64_t seq_stride, pos_stride;  // elements
+  uint32_t items, bl;
+  int vocab;
+  int shift;  // weights are multiples of 2^-shift
+  const float* u;
+  const float* temperature;  // [items], or NULL: the number beside it
+  float temperature_all;
+  const int32_t* top_k;
+  int top_k_all;
+  const float* top_p;
+  float top_p_all;
+  const float* min_p;
+  float min_p_all;
+  int64_t* token;
+  float* logprob;
+};
+
+// Floats as unsigned numbers in their order (-0 taken as +0).
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+}
+// Larger value first, then lower index: descending numbers.
+__device__ __forceinline__ uint64_t key_of(float x, int index) {
+  return static_cast<uint64_t>(order_of(x)) << 32 | (0xffffffffu - static_cast<uint32_t>(index));
+}
+
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t o = static_cast<uint32_t>(key >> 32);
+  return __uint_as_float(o ^ (o >> 31 ? 0x80000000u : 0xffffffffu));
+}
+
+// 2^-t as a multiple of 2^-shift, for t >= 0: with r = t rounded, f = t - r, the Taylor polynomial of e^(-f ln 2)
+// (|f ln 2| <= 0.347: off by 2e-13), rounded to an integer by adding 2^52.
+__device__ __forceinline__ uint64_t weight_of(double t, int shift) {
+  t = fmin(t, 1000.0);
+  const double r = __builtin_rint(t);
+  const double a = (r - t) * kLn2;
+  double p = 1.0 / 3628800;
+  p = __builtin_fma(p, a, 1.0 / 362880);
+  p = __builtin_fma(p, a, 1.0 / 40320);
+  p = __builtin_fma(p, a, 1.0 / 5040);
+  p = __builtin_fma(p, a, 1.0 / 720);
+  p = __builtin_fma(p, a, 1.0 / 120);
+  p = __builtin_fma(p, a, 1.0 / 24);
+  p = __builtin_fma(p, a, 1.0 / 6);
+  p = __builtin_fma(p, a, 0.5);
+  p = __builtin_fma(p, a, 1.0);
+  p = __builtin_fma(p, a, 1.0);
+  const double v = __builtin_ldexp(p, shift - static_cast<int>(r)) + 0x1p52;
+  return __builtin_bit_cast(uint64_t, v) - (uint64_t{0x433} << 52);
+}
+
+__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
+  const uint32_t lo = __shfl_up(static_cast<uint32_t>(v), d), hi = __shfl_up(static_cast<uint32_t>(v >> 32), d);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d) {
+  const uint32_t lo = __shfl_xor(static_cast<uint32_t>(v), d), hi = __shfl_xor(static_cast<uint32_t>(v >> 32), d);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+enum Cross { kCount, kReach, kExceed };  // the first element whose inclusive count, or sum, is at least, or exceeds, a target
+
+template <int NT>
+struct Shared {
+  uint64_t mass[kBins], mass2[kBins];
+  uint32_t count[kBins], count2[kBins];
+  uint64_t key[kList], w[kList];
+  uint64_t part[NT / 64], part2[NT / 64], z_min[NT / 64];
+  float fmx[NT / 64], fmn[NT / 64];
+  uint32_t n, bad;
+  // what a search found
+  int bin;
+  uint64_t base, sum;
+  uint32_t base_count;
+  uint64_t found;
+};
+
+// One workgroup a row, which every pass reads again (from the caches: a speech vocabulary's row is 16 KB).
+template <bool kWide, int NT>
+__global__ __launch_bounds__(NT) void sample_kernel(const SampleParams P) {
+  constexpr int G = kWide ? 4 : 8, kBytes = kWide ? 4 : 2;
+  __shared__ Shared<NT> S;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t item = blockIdx.x;
+  const uint32_t r = item / P.bl;
+  const int64_t at = (r * P.seq_stride + static_cast<int64_t>(item - r * P.bl) * P.pos_stride) * kBytes;
+  const uintptr_t row = reinterpret_cast<uintptr_t>(P.logits) + at;
+  const u32x4_t* granules = reinterpret_cast<const u32x4_t*>(row & ~uintptr_t{15});
+  const int off = static_cast<int>(row & 15) / kBytes, V = P.vocab;
+  const int n_gran = (off + V + G - 1) / G;
+
+  // a granule, what it holds beside the row as -inf
+  auto fetch = [&](int gi) {
+    u32x4_t v = granules[gi];
+    if (gi == 0 || gi == n_gran - 1) {
+#pragma unroll
+      for (int e = 0; e < G; ++e) {
+        const int i = gi * G + e - off;
+        if (i >= 0 && i < V) continue;
+        if constexpr (kWide)
+          v[e] = 0xff800000u;
+        else
+          v[e >> 1] = (v[e >> 1] & (e & 1 ? 0x0000ffffu : 0xffff0000u)) | (e & 1 ? 0xff800000u : 0x0000ff80u);
+      }
+    }
+    return v;
+  };
+  auto element = [&](const u32x4_t& v, int e) {
+    if constexpr (kWide) return __uint_as_float(v[e]);
+    return e & 1 ? bf16hi(v[e >> 1]) : bf16lo(v[e >> 1]);
+  };
+  // f(granule, its first element's index) for every granule of this thread, the next one on its way
+  auto each = [&](auto f) {
+    if (tid >= n_gran) return;
+    u32x4_t v = fetch(tid);
+    for (int gi = tid; gi < n_gran; gi += NT) {
+      const u32x4_t next = fetch(min(gi + NT, n_gran - 1));
+      f(v, gi * G - off);
+      v = next;
+    }
+  };
+  // f(key, bin) for every finite element of this thread, one at a time: for passes that are seldom made
+  auto each_key = [&](auto f) {
+    for (int i = tid; i < V; i += NT) {
+      float x;
+      if constexpr (kWide)
+        x = reinterpret_cast<const float*>(row)[i];
+      else
+        x = bf16_to_f32(reinterpret_cast<const uint16_t*>(row)[i]);
+      if (x > -INFINITY) f(x, key_of(x, i));
+    }
+  };
+
+  const float T = P.temperature ? P.temperature[item] : P.temperature_all;
+  const int k = P.top_k ? P.top_k[item] : P.top_k_all;
+  const float top_p = P.top_p ? P.top_p[item] : P.top_p_all;
+  const float min_p = P.min_p ? P.min_p[item] : P.min_p_all;
+  const float u = P.u[item];
+  for (int b = tid; b < kBins; b += NT) {
+    S.mass[b] = 0;
+    S.count[b] = 0;
+  }
+  if (tid == 0) S.bad = 0;
+
+  // the largest logit, the least of whole granules (it only decides the bins' width), and whether there is a NaN or +inf
+  float mx = -INFINITY, mn = INFINITY;
+  bool bad = false;
+  each([&](const u32x4_t& v, int i0) {
+    float lo = INFINITY;
+#pragma unroll
+    for (int e = 0; e < G; ++e) {
+      const float x = element(v, e);
+      bad |= !(x < INFINITY);
+      mx = fmaxf(mx, x);
+      lo = fminf(lo, x);
+    }
+    if (i0 >= 0 && i0 + G <= V) mn = fminf(mn, lo);
+  });
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    mx = fmaxf(mx, __shfl_xor(mx, d));
+    mn = fminf(mn, __shfl_xor(mn, d));
+  }
+  if (lane == 0) {
+    S.fmx[wave] = mx;
+    S.fmn[wave] = mn;
+  }
+  __syncthreads();
+  if (__any(bad) && lane == 0) atomicOr(&S.bad, 1u);
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    mx = fmaxf(mx, S.fmx[w]);
+    mn = fminf(mn, S.fmn[w]);
+  }
+  if (tid == 0) S.n = 0xffffffffu;
+  __syncthreads();
+  if (S.bad || mx == -INFINITY) {  // no distribution
+    if (tid == 0) {
+      P.token[item] = -1;
+      P.logprob[item] = __builtin_nanf("");
+    }
+    return;
+  }
+  if (!(T > 0.f) || k == 1) {  // the first token
+    uint32_t first = 0xffffffffu;
+    each([&](const u32x4_t& v, int i0) {
+#pragma unroll
+      for (int e = 0; e < G; ++e)
+        if (element(v, e) == mx) first = min(first, static_cast<uint32_t>(i0 + e));
+    });
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) first = min(first, __shfl_xor(first, d));
+    if (lane == 0) atomicMin(&S.n, first);
+    __syncthreads();
+    if (tid == 0) {
+      P.token[item] = S.n;
+      P.logprob[item] = 0.f;
+    }
+    return;
+  }
+
+  const double scale = kLog2e / static_cast<double>(T);
+  // bins: the row's range, or 64 octaves of weight where that is less (smaller weights than the last bin's are 0)
+  const float per_x = fminf(fmaxf((kBins - 1) / (mx - mn), static_cast<float>((kBins - 1) / 64.0 * scale)), 1e30f);
+  auto bin_of = [&](float x) { return static_cast<int>(fminf((mx - x) * per_x, static_cast<float>(kBins - 1))); };
+  auto t_of = [&](float x) { return (static_cast<double>(mx) - static_cast<double>(x)) * scale; };
+  const bool by_count = k > 0 && k < V;
+  const bool by_min = min_p > 0.f;
+  const double t_min = by_min ? -log2(static_cast<double>(fminf(min_p, 1.f))) : 0.0;
+
+  uint64_t z_min = 0;  // the weight of what min-p keeps
+  uint32_t last = 0;   // elements of the last bin
+  each([&](const u32x4_t& v, int) {
+#pragma unroll
+    for (int e = 0; e < G; ++e) {
+      const float x = element(v, e);
+      if (!(x > -INFINITY)) continue;
+      const int b = bin_of(x);
+      const double t = t_of(x);
+      const uint64_t w = weight_of(t, P.shift);
+      if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&S.mass[b]), static_cast<unsigned long long>(w));
+      if (by_count) {
+        if (b < kBins - 1)
+          atomicAdd(&S.count[b], 1u);
+        else
+          ++last;
+      }
+      if (by_min && t <= t_min) z_min += w;
+    }
+  });
+  if (last) atomicAdd(&S.count[kBins - 1], last);
+  if (by_min) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) z_min += shfl_xor64(z_min, d);
+    if (lane == 0) S.z_min[wave] = z_min;
+  }
+  __syncthreads();
+  if (by_min) {
+    z_min = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) z_min += S.z_min[w];
+  }
+
+  // bins' sums and counts become inclusive prefix sums
+  auto scan = [&](uint64_t* mass, uint32_t* count, bool counts) {
+    constexpr int kPer = kBins / NT;
+    uint64_t m[kPer], ms = 0;
+    uint32_t c[kPer], cs = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      m[j] = ms += mass[tid * kPer + j];
+      c[j] = cs += counts ? count[tid * kPer + j] : 0;
+    }
+    uint64_t mi = ms;
+    uint32_t ci = cs;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint64_t ml = shfl_up64(mi, d);
+      const uint32_t cl = __shfl_up(ci, d);
+      if (lane >= d) {
+        mi += ml;
+        ci += cl;
+      }
+    }
+    if (lane == 63) {
+      S.part[wave] = mi;
+      S.part2[wave] = ci;
+    }
+    __syncthreads();
+    mi -= ms;
+    ci -= cs;
+    for (int w = 0; w < wave; ++w) {
+      mi += S.part[w];
+      ci += static_cast<uint32_t>(S.part2[w]);
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      mass[tid * kPer + j] = mi + m[j];
+      if (counts) count[tid * kPer + j] = ci + c[j];
+    }
+    __syncthreads();
+  };
+  scan(S.mass, S.count, by_count);
+
+  // the bin in which the target is met; S.bin, S.base and S.base_count tell, after a barrier
+  auto find_bin = [&](const uint64_t* mass, const uint32_t* count, bool counts, Cross mode, uint64_t base, uint32_t base_count,
+                      double target) {
+    for (int b = tid; b < kBins; b += NT) {
+      const uint64_t before = b ? mass[b - 1] : 0, with = mass[b];
+      bool here;
+      if (mode == kCount) {
+        const uint32_t cb = base_count + (b ? count[b - 1] : 0), cw = base_count + count[b];
+        here = cw >= target && cb < target;
+      } else {
+        const double db = static_cast<double>(base + before), dw = static_cast<double>(base + with);
+        here = mode == kReach ? dw >= target && db < target : dw > target && db <= target;
+      }
+      if (here) {
+        S.bin = b;
+        S.base = base + before;
+        S.base_count = base_count + (counts && b ? count[b - 1] : 0);
+      }
+    }
+    __syncthreads();
+  };
+
+  // The element at which the target is met: its key in S.found, the inclusive sum in S.sum, after a barrier.
+  auto cross = [&](Cross mode, double target) {
+    find_bin(S.mass, S.count, by_count, mode, 0, 0, target);
+    const int bin = S.bin;
+    uint64_t base = S.base, klo = 0, khi = ~uint64_t{0};
+    uint32_t base_count = S.base_count;
+    for (;;) {  // at most 7 times: each further one leaves an interval of keys a thousandth as long
+      if (tid == 0) S.n = 0;
+      __syncthreads();
+      each([&](const u32x4_t& v, int i0) {
+#pragma unroll
+        for (int e = 0; e < G; ++e) {
+          const float x = element(v, e);
+          if (!(x > -INFINITY) || bin_of(x) != bin) continue;
+          const uint64_t key = key_of(x, i0 + e);
+          if (key < klo || key > khi) continue;
+          const uint32_t to = atomicAdd(&S.n, 1u);
+          if (to < kList) S.key[to] = key;
+        }
+      });
+      __syncthreads();
+      const int n = static_cast<int>(S.n);
+      if (n <= kList) {
+        for (int i = tid; i < n; i += NT) S.w[i] = weight_of(t_of(value_of(S.key[i])), P.shift);
+        __syncthreads();
+        for (int i = tid; i < n; i += NT) {
+          const uint64_t key = S.key[i], w = S.w[i];
+          uint64_t sum = base;
+          uint32_t count = base_count;
+          for (int j = 0; j < n; ++j) {
+            const bool in = S.key[j] >= key;
+            sum += in ? S.w[j] : 0;
+            count += in;
+          }
+          const double with = static_cast<double>(sum), before = static_cast<double>(sum - w);
+          const bool here = mode == kCount ? count == target
+                            : mode == kReach ? with >= target && before < target
+                                             : with > target && before <= target;
+          if (here) {
+            S.found = key;
+            S.sum = sum;
+          }
+        }
+        __syncthreads();
+        return;
+      }
+      // the interval of the keys, then bins of it
+      uint64_t lo = ~uint64_t{0}, hi = 0;
+      each_key([&](float x, uint64_t key) {
+        if (bin_of(x) != bin || key < klo || key > khi) return;
+        lo = min(lo, key);
+        hi = max(hi, key);
+      });
+      for (int d = 1; d < 64; d <<= 1) {
+        lo = min(lo, shfl_xor64(lo, d));
+        hi = max(hi, shfl_xor64(hi, d));
+      }
+      if (lane == 0) {
+        S.part[wave] = lo;
+        S.part2[wave] = hi;
+      }
+      for (int b = tid; b < kBins; b += NT) {
+        S.mass2[b] = 0;
+        S.count2[b] = 0;
+      }
+      __syncthreads();
+      for (int w = 0; w < NT / 64; ++w) {
+        lo = min(lo, S.part[w]);
+        hi = max(hi, S.part2[w]);
+      }
+      klo = lo;
+      khi = hi;
+      const int bits = max(64 - __clzll(static_cast<long long>(khi - klo)) - 10, 0);  // khi > klo: keys differ
+      each_key([&](float x, uint64_t key) {
+        if (bin_of(x) != bin || key < klo || key > khi) return;
+        const int b = static_cast<int>((khi - key) >> bits);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&S.mass2[b]),
+                  static_cast<unsigned long long>(weight_of(t_of(x), P.shift)));
+        atomicAdd(&S.count2[b], 1u);
+      });
+      __syncthreads();
+      scan(S.mass2, S.count2, true);
+      find_bin(S.mass2, S.count2, true, mode, base, base_count, target);
+      base = S.base;
+      base_count = S.base_count;
+      const uint64_t top = khi - (static_cast<uint64_t>(S.bin) << bits);
+      const uint64_t width = (uint64_t{1} << bits) - 1;
+      klo = top - klo > width ? top - width : klo;
+      khi = top;
+      __syncthreads();  // S.bin has been read
+    }
+  };
+
+  uint64_t z = S.mass[kBins - 1];
+  for (int step = 0; step < 3; ++step) {
+    Cross mode = kExceed;
+    double target;
+    if (step == 0) {
+      if (!by_count || static_cast<uint32_t>(k) >= S.count[kBins - 1]) continue;
+      mode = kCount;
+      target = k;
+    } else if (step == 1) {
+      if (!(top_p < 1.f)) continue;
+      mode = kReach;
+      target = fmax(static_cast<double>(top_p) * static_cast<double>(z), 0.5);
+    } else {
+      if (by_min) z = min(z, z_min);
+      // u is held to [0, 1 - 2^-24] (a NaN to 0)
+      target = static_cast<double>(fminf(fmaxf(u, 0.f), 0x1.fffffep-1f)) * static_cast<double>(z);
+    }
+    cross(mode, target);
+    if (step < 2) {
+      z = S.sum;
+      __syncthreads();
+    }
+  }
+  if (tid == 0) {
+    const uint64_t key = S.found;
+    P.token[item] = 0xffffffffu - static_cast<uint32_t>(key);
+    P.logprob[item] = static_cast<float>(-t_of(value_of(key)) * kLn2 - log(__builtin_ldexp(static_cast<double>(z), -P.shift)));
+  }
+}
+
+template <bool kWide>
+void launch(const SampleParams& P, hipStream_t st) {
+  if (P.vocab <= 16384)
+    hipLaunchKernelGGL((sample_kernel<kWide, 256>), dim3(P.items), dim3(256), 0, st, P);
+  else
+    hipLaunchKernelGGL((sample_kernel<kWide, 1024>), dim3(P.items), dim3(1024), 0, st, P);
+}
+
+}  // namespace
+}  // namespace yapd
+
+extern "C" int yapd_sample_tokens(const void* logits, int wide, int64_t seq_stride, int64_t pos_stride, int rows, int bl,
+                                  int vocab, const float* uniform, const float* temperature, float temperature_all,
+                                  const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all,
+                                  const float* min_p, float min_p_all, int64_t* token, float* logprob, void* stream) {
+  YAPD_REQUIRE(rows >= 0 && bl >= 0, "sample_tokens: need rows and bl >= 0 (got %d, %d)", rows, bl);
+  const int64_t items = static_cast<int64_t>(rows) * bl;
+  YAPD_REQUIRE(items < (int64_t{1} << 22), "sample_tokens: rows * bl must be below 2^22");
+  YAPD_REQUIRE(vocab >= 1 && vocab <= (1 << 24), "sample_tokens: need 1 <= vocab <= 2^24 (got %d)", vocab);
+  YAPD_REQUIRE(temperature || temperature_all >= 0.f, "sample_tokens: temperature must be >= 0");
+  YAPD_REQUIRE(top_p || top_p_all == top_p_all, "sample_tokens: top_p is NaN");
+  YAPD_REQUIRE(min_p || min_p_all == min_p_all, "sample_tokens: min_p is NaN");
+  if (items == 0) return YAPD_OK;
+  YAPD_REQUIRE(logits && uniform && token && logprob, "sample_tokens: NULL pointer");
+  YAPD_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (wide ? 3u : 1u)) == 0, "sample_tokens: misaligned logits");
+  int bits = 0;  // vocab <= 2^bits, so that all weights together stay below 2^63
+  while ((int64_t{1} << bits) < vocab) ++bits;
+  const yapd::SampleParams P{logits, seq_stride, pos_stride, static_cast<uint32_t>(items), static_cast<uint32_t>(bl), vocab,
+                             62 - bits < 51 ? 62 - bits : 51, uniform, temperature, temperature_all, top_k, top_k_all, top_p,
+                             top_p_all, min_p, min_p_all, token, logprob};
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (wide)
+    yapd::launch<true>(P, st);
+  else
+    yapd::launch<false>(P, st);
+  YAPD_LAUNCH_CHECK("sample_kernel launch");
+  return YAPD_OK;
+}

@@ -35,6 +35,8 @@ _SIGNATURES = {
         c_float, c_int, c_u64, c_u64, c_void, c_void, c_void, c_void, c_void, c_void, c_void]),
     "yapd_token_logprobs": (c_int, [c_void, c_int, c_i64, c_i64, c_int, c_int, c_int, c_void, c_int, c_void, c_void,
                                     c_void, c_void, c_void]),
+    "yapd_sample_tokens": (c_int, [c_void, c_int, c_i64, c_i64, c_int, c_int, c_int, c_void, c_void, c_float, c_void,
+                                   c_int, c_void, c_float, c_void, c_float, c_void, c_void, c_void]),
     "yapd_attn_plan": (c_int, [c_void, c_int, c_int, c_int, c_void, c_int, c_void, c_int, c_void, c_void, c_void]),
     "yapd_attn_paged_block": (c_int, [
         c_void, c_void, c_i64, c_void, c_int, c_int, c_void, c_int, c_int, c_int, c_void, c_int, c_void, c_int,
@@ -295,6 +297,40 @@ def launch_token_logprobs(logits, tokens, k: int, logprob, entropy, top_logprob,
     check(load_library().yapd_token_logprobs(
         logits.data_ptr(), logits.dtype == torch.float32, seq, pos, rows, bl, shape[-1], tokens.data_ptr(), k,
         logprob.data_ptr(), entropy.data_ptr(), ptr(top_logprob), ptr(top_token), stream_ptr(logits.device)))
+
+
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, token: torch.Tensor, logprob: torch.Tensor, *,
+                  temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> None:
+    """A token drawn from every row of ``logits`` with the random number ``uniform`` (``yapd_sample_tokens``), into
+    caller tensors; see :func:`yapd_amd.scoring.sample_tokens`."""
+    dev = logits.device
+    if logits.is_cuda and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):  # the launch goes to the current device
+            return sample_tokens(logits, uniform, token, logprob, temperature=temperature, top_k=top_k, top_p=top_p,
+                                 min_p=min_p)
+    f32, shape, stride = torch.float32, logits.shape, logits.stride()
+    require_cuda(logits, "logits", f32 if logits.dtype == f32 else torch.bfloat16, dev, contiguous=False)
+    require(len(shape) in (2, 3) and (shape[-1] <= 1 or stride[-1] == 1),
+            "logits must be [n, V] or [rows, bl, V] with unit last stride")
+    lead = shape[:-1]
+    args = []
+    for name, t, dtype in (("uniform", uniform, f32), ("temperature", temperature, f32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, f32), ("min_p", min_p, f32), ("token", token, torch.int64),
+                           ("logprob", logprob, f32)):
+        if isinstance(t, torch.Tensor):
+            require_cuda(t, name, dtype, dev)
+            if t.shape != lead:
+                raise ValueError(f"{name} must have the logits' leading shape")
+            args.append((t.data_ptr(), 0))
+        else:
+            require(name not in ("uniform", "token", "logprob"), f"{name} must be a tensor")
+            args.append((None, t))
+    (u, _), (t, t_all), (k, k_all), (p, p_all), (m, m_all), (tok, _), (lp, _) = args
+    require(k_all == int(k_all), "top_k must be an integer")
+    rows, bl = (shape[0], 1) if len(shape) == 2 else lead
+    check(load_library().yapd_sample_tokens(
+        logits.data_ptr(), logits.dtype == f32, stride[0], 0 if len(shape) == 2 else stride[1], rows, bl, shape[-1], u, t,
+        t_all, k, max(min(int(k_all), 2**31 - 1), 0), p, p_all, m, m_all, tok, lp, stream_ptr(dev)))
 
 
 # --------------------------------------------------------------------------- #

@@ -96,6 +96,30 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
     return TokenLogprobs(logprob, entropy, top_logprob, top_token)
 
 
+@dataclass
+class SampledTokens:
+    token: torch.Tensor    # [...] int64  (-1: the row holds no distribution)
+    logprob: torch.Tensor  # [...] fp32   ln of the token's share of what the filters keep
+
+
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0,
+                  min_p=0.0) -> SampledTokens:
+    """A token of every row of ``logits``, drawn with the given random numbers ``uniform`` (``yapd_sample_tokens``).
+
+    ``logits`` is bf16 or fp32, ``[n, V]`` or ``[rows, bl, V]`` with a unit last stride; ``uniform`` (fp32, in [0, 1)) has its
+    leading shape.  Each setting is a number, or a device tensor of that shape with one for every row (fp32; ``top_k``
+    int32).  Tokens stand in order, the larger logit first, of equal ones the lower index, with weights
+    ``exp((x - max) / temperature)``; of these are kept the first ``top_k`` (0: all), of those the fewest whose weight is at
+    least ``top_p`` of theirs (1: all), and of these the ones whose weight is at least ``min_p`` of the first's (0: all).
+    The token is the first at which the weights' running sum exceeds ``uniform`` of the weight kept.
+    ``temperature`` 0 gives the largest logit.  Logits of -inf are never drawn; a row that holds a
+    NaN or +inf, or -inf alone, gives token -1 and log probability NaN."""
+    token = torch.empty(logits.shape[:-1], dtype=torch.int64, device=logits.device)
+    logprob = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
+    kernels.sample_tokens(logits, uniform, token, logprob, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    return SampledTokens(token, logprob)
+
+
 class BlockScorer:
     """Persistent buffers + launcher for one block size and batch.
 
