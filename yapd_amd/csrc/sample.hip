@@ -89,12 +89,22 @@ __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d) {
 
 enum Cross { kCount, kReach, kExceed };  // the first element whose inclusive count, or sum, is at least, or exceeds, a target
 
+constexpr int kValues = 4096;             // bins of the bf16 form: one a value, 2047 on either side of the tiny ones
+constexpr int kTiny = kValues / 2, kLow = kValues - 1;
+constexpr int kFloor = (127 - 10) * 128;  // |x| <= 2^-10 is tiny, 64 and above high: bits of the usual window's floor
+
 template <int NT>
 struct Shared {
-  uint64_t mass[kBins], mass2[kBins];
-  uint32_t count[kBins], count2[kBins];
+  union {
+    struct {
+      uint64_t mass[kBins], mass2[kBins];
+      uint32_t count[kBins], count2[kBins];
+    };
+    uint32_t values[kValues];
+  };
   uint64_t key[kList], w[kList];
   uint64_t part[NT / 64], part2[NT / 64], z_min[NT / 64];
+  double sum_a[NT / 64], sum_b[NT / 64];
   float fmx[NT / 64], fmn[NT / 64];
   uint32_t n, bad;
   // what a search found
@@ -102,11 +112,452 @@ struct Shared {
   uint64_t base, sum;
   uint32_t base_count;
   uint64_t found;
+  // the bf16 form's
+  uint32_t first, bits, nth, ties, mixed;
+  double z;
 };
+
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// 2^-t in 64 bits (0 from t = 1000 on), t >= 0: weight_of's polynomial.
+__device__ __forceinline__ double exp2_neg(double t) {
+  t = fmin(t, 1000.0);
+  const double r = __builtin_rint(t), a = (r - t) * kLn2;
+  double p = 1.0 / 3628800;
+  p = __builtin_fma(p, a, 1.0 / 362880);
+  p = __builtin_fma(p, a, 1.0 / 40320);
+  p = __builtin_fma(p, a, 1.0 / 5040);
+  p = __builtin_fma(p, a, 1.0 / 720);
+  p = __builtin_fma(p, a, 1.0 / 120);
+  p = __builtin_fma(p, a, 1.0 / 24);
+  p = __builtin_fma(p, a, 1.0 / 6);
+  p = __builtin_fma(p, a, 0.5);
+  p = __builtin_fma(p, a, 1.0);
+  p = __builtin_fma(p, a, 1.0);
+  return t >= 1000.0 ? 0.0 : __builtin_ldexp(p, -static_cast<int>(r));
+}
+
+struct Settings {
+  float T;
+  int k;
+  float top_p, min_p, u;
+};
+
+// Rows of bf16 logits, where a bin is one value: 16 octaves of positive and of negative values from a floor 2^f on, with
+// a bin for what is smaller in magnitude (tiny; also high and low, beyond the window).  Elements are only counted; a
+// bin's weight is its count times its value's, the values of 16 consecutive bins being an arithmetic progression
+// (so their weights are a geometric one), and of equal logits the n-th is found by division.  No element's weight
+// is computed but those of the tiny and low ones, in a pass of their own that most rows do without or fill with
+// masked tokens.  false: the token is among several values of such a bin.
+template <int NT, int RD>
+__device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>& S, const u32x4_t* granules, int off,
+                                              int n_gran, const Settings& s, uint32_t item) {
+  constexpr int kPer = kValues / NT;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int V = P.vocab;
+  const uint32_t pads = static_cast<uint32_t>(n_gran * 8 - V);
+  auto fetch = [&](int gi) {
+    u32x4_t v = granules[gi];
+    if (gi == 0 || gi == n_gran - 1) {  // what a granule holds beside the row: -inf
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int i = gi * 8 + e - off;
+        if (i < 0 || i >= V)
+          v[e >> 1] = (v[e >> 1] & (e & 1 ? 0x0000ffffu : 0xffff0000u)) | (e & 1 ? 0xff800000u : 0x0000ff80u);
+      }
+    }
+    return v;
+  };
+  // The row in tiles of RD granules a thread, requested together; a row of one tile stays in registers.
+  u32x4_t held[RD];
+  auto load_tile = [&](int t0) {
+#pragma unroll
+    for (int j = 0; j < RD; ++j) {
+      const int gi = t0 + tid + j * NT;
+      if (gi < n_gran) held[j] = fetch(gi);
+    }
+  };
+  load_tile(0);
+  auto each = [&](auto f) {
+    for (int t0 = 0; t0 < n_gran; t0 += NT * RD) {
+      if (n_gran > NT * RD) load_tile(t0);
+#pragma unroll
+      for (int j = 0; j < RD; ++j)
+        if (t0 + tid + j * NT < n_gran) f(held[j], (t0 + tid + j * NT) * 8 - off);
+    }
+  };
+  int fl = kFloor;
+  // a word's two magnitudes in values above the floor, 0 for tiny ones
+  auto above_floor = [&](u16x2 m) {
+    const u16x2 f = {static_cast<unsigned short>(fl), static_cast<unsigned short>(fl)};
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(m, f) - f);
+  };
+  // their bins: kTiny less that number, with the sign
+  auto bins_of = [&](uint32_t word, uint32_t above) {
+    const s16x2 sign = __builtin_bit_cast(s16x2, word) >> 15;
+    const s16x2 y = (__builtin_bit_cast(s16x2, above) ^ sign) - sign;
+    const s16x2 mid = {kTiny, kTiny}, top = {kLow, kLow}, zero = {0, 0};
+    return __builtin_elementwise_max(__builtin_elementwise_min(__builtin_elementwise_sub_sat(mid, y), top), zero);
+  };
+  auto value_of_bin = [&](int b) {
+    const int y = kTiny - b;
+    return __uint_as_float(static_cast<uint32_t>(fl + (y < 0 ? -y : y)) << 16 | (y < 0 ? 0x80000000u : 0u));
+  };
+
+  uint32_t c[kPer];  // elements of this thread's bins, tid * kPer and on
+  float mx = 0.f;
+  uint32_t tiny, low;
+  for (int round = 0;; ++round) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) S.values[tid + j * NT] = 0;
+    if (tid == 0) {
+      S.first = kValues;
+      S.bad = S.n = 0;
+    }
+    __syncthreads();
+    u16x2 most = {0, 0};  // magnitudes: above 0x7f80 a NaN's
+    each([&](const u32x4_t& v, int) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const u16x2 m = __builtin_bit_cast(u16x2, v[w] & 0x7fff7fffu);
+        most = __builtin_elementwise_max(most, m);
+        const uint32_t c = above_floor(m);
+        const s16x2 b = bins_of(v[w], c);
+        atomicAdd(&S.values[b[0]], 1u);
+        atomicAdd(&S.values[b[1]], 1u);
+        if ((c - 0x00010001u) & ~c & 0x80008000u) {  // a tiny value
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t bits = e ? v[w] >> 16 : v[w] & 0xffffu;
+            if (static_cast<int>(bits & 0x7fffu) > fl || (bits & 0x7fffu) == 0) continue;
+            const uint32_t to = atomicAdd(&S.n, 1u);
+            if (to < kList) S.key[to] = bits;
+          }
+        }
+      }
+    });
+    if (__any(most[0] > 0x7f80 || most[1] > 0x7f80) && lane == 0) atomicOr(&S.bad, 1u);
+    __syncthreads();
+    if (S.bad) {
+      if (tid == 0) {
+        P.token[item] = -1;
+        P.logprob[item] = __builtin_nanf("");
+      }
+      return true;
+    }
+    uint32_t first = kValues;
+#pragma unroll
+    for (int j = 0; j < kPer; j += 4) {
+      const u32x4_t four = *reinterpret_cast<const u32x4_t*>(&S.values[tid * kPer + j]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[j + i] = four[i];
+    }
+    if (tid == NT - 1) c[kPer - 1] -= pads;  // pads count as low
+#pragma unroll
+    for (int j = kPer - 1; j >= 0; --j)
+      if (c[j]) first = tid * kPer + j;
+    for (int d = 1; d < 64; d <<= 1) first = min(first, __shfl_xor(first, d));
+    if (lane == 0) atomicMin(&S.first, first);
+    tiny = S.values[kTiny];
+    low = S.values[kLow] - pads;
+    const uint32_t high = S.values[0];
+    __syncthreads();
+    first = S.first;
+    if (high == 0 && first != kTiny && first != kLow) {
+      mx = value_of_bin(first);
+      break;
+    }
+    if (round > 0) break;  // the largest is 0 and the first bin the tiny one
+    // a window around the largest logit
+    float m = -INFINITY;
+    each([&](const u32x4_t& v, int) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) m = fmaxf(m, fmaxf(bf16lo(v[w]), bf16hi(v[w])));
+    });
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    if (lane == 0) S.fmx[wave] = m;
+    __syncthreads();
+    for (int w = 0; w < NT / 64; ++w) m = fmaxf(m, S.fmx[w]);
+    if (fabsf(m) == INFINITY) {
+      if (tid == 0) {
+        P.token[item] = -1;
+        P.logprob[item] = __builtin_nanf("");
+      }
+      return true;
+    }
+    mx = m + 0.f;
+    const int mag = static_cast<int>(__float_as_uint(m) >> 16 & 0x7fffu);
+    if (mx > 0.f)
+      fl = max((mag - 2047 + 127) & ~127, 0);
+    else if (mx < 0.f)
+      fl = (mag - 1) & ~127;
+    if (fl + 2047 > 0x7f80) return false;  // -inf would not be low
+    __syncthreads();
+  }
+
+  const bool greedy = !(s.T > 0.f) || s.k == 1;
+  const double scale = greedy ? 0.0 : kLog2e / static_cast<double>(s.T);
+  auto t_of = [&](float x) { return (static_cast<double>(mx) - static_cast<double>(x)) * scale; };
+  const bool by_min = s.min_p > 0.f;
+  const double min_p = fminf(s.min_p, 1.f);
+
+  // Tiny values other than 0 were listed; low ones are -inf, or weigh nothing next to the largest, or else are counted
+  // one by one below (by returning false).
+  double tiny_mass = 0.0, tiny_min = 0.0;
+  const uint32_t listed = S.n;
+  if (tiny && !greedy) {
+    if (listed > kList) return false;
+    const double zero = exp2_neg(t_of(0.f));
+    tiny_mass = static_cast<double>(tiny - listed) * zero;
+    tiny_min = zero >= min_p ? tiny_mass : 0.0;
+    if (listed) {  // every thread adds them up in one order: by their bits (equal ones weigh the same)
+      for (uint32_t i = tid; i < listed; i += NT) {
+        const uint64_t mine = S.key[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < listed; ++j) rank += S.key[j] < mine || (S.key[j] == mine && j < i);
+        S.w[rank] = mine;
+      }
+      __syncthreads();
+      for (uint32_t i = 0; i < listed; ++i) {
+        const double w = exp2_neg(t_of(__uint_as_float(static_cast<uint32_t>(S.w[i]) << 16)));
+        tiny_mass += w;
+        tiny_min += w >= min_p ? w : 0.0;
+      }
+    }
+  }
+  if (low && !greedy) {
+    // the weight of all low elements is below 2^-60 of the largest's: what top-k and top-p keep of them counts for nothing
+    const double t = t_of(-__uint_as_float(static_cast<uint32_t>(fl + 2047) << 16));
+    if (t < 60.0 + 24.0) {
+      bool finite = false;
+      each([&](const u32x4_t& v, int) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const s16x2 b = bins_of(v[w], above_floor(__builtin_bit_cast(u16x2, v[w] & 0x7fff7fffu)));
+          finite |= (b[0] == kLow && (v[w] & 0xffffu) != 0xff80u) || (b[1] == kLow && v[w] >> 16 != 0xff80u);
+        }
+      });
+      if (__any(finite) && lane == 0) atomicOr(&S.bad, 1u);
+      __syncthreads();
+      if (S.bad) return false;
+    }
+  }
+  if (tid == 0) S.mixed = listed != 0;
+
+  double z = 1.0;
+  if (greedy) {
+    if (tid == 0) {
+      S.bits = __float_as_uint(mx) >> 16;
+      S.nth = 1;
+      S.ties = S.values[S.first];
+    }
+    __syncthreads();
+    if (mx == 0.f && S.mixed) return false;
+  } else {
+    const int b0 = tid * kPer;
+    const double tiny_each = listed ? 0.5 : exp2_neg(fmax(t_of(0.f), 0.0));  // with others than 0 among them not used
+    // The weights of this thread's values, from the first that occurs on: a progression of ratio r.  f(j, count, weight, mass).
+    double w_first = 0.0, r = 0.0;
+    int j_first = kPer;
+#pragma unroll
+    for (int j = kPer - 1; j >= 0; --j)
+      if (c[j] && b0 + j != kTiny && b0 + j != kLow) j_first = j;  // what is low counts for nothing
+    if (j_first < kPer) {
+      w_first = exp2_neg(t_of(value_of_bin(b0 + j_first)));
+      r = exp2_neg((static_cast<double>(value_of_bin(b0 + 1)) - static_cast<double>(value_of_bin(b0 + 2))) * scale);
+    }
+    auto each_value = [&](auto f) {
+      double w = w_first;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int b = b0 + j;
+        const uint32_t n = b == kLow ? 0 : c[j];
+        if (j == 0 && b == kTiny) {
+          f(b, n, tiny_each, tiny_mass);
+        } else if (j >= j_first) {
+          f(b, n, w, n * w);
+          w *= r;
+        }
+      }
+    };
+    double mass = 0.0, min_mass = 0.0;
+    uint32_t n = 0;
+    each_value([&](int b, uint32_t count, double w, double m) {
+      mass += m;
+      n += count;
+      if (by_min && b != kTiny && w >= min_p) min_mass += m;
+    });
+    double mi = mass;
+    uint32_t ni = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const double ml = __shfl_up(mi, d);
+      const uint32_t nl = __shfl_up(ni, d);
+      if (lane >= d) {
+        mi += ml;
+        ni += nl;
+      }
+    }
+    if (by_min)
+      for (int d = 1; d < 64; d <<= 1) min_mass += __shfl_xor(min_mass, d);
+    if (lane == 63) {
+      S.sum_b[wave] = mi;
+      S.part[wave] = ni;
+      S.sum_a[wave] = min_mass;
+    }
+    double me = __shfl_up(mi, 1);
+    uint32_t ne = __shfl_up(ni, 1);
+    if (lane == 0) me = ne = 0;
+    __syncthreads();
+    double before = 0.0, total = 0.0, z_min = tiny_min;
+    uint32_t n_before = 0, n_total = 0;
+    for (int w = 0; w < NT / 64; ++w) {
+      if (w == wave) {
+        before = total;
+        n_before = n_total;
+      }
+      total += S.sum_b[w];
+      z_min += S.sum_a[w];
+      n_total += static_cast<uint32_t>(S.part[w]);
+    }
+    me += before;  // the sums up to this thread's values; a thread's end is the next one's begin to the last bit
+    mi += before;
+    ne += n_before;
+    ni += n_before;
+
+    z = total;
+    const bool by_count = s.k > 0 && static_cast<uint32_t>(s.k) < n_total;
+#pragma unroll 1
+    for (int step = 0; step < 3; ++step) {
+      Cross mode = kExceed;
+      double target;
+      if (step == 0) {
+        if (!by_count) continue;
+        mode = kCount;
+        target = s.k;
+      } else if (step == 1) {
+        if (!(s.top_p < 1.f)) continue;
+        mode = kReach;
+        target = fmax(static_cast<double>(s.top_p) * z, 1e-30);
+      } else {
+        if (by_min) z = fmin(z, z_min);
+        target = static_cast<double>(fminf(fmaxf(s.u, 0.f), 0x1.fffffep-1f)) * z;
+      }
+      const bool here = mode == kCount   ? ne < target && ni >= target
+                        : mode == kReach ? me < target && mi >= target
+                                         : me <= target && mi > target;
+      if (here) {  // one thread: the value at which the target is met, else (by rounding) the last that occurs
+        double run = me, base = me, w1 = 0.0;
+        double count = ne, base_n = ne;
+        int at = b0;
+        uint32_t ties = 0;
+        bool met = false;
+        each_value([&](int b, uint32_t c, double w, double m) {
+          if (met || c == 0 || (mode != kCount && w == 0.0)) return;
+          at = b;
+          ties = c;
+          w1 = w;
+          base = run;
+          base_n = count;
+          run += m;
+          count += c;
+          met = mode == kCount ? count >= target : mode == kReach ? run >= target : run > target;
+        });
+        double nth;
+        if (mode == kCount) {
+          nth = target - base_n;
+        } else {
+          nth = mode == kReach ? ceil((target - base) / w1) : floor((target - base) / w1) + 1.0;
+          const double with = __builtin_fma(nth, w1, base), less = __builtin_fma(nth - 1.0, w1, base);
+          if (mode == kReach ? less >= target : less > target)
+            nth -= 1.0;
+          else if (mode == kReach ? with < target : with <= target)
+            nth += 1.0;
+          nth = fmin(fmax(nth, 1.0), static_cast<double>(ties));
+        }
+        if (at == kTiny && S.mixed) S.mixed = 2;
+        S.bits = at == kTiny ? 0u : __float_as_uint(value_of_bin(at)) >> 16;
+        S.nth = static_cast<uint32_t>(nth);
+        S.ties = ties;
+        S.z = __builtin_fma(nth, w1, base);
+      }
+      __syncthreads();
+      if (S.mixed == 2) return false;
+      if (step < 2) {
+        z = S.z;
+        __syncthreads();
+      }
+    }
+  }
+
+  // the nth element of these bits (0: of either zero), in the order of the row
+  const uint32_t bits = S.bits, nth = S.nth, ties = S.ties;
+  const uint32_t both = bits << 16 | bits, care = bits ? 0xffffffffu : 0x7fff7fffu;
+  auto store = [&](int64_t token) {
+    P.token[item] = token;
+    P.logprob[item] = greedy ? 0.f : static_cast<float>(-t_of(__uint_as_float(bits << 16)) * kLn2 - log(z));
+  };
+  if (ties <= kList) {
+    if (tid == 0) S.n = 0;
+    __syncthreads();
+    each([&](const u32x4_t& v, int i0) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t d = (v[w] ^ both) & care;
+        if ((d & 0xffffu) == 0) S.key[atomicAdd(&S.n, 1u) % kList] = i0 + 2 * w;
+        if ((d >> 16) == 0) S.key[atomicAdd(&S.n, 1u) % kList] = i0 + 2 * w + 1;
+      }
+    });
+    __syncthreads();
+    for (uint32_t i = tid; i < ties; i += NT) {
+      const uint64_t mine = S.key[i];
+      uint32_t rank = 0;
+      for (uint32_t j = 0; j < ties; ++j) rank += S.key[j] < mine;
+      if (rank == nth - 1) store(static_cast<int64_t>(mine));
+    }
+    return true;
+  }
+  uint32_t seen = 0;
+  for (int g0 = 0; g0 < n_gran; g0 += NT) {
+    const int gi = g0 + tid;
+    uint32_t n = 0, match = 0;
+    if (gi < n_gran) {
+      const u32x4_t v = fetch(gi);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t d = (v[e >> 1] ^ both) & care;
+        match |= (e & 1 ? d >> 16 : d & 0xffffu) == 0 ? 1u << e : 0u;
+      }
+      n = __popc(match);
+    }
+    uint32_t ni = n;
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t l = __shfl_up(ni, d);
+      if (lane >= d) ni += l;
+    }
+    __syncthreads();
+    if (lane == 63) S.part[wave] = ni;
+    __syncthreads();
+    uint32_t before = seen, after = seen;
+    for (int w = 0; w < NT / 64; ++w) {
+      if (w == wave) before = after;
+      after += static_cast<uint32_t>(S.part[w]);
+    }
+    const uint32_t left = nth - (before + ni - n);  // the wanted one's place among this thread's
+    if (before + ni - n < nth && nth <= before + ni) {
+      for (uint32_t i = 1; i < left; ++i) match &= match - 1;
+      store(gi * 8 - off + __ffs(match) - 1);
+    }
+    seen = after;
+    if (seen >= nth) break;
+  }
+  return true;
+}
 
 // One workgroup a row, which every pass reads again (from the caches: a speech vocabulary's row is 16 KB).
 template <bool kWide, int NT>
-__global__ __launch_bounds__(NT) void sample_kernel(const SampleParams P) {
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sample_kernel(const SampleParams P) {
   constexpr int G = kWide ? 4 : 8, kBytes = kWide ? 4 : 2;
   __shared__ Shared<NT> S;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -165,6 +616,10 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleParams P) {
   const float top_p = P.top_p ? P.top_p[item] : P.top_p_all;
   const float min_p = P.min_p ? P.min_p[item] : P.min_p_all;
   const float u = P.u[item];
+  if constexpr (!kWide) {
+    if (sample_values<NT, NT == 256 ? 5 : 4>(P, S, granules, off, n_gran, Settings{T, k, top_p, min_p, u}, item)) return;
+    __syncthreads();
+  }
   for (int b = tid; b < kBins; b += NT) {
     S.mass[b] = 0;
     S.count[b] = 0;
