@@ -57,10 +57,23 @@ __device__ __forceinline__ float value_of(uint64_t key) {
   return __uint_as_float(o ^ (o >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
+// The largest and the least of three without quieting the operands first (they come from memory, so the compiler
+// would); a NaN operand is left out.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // 2^-t as a multiple of 2^-shift, for t >= 0: with r = t rounded, f = t - r, the Taylor polynomial of e^(-f ln 2)
 // (|f ln 2| <= 0.347: off by 2e-13), rounded to an integer by adding 2^52.
 __device__ __forceinline__ uint64_t weight_of(double t, int shift) {
-  t = fmin(t, 1000.0);
+  t = fmin(t, 100.0);  // 0 from 64 on
   const double r = __builtin_rint(t);
   const double a = (r - t) * kLn2;
   double p = 1.0 / 3628800;
@@ -156,35 +169,35 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
   constexpr int kPer = kValues / NT;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int V = P.vocab;
-  const uint32_t pads = static_cast<uint32_t>(n_gran * 8 - V);
-  auto fetch = [&](int gi) {
-    u32x4_t v = granules[gi];
-    if (gi == 0 || gi == n_gran - 1) {  // what a granule holds beside the row: -inf
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int i = gi * 8 + e - off;
-        if (i < 0 || i >= V)
-          v[e >> 1] = (v[e >> 1] & (e & 1 ? 0x0000ffffu : 0xffff0000u)) | (e & 1 ? 0xff800000u : 0x0000ff80u);
-      }
-    }
-    return v;
-  };
-  // The row in tiles of RD granules a thread, requested together; a row of one tile stays in registers.
-  u32x4_t held[RD];
+  // Granules that the row fills, in tiles of RD a thread, requested together (a row of one tile stays in registers), and
+  // those it fills in part, one each of the first two threads, with -inf for what is beside the row.
+  const int f0 = off > 0 ? 1 : 0, n_full = max((off + V) / 8 - f0, 0);
+  const bool tail = (off + V) % 8 != 0 && (n_gran > 1 || off == 0);
+  const bool has_edge = (tid == 0 && off > 0) || (tid == 1 && tail);
+  const int edge_gi = tid == 0 ? 0 : n_gran - 1;
+  const uint32_t pads = static_cast<uint32_t>((f0 + (tail ? 1 : 0)) * 8 - (V - n_full * 8));
+  u32x4_t held[RD], edge = {0, 0, 0, 0};
   auto load_tile = [&](int t0) {
 #pragma unroll
-    for (int j = 0; j < RD; ++j) {
-      const int gi = t0 + tid + j * NT;
-      if (gi < n_gran) held[j] = fetch(gi);
-    }
+    for (int j = 0; j < RD; ++j) held[j] = granules[f0 + min(t0 + tid + j * NT, max(n_full - 1, 0))];
   };
   load_tile(0);
+  if (has_edge) {
+    edge = granules[edge_gi];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = edge_gi * 8 + e - off;
+      if (i < 0 || i >= V)
+        edge[e >> 1] = (edge[e >> 1] & (e & 1 ? 0x0000ffffu : 0xffff0000u)) | (e & 1 ? 0xff800000u : 0x0000ff80u);
+    }
+  }
   auto each = [&](auto f) {
-    for (int t0 = 0; t0 < n_gran; t0 += NT * RD) {
-      if (n_gran > NT * RD) load_tile(t0);
+    if (has_edge) f(edge, edge_gi * 8 - off);
+    for (int t0 = 0; t0 < n_full; t0 += NT * RD) {
+      if (n_full > NT * RD) load_tile(t0);
 #pragma unroll
       for (int j = 0; j < RD; ++j)
-        if (t0 + tid + j * NT < n_gran) f(held[j], (t0 + tid + j * NT) * 8 - off);
+        if (t0 + tid + j * NT < n_full) f(held[j], (f0 + t0 + tid + j * NT) * 8 - off);
     }
   };
   int fl = kFloor;
@@ -218,22 +231,24 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
     __syncthreads();
     u16x2 most = {0, 0};  // magnitudes: above 0x7f80 a NaN's
     each([&](const u32x4_t& v, int) {
+      u16x2 least = {0xffff, 0xffff};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const u16x2 m = __builtin_bit_cast(u16x2, v[w] & 0x7fff7fffu);
         most = __builtin_elementwise_max(most, m);
-        const uint32_t c = above_floor(m);
-        const s16x2 b = bins_of(v[w], c);
-        atomicAdd(&S.values[b[0]], 1u);
-        atomicAdd(&S.values[b[1]], 1u);
-        if ((c - 0x00010001u) & ~c & 0x80008000u) {  // a tiny value
+        least = __builtin_elementwise_min(least, m);
+        const uint32_t at = __builtin_bit_cast(uint32_t, bins_of(v[w], above_floor(m)) << 2);  // bytes
+        char* const to = reinterpret_cast<char*>(S.values);
+        atomicAdd(reinterpret_cast<uint32_t*>(to + (at & 0xffffu)), 1u);
+        atomicAdd(reinterpret_cast<uint32_t*>(to + (at >> 16)), 1u);
+      }
+      if (min(least[0], least[1]) <= fl) {  // a tiny value
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t bits = e ? v[w] >> 16 : v[w] & 0xffffu;
-            if (static_cast<int>(bits & 0x7fffu) > fl || (bits & 0x7fffu) == 0) continue;
-            const uint32_t to = atomicAdd(&S.n, 1u);
-            if (to < kList) S.key[to] = bits;
-          }
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t bits = e & 1 ? v[e >> 1] >> 16 : v[e >> 1] & 0xffffu;
+          if (static_cast<int>(bits & 0x7fffu) > fl || (bits & 0x7fffu) == 0) continue;
+          const uint32_t to = atomicAdd(&S.n, 1u);
+          if (to < kList) S.key[to] = bits;
         }
       }
     });
@@ -523,11 +538,12 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
     const int gi = g0 + tid;
     uint32_t n = 0, match = 0;
     if (gi < n_gran) {
-      const u32x4_t v = fetch(gi);
+      const u32x4_t v = granules[gi];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
+        const int i = gi * 8 + e - off;
         const uint32_t d = (v[e >> 1] ^ both) & care;
-        match |= (e & 1 ? d >> 16 : d & 0xffffu) == 0 ? 1u << e : 0u;
+        match |= (e & 1 ? d >> 16 : d & 0xffffu) == 0 && i >= 0 && i < V ? 1u << e : 0u;
       }
       n = __popc(match);
     }
@@ -570,8 +586,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   const int n_gran = (off + V + G - 1) / G;
 
   // a granule, what it holds beside the row as -inf
-  auto fetch = [&](int gi) {
-    u32x4_t v = granules[gi];
+  auto whole = [&](u32x4_t v, int gi) {
     if (gi == 0 || gi == n_gran - 1) {
 #pragma unroll
       for (int e = 0; e < G; ++e) {
@@ -592,10 +607,10 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   // f(granule, its first element's index) for every granule of this thread, the next one on its way
   auto each = [&](auto f) {
     if (tid >= n_gran) return;
-    u32x4_t v = fetch(tid);
+    u32x4_t v = granules[tid];
     for (int gi = tid; gi < n_gran; gi += NT) {
-      const u32x4_t next = fetch(min(gi + NT, n_gran - 1));
-      f(v, gi * G - off);
+      const u32x4_t next = granules[min(gi + NT, n_gran - 1)];
+      f(whole(v, gi), gi * G - off);
       v = next;
     }
   };
@@ -617,7 +632,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   const float min_p = P.min_p ? P.min_p[item] : P.min_p_all;
   const float u = P.u[item];
   if constexpr (!kWide) {
-    if (sample_values<NT, NT == 256 ? 5 : 4>(P, S, granules, off, n_gran, Settings{T, k, top_p, min_p, u}, item)) return;
+    if (sample_values<NT, 4>(P, S, granules, off, n_gran, Settings{T, k, top_p, min_p, u}, item)) return;
     __syncthreads();
   }
   for (int b = tid; b < kBins; b += NT) {
@@ -626,17 +641,17 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   }
   if (tid == 0) S.bad = 0;
 
-  // the largest logit, the least of whole granules (it only decides the bins' width), and whether there is a NaN or +inf
+  // the largest logit, the least of whole granules (it only decides the bins' width), and whether there is a NaN
   float mx = -INFINITY, mn = INFINITY;
   bool bad = false;
   each([&](const u32x4_t& v, int i0) {
     float lo = INFINITY;
 #pragma unroll
-    for (int e = 0; e < G; ++e) {
-      const float x = element(v, e);
-      bad |= !(x < INFINITY);
-      mx = fmaxf(mx, x);
-      lo = fminf(lo, x);
+    for (int e = 0; e < G; e += 2) {
+      const float x = element(v, e), y = element(v, e + 1);
+      bad |= x != x || y != y;
+      mx = max3(mx, x, y);
+      lo = min3(lo, x, y);
     }
     if (i0 >= 0 && i0 + G <= V) mn = fminf(mn, lo);
   });
@@ -658,7 +673,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   }
   if (tid == 0) S.n = 0xffffffffu;
   __syncthreads();
-  if (S.bad || mx == -INFINITY) {  // no distribution
+  if (S.bad || fabsf(mx) == INFINITY) {  // no distribution
     if (tid == 0) {
       P.token[item] = -1;
       P.logprob[item] = __builtin_nanf("");
@@ -688,42 +703,9 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   const float per_x = fminf(fmaxf((kBins - 1) / (mx - mn), static_cast<float>((kBins - 1) / 64.0 * scale)), 1e30f);
   auto bin_of = [&](float x) { return static_cast<int>(fminf((mx - x) * per_x, static_cast<float>(kBins - 1))); };
   auto t_of = [&](float x) { return (static_cast<double>(mx) - static_cast<double>(x)) * scale; };
-  const bool by_count = k > 0 && k < V;
+  bool by_count = k > 0 && k < V;
   const bool by_min = min_p > 0.f;
   const double t_min = by_min ? -log2(static_cast<double>(fminf(min_p, 1.f))) : 0.0;
-
-  uint64_t z_min = 0;  // the weight of what min-p keeps
-  uint32_t last = 0;   // elements of the last bin
-  each([&](const u32x4_t& v, int) {
-#pragma unroll
-    for (int e = 0; e < G; ++e) {
-      const float x = element(v, e);
-      if (!(x > -INFINITY)) continue;
-      const int b = bin_of(x);
-      const double t = t_of(x);
-      const uint64_t w = weight_of(t, P.shift);
-      if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&S.mass[b]), static_cast<unsigned long long>(w));
-      if (by_count) {
-        if (b < kBins - 1)
-          atomicAdd(&S.count[b], 1u);
-        else
-          ++last;
-      }
-      if (by_min && t <= t_min) z_min += w;
-    }
-  });
-  if (last) atomicAdd(&S.count[kBins - 1], last);
-  if (by_min) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) z_min += shfl_xor64(z_min, d);
-    if (lane == 0) S.z_min[wave] = z_min;
-  }
-  __syncthreads();
-  if (by_min) {
-    z_min = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) z_min += S.z_min[w];
-  }
 
   // bins' sums and counts become inclusive prefix sums
   auto scan = [&](uint64_t* mass, uint32_t* count, bool counts) {
@@ -764,8 +746,6 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
     }
     __syncthreads();
   };
-  scan(S.mass, S.count, by_count);
-
   // the bin in which the target is met; S.bin, S.base and S.base_count tell, after a barrier
   auto find_bin = [&](const uint64_t* mass, const uint32_t* count, bool counts, Cross mode, uint64_t base, uint32_t base_count,
                       double target) {
@@ -787,6 +767,60 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
     }
     __syncthreads();
   };
+
+  // Weights are needed up to bin `cut`: that of the last element of top-k or, with neither top-k nor top-p, of min-p.
+  int cut = kBins - 1;
+  if (by_count) {
+    uint32_t last = 0;  // elements of the last bin
+    each([&](const u32x4_t& v, int) {
+#pragma unroll
+      for (int e = 0; e < G; ++e) {
+        const float x = element(v, e);
+        if (!(x > -INFINITY)) continue;
+        const int b = bin_of(x);
+        if (b < kBins - 1)
+          atomicAdd(&S.count[b], 1u);
+        else
+          ++last;
+      }
+    });
+    if (last) atomicAdd(&S.count[kBins - 1], last);
+    __syncthreads();
+    scan(S.mass, S.count, true);
+    by_count = static_cast<uint32_t>(k) < S.count[kBins - 1];
+    if (by_count) {
+      find_bin(S.mass, S.count, true, kCount, 0, 0, k);
+      cut = S.bin;
+    }
+  } else if (by_min && !(top_p < 1.f)) {
+    cut = static_cast<int>(fmin(t_min / scale * static_cast<double>(per_x) + 1.0, kBins - 1.0));  // one more for rounding
+  }
+  const float small = static_cast<float>(scale);  // weights from 2^-64 on are 0
+  uint64_t z_min = 0;  // the weight of what min-p keeps
+  each([&](const u32x4_t& v, int) {
+#pragma unroll
+    for (int e = 0; e < G; ++e) {
+      const float x = element(v, e);
+      const int b = bin_of(x);
+      if (b > cut || !(x > -INFINITY) || (mx - x) * small >= 64.f) continue;
+      const double t = t_of(x);
+      const uint64_t w = weight_of(t, P.shift);
+      atomicAdd(reinterpret_cast<unsigned long long*>(&S.mass[b]), static_cast<unsigned long long>(w));
+      if (by_min && t <= t_min) z_min += w;
+    }
+  });
+  if (by_min) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) z_min += shfl_xor64(z_min, d);
+    if (lane == 0) S.z_min[wave] = z_min;
+  }
+  __syncthreads();
+  if (by_min) {
+    z_min = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) z_min += S.z_min[w];
+  }
+  scan(S.mass, S.count, false);
 
   // The element at which the target is met: its key in S.found, the inclusive sum in S.sum, after a barrier.
   auto cross = [&](Cross mode, double target) {
@@ -886,7 +920,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
     Cross mode = kExceed;
     double target;
     if (step == 0) {
-      if (!by_count || static_cast<uint32_t>(k) >= S.count[kBins - 1]) continue;
+      if (!by_count) continue;
       mode = kCount;
       target = k;
     } else if (step == 1) {
@@ -913,7 +947,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
 
 template <bool kWide>
 void launch(const SampleParams& P, hipStream_t st) {
-  if (P.vocab <= 16384)
+  if (P.vocab <= 10000)
     hipLaunchKernelGGL((sample_kernel<kWide, 256>), dim3(P.items), dim3(256), 0, st, P);
   else
     hipLaunchKernelGGL((sample_kernel<kWide, 1024>), dim3(P.items), dim3(1024), 0, st, P);
