@@ -104,8 +104,14 @@ __device__ __forceinline__ u32x2_t bytes_to_bf16(uint32_t four) {
                  __builtin_amdgcn_perm(__float_as_uint(d), __float_as_uint(c), 0x07060302u)};
 }
 
-// Scale byte i of the four in a word as fp32.
-__device__ __forceinline__ float scale_of(uint32_t word, int i) { return kv8_scale(word >> (8 * i) & 0xffu); }
+// The exponent that scale byte i of the four in a word stands for.
+__device__ __forceinline__ int exponent_of(uint32_t word, int i) { return static_cast<int>(word >> (8 * i) & 0xffu) - 127; }
+
+// A product that is rounded wherever it is used: never fused into a sum.
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
 
 // A chunk's loads, as they come.
 template <bool k8>
@@ -150,7 +156,7 @@ struct Chunk<true> {
   u32x4_t kf[4], vf[4], ks, vs;
   const uint8_t *kp, *tile;
   static __device__ __forceinline__ u32x4_t load16b(const uint8_t* p) {
-    return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+    return *reinterpret_cast<const u32x4_t*>(p);  // cached: planes of 1040 bytes share lines with the next head's
   }
   __device__ __forceinline__ void load_k(const TreeParams& P, TreePages& pages, int k0, int h, int g, int n) {
     const int pi = k0 / kPageSize;
@@ -169,16 +175,6 @@ struct Chunk<true> {
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) vf[mt] = load16b(vp + (16 * mt + n) * kPageSize);
   }
-  // codes are finite; a stale scale may be anything: 0 stands for none
-  __device__ __forceinline__ void clear(uint32_t seen) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      uint32_t keep = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) keep |= seen >> (4 * w + i) & 1u ? 0xffu << (8 * i) : 0u;
-      vs[w] &= keep;
-    }
-  }
   static __device__ __forceinline__ int q_dim(int s, int g) { return 16 * g + 8 * s; }
 };
 
@@ -196,7 +192,7 @@ constexpr int kWaveFloats = 4 * 64 * 4;  // a wave's O^T tile in LDS: fragment m
 // W waves a head.  They take the chunks in runs; of rows with more than 16 NQT nodes every other one takes the
 // nodes from 16 NQT on (the host gives those two waves at least), and two waves have each run.
 template <bool k8, int NQT, int W>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(k8 && NQT > 1 ? 2 : 3))) void attn_tree_kernel(const TreeParams P) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NQT > 1 ? 2 : k8 ? 4 : 3))) void attn_tree_kernel(const TreeParams P) {
   using C = Chunk<k8>;
   constexpr int HPW = 4 / W;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -215,74 +211,76 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(k8 && NQT >
   const int q0 = half * 16 * NQT;  // this wave's first node
 
   // Q^T fragments (B operand) and the masks of this lane's queries q0 + qt * 16 + n
-  bf16x8_t qf[NQT][2];
+  u32x4_t qraw[NQT][2];
   uint64_t mask[NQT];
-  int q_lo[NQT];  // context keys from here on are in the node's window
-  const uint64_t nodes = t.n >= 64 ? ~uint64_t{0} : (uint64_t{1} << t.n) - 1;
-  uint64_t any = 0;                     // nodes that some node sees
-  int lo = 0x7fffffff, all_lo = -kCap;  // the first and last window's begin
 #pragma unroll
   for (int qt = 0; qt < NQT; ++qt) {
-    const int q = q0 + qt * 16 + n;
-    const bool live = q < t.qc;
+    const int q = min(q0 + qt * 16 + n, t.qc - 1);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      u32x4_t v = {0u, 0u, 0u, 0u};
-      if (live) v = load16(P.q + (t.qs + q) * P.q_stride + h * kHeadDim + C::q_dim(s, g));
-      qf[qt][s] = as_bf16x8(v);
+    for (int s = 0; s < 2; ++s)
+      qraw[qt][s] = load16(P.q + (t.qs + q) * P.q_stride + h * kHeadDim + C::q_dim(s, g));
+    mask[qt] = static_cast<uint64_t>(P.mask[t.qs + q]);
+  }
+  const uint64_t nodes = t.n >= 64 ? ~uint64_t{0} : (uint64_t{1} << t.n) - 1;
+  int q_lo[NQT];  // context keys from here on are in the node's window
+  int lo = 0, all_lo = -kCap;  // the first and the last window's begin
+#pragma unroll
+  for (int qt = 0; qt < NQT; ++qt) q_lo[qt] = -kCap;
+  if (P.window < kCap) {
+    lo = 0x7fffffff;
+#pragma unroll
+    for (int qt = 0; qt < NQT; ++qt) {
+      const int q = min(q0 + qt * 16 + n, t.qc - 1);  // lanes without a node repeat the last
+      q_lo[qt] = t.ctx + __popcll(mask[qt] & nodes & ~(uint64_t{1} << q)) - P.window + 1;
+      lo = min(lo, q_lo[qt]);
+      all_lo = max(all_lo, q_lo[qt]);
     }
-    mask[qt] = live ? static_cast<uint64_t>(P.mask[t.qs + q]) & nodes : 0;
-    q_lo[qt] = t.ctx + __popcll(mask[qt] & ~(uint64_t{1} << q)) - P.window + 1;
-    any |= mask[qt];
-    lo = live ? min(lo, q_lo[qt]) : lo;
-    all_lo = live ? max(all_lo, q_lo[qt]) : all_lo;
-  }
-  uint32_t any_lo = static_cast<uint32_t>(any), any_hi = static_cast<uint32_t>(any >> 32);
 #pragma unroll
-  for (int d = 1; d < 16; d <<= 1) {
-    any_lo |= __shfl_xor(any_lo, d);
-    any_hi |= __shfl_xor(any_hi, d);
-    lo = min(lo, __shfl_xor(lo, d));
-    all_lo = max(all_lo, __shfl_xor(all_lo, d));
+    for (int d = 1; d < 16; d <<= 1) {
+      lo = min(lo, __shfl_xor(lo, d));
+      all_lo = max(all_lo, __shfl_xor(all_lo, d));
+    }
+    lo = max(__builtin_amdgcn_readfirstlane(lo), 0);
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
   }
-  any_lo = __builtin_amdgcn_readfirstlane(any_lo);
-  any_hi = __builtin_amdgcn_readfirstlane(any_hi);
-  any = static_cast<uint64_t>(any_hi) << 32 | any_lo;
-  lo = max(__builtin_amdgcn_readfirstlane(lo), 0);
-  all_lo = __builtin_amdgcn_readfirstlane(all_lo);
 
   // the list of chunks: entry c is chunk c below n_sink, chunk skip + c from there on; keys seen are below hi
-  const int hi = max(any ? t.ctx + 64 - __clzll(any) : t.ctx, 0);
+  const int hi = t.kvl;
   const int cb = min(lo, hi) / C::kSize, ce = (hi + C::kSize - 1) / C::kSize;
   const int n_sink = min((min(P.sinks, hi) + C::kSize - 1) / C::kSize, cb);
   const int skip = cb - n_sink, n_chunks = n_sink + ce - cb;
   const auto chunk = [&](int c) { return c < n_sink ? c : c + skip; };
 
   f32x4_t o[NQT][4];
-  float m[NQT], l[NQT];
+  float m[NQT], mref[NQT], l[NQT];
 #pragma unroll
   for (int qt = 0; qt < NQT; ++qt) {
     m[qt] = -INFINITY;
-    l[qt] = 0.f;
+    mref[qt] = l[qt] = 0.f;
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) o[qt][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
 
   // this wave's run of the list
-  const int64_t all_runs = static_cast<int64_t>(P.parts) * runs, run = static_cast<int64_t>(part) * runs + run_w;
-  const int c0 = static_cast<int>(n_chunks * run / all_runs), c1 = static_cast<int>(n_chunks * (run + 1) / all_runs);
+  const int all_runs = P.parts * runs, run = part * runs + run_w;
+  const int each_run = n_chunks / all_runs, more_runs = n_chunks - each_run * all_runs;  // the first ones have one more
+  const int c0 = each_run * run + min(run, more_runs), c1 = c0 + each_run + (run < more_runs ? 1 : 0);
+  bf16x8_t qf[NQT][2];
+  const auto take_queries = [&] {
+#pragma unroll
+    for (int qt = 0; qt < NQT; ++qt) {
+      const bool live = q0 + qt * 16 + n < t.qc;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) qf[qt][s] = as_bf16x8(live ? qraw[qt][s] : u32x4_t{0u, 0u, 0u, 0u});
+      mask[qt] = live ? mask[qt] & nodes : 0;
+    }
+  };
   if (c0 < c1) {
     TreePages pages(P, t, row, chunk(c0) * (C::kSize / kPageSize), lane);
     const auto is_edge = [&](int k0) { return k0 + C::kSize > t.ctx || (k0 < all_lo && k0 + C::kSize > P.sinks); };
-    // bit i: some node of the wave sees this lane's key i of the chunk
-    const auto seen_of = [&](int key0) {
-      uint32_t seen = bits_from(any, key0 - t.ctx);
-#pragma unroll
-      for (int i = 0; i < C::kKeys; ++i)
-        if (key0 + i < lo && key0 + i >= P.sinks) seen &= ~(1u << i);
-      return seen;
-    };
-    // the scores of tile qt become weights, against the maximum as it is now; returns the old sums' factor
+    // The scores of tile qt become weights, against the maximum as it is now.  Exponents are taken as s scale - mref, mref
+    // the maximum times scale, rounded once and the same wherever it is used; the old sums are rescaled only where some
+    // query's maximum has moved, by the factor between its references (exactly 1 for the others).
     const auto weights = [&](int qt, int key0, bool edge, float (&sv)[C::kKeys]) {
       if (edge) {
         const uint32_t bits = bits_from(mask[qt], key0 - t.ctx);
@@ -294,39 +292,38 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(k8 && NQT >
 #pragma unroll
       for (int i = 1; i < C::kKeys; ++i) cm = fmaxf(cm, sv[i]);
       cm = max_xor16_32(cm);
-      const float mn = fmaxf(m[qt], cm);
-      // no key seen yet: exponents against 0 give alpha = 0 and p = 0 instead of NaN
-      const float mref = mn == -INFINITY ? 0.f : mn;
-      const float alpha = __builtin_amdgcn_exp2f(m[qt] - mref);
+      if (__any(cm > m[qt])) {
+        m[qt] = fmaxf(m[qt], cm);
+        // no key seen yet: exponents against 0 give weights of 0 instead of NaN
+        const float to = m[qt] == -INFINITY ? 0.f : rounded_product(m[qt], P.scale_log2);
+        const float alpha = __builtin_amdgcn_exp2f(fminf(mref[qt] - to, 0.f));  // a first maximum's is of sums that are 0
+        mref[qt] = to;
+        l[qt] *= alpha;
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) o[qt][mt] *= alpha;
+      }
       float ps = 0.f;
 #pragma unroll
       for (int i = 0; i < C::kKeys; ++i) {
-        sv[i] = __builtin_amdgcn_exp2f(sv[i] - mref);
+        sv[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], P.scale_log2, -mref[qt]));
         ps += sv[i];
       }
-      l[qt] = l[qt] * alpha + ps;
-      m[qt] = mn;
-      return alpha;
+      l[qt] += ps;
     };
     if constexpr (k8) {
       C x;
       x.load_k(P, pages, chunk(c0) * C::kSize, h, g, n);
       x.load_v(P, n);
+      take_queries();
       // A chunk's codes are operands before its products begin, so the registers they came in take the next chunk's.
       auto step = [&](int c, auto more) {
         const int k0 = chunk(c) * C::kSize, key0 = k0 + C::kKeys * g;
         const bool edge = is_edge(k0);  // uniform
-        bf16x8_t kb[4][2];
-        float ksc[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) ksc[i] = scale_of(x.ks[i >> 2], i & 3) * P.scale_log2;
+        bf16x8_t kb[4][2], vb[4][2];
+        const u32x4_t ks = x.ks, vs = x.vs;
 #pragma unroll
         for (int i = 0; i < 4; ++i) codes_to_bf16(x.kf[i], kb[i]);
-        if (edge) x.clear(seen_of(key0));
-        const u32x4_t vs = x.vs;
-        bf16x8_t vb[4][2];
         u32x4_t pw[NQT][2];
-        float alpha[NQT];
 #pragma unroll
         for (int qt = 0; qt < NQT; ++qt) {
           if (qt > 0 && q0 + qt * 16 >= t.qc) break;  // uniform
@@ -335,16 +332,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(k8 && NQT >
           for (int i = 0; i < 4; ++i) {
             f32x4_t s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb[i][0], qf[qt][0], f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
             s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb[i][1], qf[qt][1], s, 0, 0, 0);
-            // s[j] = q n . key key0 + 4 i + j
+            // s[j] = q n . codes of key key0 + 4 i + j
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sv[4 * i + j] = s[j] * ksc[4 * i + j];
+            for (int j = 0; j < 4; ++j) sv[4 * i + j] = __builtin_ldexpf(s[j], exponent_of(ks[i], j));
           }
-          alpha[qt] = weights(qt, key0, edge, sv);
-          // the weights times V's scales in bf16: the operand type of the product with V, a rounding of 2^-9 of each
+          weights(qt, key0, edge, sv);
+          // The weights times V's scales in bf16: the operand type of the product with V, a rounding of 2^-9 of each.  A key
+          // that a query does not see has a weight of 0 there whatever its scale byte is.
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            pw[qt][i >> 2][i & 3] = pack_bf16x2(sv[2 * i] * scale_of(vs[i >> 1], 2 * i & 3),
-                                                sv[2 * i + 1] * scale_of(vs[i >> 1], (2 * i + 1) & 3));
+            pw[qt][i >> 2][i & 3] = pack_bf16x2(__builtin_ldexpf(sv[2 * i], exponent_of(vs[i >> 1], 2 * i & 3)),
+                                                __builtin_ldexpf(sv[2 * i + 1], exponent_of(vs[i >> 1], (2 * i + 1) & 3)));
         }
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) codes_to_bf16(x.vf[mt], vb[mt]);
@@ -356,12 +354,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(k8 && NQT >
         for (int qt = 0; qt < NQT; ++qt) {
           if (qt > 0 && q0 + qt * 16 >= t.qc) break;
 #pragma unroll
-          for (int mt = 0; mt < 4; ++mt) {
-            o[qt][mt] *= alpha[qt];
+          for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
             for (int st = 0; st < 2; ++st)
               o[qt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb[mt][st], as_bf16x8(pw[qt][st]), o[qt][mt], 0, 0, 0);
-          }
         }
       };
       int c = c0;
@@ -370,6 +366,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(k8 && NQT >
     } else {
       C a, b;
       a.load(P, pages, chunk(c0) * C::kSize, h, g, n);
+      take_queries();
+      uint32_t any_lo = 0, any_hi = 0;  // nodes that some node of the wave sees
+#pragma unroll
+      for (int qt = 0; qt < NQT; ++qt) {
+        any_lo |= static_cast<uint32_t>(mask[qt]);
+        any_hi |= static_cast<uint32_t>(mask[qt] >> 32);
+      }
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) {
+        any_lo |= __shfl_xor(any_lo, d);
+        any_hi |= __shfl_xor(any_hi, d);
+      }
+      const uint64_t any = static_cast<uint64_t>(any_hi) << 32 | any_lo;
+      // bit i: some node of the wave sees this lane's key i of the chunk
+      const auto seen_of = [&](int key0) {
+        uint32_t seen = bits_from(any, key0 - t.ctx);
+#pragma unroll
+        for (int i = 0; i < C::kKeys; ++i)
+          if (key0 + i < lo && key0 + i >= P.sinks) seen &= ~(1u << i);
+        return seen;
+      };
       auto step = [&](int c, C& x) {
         const int k0 = chunk(c) * C::kSize, key0 = k0 + C::kKeys * g;
         const bool edge = is_edge(k0);  // uniform
@@ -384,18 +401,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(k8 && NQT >
                                                                 f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
             s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(x.kf[i][1]), qf[qt][1], s, 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sv[4 * i + j] = s[j] * P.scale_log2;
+            for (int j = 0; j < 4; ++j) sv[4 * i + j] = s[j];
           }
-          const float alpha = weights(qt, key0, edge, sv);
+          weights(qt, key0, edge, sv);
           // P in bf16: the operand type of the product with V, a rounding of 2^-9 of each weight
           u32x4_t pw;
 #pragma unroll
           for (int i = 0; i < 4; ++i) pw[i] = pack_bf16x2(sv[2 * i], sv[2 * i + 1]);
 #pragma unroll
-          for (int mt = 0; mt < 4; ++mt) {
-            o[qt][mt] *= alpha;
+          for (int mt = 0; mt < 4; ++mt)
             o[qt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(x.vf[mt]), as_bf16x8(pw), o[qt][mt], 0, 0, 0);
-          }
         }
       };
       // chunk c + 1 is on its way while chunk c is multiplied
@@ -425,7 +440,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(k8 && NQT >
     if (qt > 0 && qt * 16 >= t.qc) break;  // uniform in the workgroup
     const int q = q0 + qt * 16 + n;
     const int64_t token = t.qs + q;
-    float M = m[qt], L = sum_xor16_32(l[qt]);
+    float M = m[qt] == -INFINITY ? m[qt] : mref[qt], L = sum_xor16_32(l[qt]);
     auto finish = [&](int mt, f32x4_t acc) {
       if (q >= t.qc) return;
       const int64_t at = (token * H + h) * kHeadDim + 16 * mt + 4 * g;
@@ -541,22 +556,31 @@ struct Cut {
   int nqt, w, parts;
 };
 
-// Waves to a head's chunks, by how many (row, head) pairs there are; parts as many as bring the workgroups to the
-// number of CUs, of at least kLeast chunks each, where there are at least kCutChunks.
-constexpr int64_t kFour = 512, kTwo = 2560, kCutChunks = 40, kLeast = 8, kWanted = 256;
+// Waves to a head's chunks: four where each has something to do, because four waves on one row's keys end together and
+// leave less of a tail than one wave on each of four rows.  us a call with 1, 2 and 4 waves a head, 16 heads:
+//   one token, 8 bits: one row of 1500 keys 29.0, 17.2, 8.5 (cut into parts); 64 ragged rows of 60 to 2000 keys 51.0,
+//   37.5, 36.7; 256 of them 136, 120, 114; 256 of 60 to 4000 266, 235, 217; but 256 rows of 350 keys 36.3, 38.0, 41.4, of 90
+//   14.2, 16.3, 22.3, of 15 8.2, 12.2, 19.0.  24 nodes: 16 rows of 200 to 1500 44, 26.6, 17.0; 128 of them 70.6, 66.5, 68.3;
+//   128 of 350 26.6, 32.3, 38.0.
+// So six chunks a wave where the pairs fill the chip with one wave each, two where they do not.
+// Parts: as many as bring the workgroups to 512 (to 256 where a wave has two query tiles and so fewer fit a CU), of at least
+// four chunks.  One part and as cut here: one token on 1500 keys 13.4, 8.5; eight rows of 60 to 2000 16.9, 11.9;
+// three rows of 13 nodes on 30000 keys 197, 59; four rows of 24 nodes on 1500 keys 15.3, 13.3.
+constexpr int64_t kFull = 1024;  // (row, head) pairs that fill the chip with a wave each
 
 Cut cut_of(int rows, int max_q, int n_heads, int window, int sinks, int max_kv, int bits) {
   Cut c;
   c.nqt = max_q <= 16 ? 1 : 2;
   const int64_t keys = std::min<int64_t>(max_kv, static_cast<int64_t>(window) + sinks + max_q);
   const int size = bits == 8 ? 64 : 32;
-  const int64_t chunks = (keys + size - 1) / size + 1;
+  const int64_t chunks = (keys + size - 1) / size;
   const int64_t pairs = static_cast<int64_t>(rows) * n_heads;
-  c.w = pairs <= kFour && chunks >= 4 ? 4 : pairs <= kTwo && chunks >= 2 ? 2 : 1;
+  const int64_t few = pairs >= kFull ? 6 : 2;  // chunks a wave
+  c.w = chunks >= 4 * few ? 4 : chunks >= 2 * few ? 2 : 1;
   if (max_q > 32) c.w = std::max(c.w, 2);
   c.parts = 1;
-  if (c.w == 4 && chunks >= kCutChunks)
-    c.parts = static_cast<int>(std::max<int64_t>(1, std::min(kWanted / pairs, chunks / kLeast)));
+  const int64_t wanted = c.nqt == 1 ? 512 : 256;
+  if (c.w == 4) c.parts = static_cast<int>(std::max<int64_t>(1, std::min(wanted / pairs, chunks / 4)));
   return c;
 }
 
