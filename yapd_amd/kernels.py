@@ -304,33 +304,42 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, token: torch.Tens
     """A token drawn from every row of ``logits`` with the random number ``uniform`` (``yapd_sample_tokens``), into
     caller tensors; see :func:`yapd_amd.scoring.sample_tokens`."""
     dev = logits.device
-    if logits.is_cuda and dev.index != torch.cuda.current_device():
+    if elsewhere(logits):
         with torch.cuda.device(dev):  # the launch goes to the current device
             return sample_tokens(logits, uniform, token, logprob, temperature=temperature, top_k=top_k, top_p=top_p,
                                  min_p=min_p)
     f32, shape, stride = torch.float32, logits.shape, logits.stride()
-    require_cuda(logits, "logits", f32 if logits.dtype == f32 else torch.bfloat16, dev, contiguous=False)
+    wide = logits.dtype is f32
+    require_cuda(logits, "logits", f32 if wide else torch.bfloat16, dev, contiguous=False)
     require(len(shape) in (2, 3) and (shape[-1] <= 1 or stride[-1] == 1),
             "logits must be [n, V] or [rows, bl, V] with unit last stride")
     lead = shape[:-1]
-    args = []
-    for name, t, dtype in (("uniform", uniform, f32), ("temperature", temperature, f32), ("top_k", top_k, torch.int32),
-                           ("top_p", top_p, f32), ("min_p", min_p, f32), ("token", token, torch.int64),
-                           ("logprob", logprob, f32)):
-        if isinstance(t, torch.Tensor):
-            require_cuda(t, name, dtype, dev)
-            if t.shape != lead:
-                raise ValueError(f"{name} must have the logits' leading shape")
-            args.append((t.data_ptr(), 0))
-        else:
-            require(name not in ("uniform", "token", "logprob"), f"{name} must be a tensor")
-            args.append((None, t))
-    (u, _), (t, t_all), (k, k_all), (p, p_all), (m, m_all), (tok, _), (lp, _) = args
+
+    def setting(name, t, dtype):
+        """(address or None, number) of a setting."""
+        if not isinstance(t, torch.Tensor):
+            return None, t
+        require_cuda(t, name, dtype, dev)
+        if t.shape != lead:
+            raise ValueError(f"{name} must have the logits' leading shape")
+        return t.data_ptr(), 0
+
+    for name, t, dtype in (("uniform", uniform, f32), ("token", token, torch.int64), ("logprob", logprob, f32)):
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{name} must be a tensor")
+        require_cuda(t, name, dtype, dev)
+        if t.shape != lead:
+            raise ValueError(f"{name} must have the logits' leading shape")
+    t, t_all = setting("temperature", temperature, f32)
+    k, k_all = setting("top_k", top_k, torch.int32)
+    p, p_all = setting("top_p", top_p, f32)
+    m, m_all = setting("min_p", min_p, f32)
     require(k_all == int(k_all), "top_k must be an integer")
     rows, bl = (shape[0], 1) if len(shape) == 2 else lead
     check(load_library().yapd_sample_tokens(
-        logits.data_ptr(), logits.dtype == f32, stride[0], 0 if len(shape) == 2 else stride[1], rows, bl, shape[-1], u, t,
-        t_all, k, max(min(int(k_all), 2**31 - 1), 0), p, p_all, m, m_all, tok, lp, stream_ptr(dev)))
+        logits.data_ptr(), wide, stride[0], 0 if len(shape) == 2 else stride[1], rows, bl, shape[-1], uniform.data_ptr(), t,
+        t_all, k, max(min(int(k_all), 2**31 - 1), 0), p, p_all, m, m_all, token.data_ptr(), logprob.data_ptr(),
+        stream_ptr(dev)))
 
 
 # --------------------------------------------------------------------------- #
@@ -595,6 +604,11 @@ TILE8 = 16 * 64 + 16  # bytes of one head's plane on a page of an 8-bit pool: co
 MAX_NODES = 64        # nodes of a drafted tree: bits of a mask
 
 
+def elsewhere(t: torch.Tensor) -> bool:
+    """Whether ``t`` is on another GPU than the current one, to which launches go."""
+    return t.is_cuda and t.get_device() != torch._C._cuda_getDevice()
+
+
 def kv_bits(pool: torch.Tensor) -> int:
     """8 or 16: the width of a pool's values."""
     return 8 if pool.dtype is torch.uint8 else 16
@@ -611,9 +625,10 @@ def check_table(table: torch.Tensor, name: str, dev: torch.device, rows: int):
     """``(columns, row pitch)`` of an int32 page table of at least ``rows`` rows."""
     require_cuda(table, name, torch.int32, dev, contiguous=False)
     shape, stride = table.shape, table.stride()
-    require(len(shape) == 2 and shape[0] >= rows and shape[1] >= 1 and (shape[1] == 1 or stride[1] == 1),
-            f"{name} must be [>= rows, max_pages] with unit column stride")
-    require(rows <= 1 or stride[0] >= shape[1], f"{name}'s rows must not overlap")
+    if len(shape) != 2 or shape[0] < rows or shape[1] < 1 or (shape[1] != 1 and stride[1] != 1):
+        raise ValueError(f"{name} must be [>= rows, max_pages] with unit column stride")
+    if rows > 1 and stride[0] < shape[1]:
+        raise ValueError(f"{name}'s rows must not overlap")
     return shape[1], max(stride[0], shape[1])
 
 
@@ -627,14 +642,16 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: torch
     map to a page of the pool are left out; every other byte of the pool stays.  NaN is written as 0, infinities as
     the largest finite value."""
     dev = k.device
-    if k.is_cuda and dev.index != torch.cuda.current_device():
+    if elsewhere(k):
         with torch.cuda.device(dev):  # the launch goes to the current device
             return kv8_write(k, v, pool, table, pos0, q_start=q_start)
     for name, t in (("k", k), ("v", v)):
         require_cuda(t, name, torch.bfloat16, dev, contiguous=False)
-        require(t.dim() == 3 and t.shape == k.shape and t.shape[2] == 64, "k and v must be [tokens, H, 64]")
-        require(t.numel() == 0 or (t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == 64)), f"{name}'s heads must be packed")
-    n, H, _ = k.shape
+    shape, k_stride, v_stride = k.shape, k.stride(), v.stride()
+    require(len(shape) == 3 and shape == v.shape and shape[2] == 64, "k and v must be [tokens, H, 64]")
+    n, H, _ = shape
+    require(n * H == 0 or (k_stride[2] == v_stride[2] == 1 and (H == 1 or k_stride[1] == v_stride[1] == 64)),
+            "k's and v's heads must be packed")
     check_pool(pool, "pool", torch.uint8, dev, H)
     require_cuda(pos0, "pos0", torch.int32, dev)
     rows = pos0.numel()
@@ -646,9 +663,9 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: torch
         require(q_start.numel() == rows + 1, "q_start must be [rows + 1]")
     if n == 0 or rows == 0:
         return
-    tok = [t.stride(0) if n > 1 else H * 64 for t in (k, v)]
+    k_tok, v_tok = (k_stride[0], v_stride[0]) if n > 1 else (H * 64, H * 64)
     check(load_library().yapd_kv8_write(
-        k.data_ptr(), v.data_ptr(), tok[0], tok[1], pool.data_ptr(), pool.shape[0], table.data_ptr(), pitch, cols,
+        k.data_ptr(), v.data_ptr(), k_tok, v_tok, pool.data_ptr(), pool.shape[0], table.data_ptr(), pitch, cols,
         pos0.data_ptr(), ptr(q_start), rows, n, H, stream_ptr(dev)))
 
 
@@ -661,7 +678,7 @@ def kv8_unpack(pool8: torch.Tensor, table8: torch.Tensor, kv_len: torch.Tensor, 
     ``kv_len`` is read on the device; ``max_kv`` is the host's upper bound (default: all that both tables map),
     past which nothing is converted.  Columns that either table does not map to a page of its pool are left out."""
     dev = pool8.device
-    if pool8.is_cuda and dev.index != torch.cuda.current_device():
+    if elsewhere(pool8):
         with torch.cuda.device(dev):  # the launch goes to the current device
             return kv8_unpack(pool8, table8, kv_len, pool, table, max_kv=max_kv)
     require(pool8.dim() == 4, "pool8 must be [pages, 2, H, 16*64 + 16]")
@@ -716,17 +733,18 @@ def attn_tree(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len: 
     ``max_q``.  Scores have to stay below 2^30 in magnitude.  Few nodes over many keys need a float32 ``workspace``
     (``yapd_attn_tree_workspace``), allocated here unless given."""
     dev = q.device
-    if q.is_cuda and dev.index != torch.cuda.current_device():
+    if elsewhere(q):
         with torch.cuda.device(dev):  # the launch goes to the current device
             return attn_tree(q, pool, table, kv_len, mask, out, scale, window=window, sinks=sinks, q_start=q_start,
                              max_q=max_q, max_kv=max_kv, workspace=workspace)
-    require_cuda(q, "q", torch.bfloat16, dev, contiguous=False)
+    bf16, i32 = torch.bfloat16, torch.int32
+    require_cuda(q, "q", bf16, dev, contiguous=False)
+    # sizes and strides are asked for once, and messages made only for what fails: a single token's call is host time
     shape, stride = q.shape, q.stride()
-    packed = q_start is not None
-    if packed:
+    if q_start is not None:
         require(len(shape) == 3 and shape[2] == 64, "packed q must be [n_q, H, 64]")
         n_q, H, _ = shape
-        require_cuda(q_start, "q_start", torch.int32, dev)
+        require_cuda(q_start, "q_start", i32, dev)
         rows = q_start.numel() - 1
         require(rows >= 0, "q_start must be [rows + 1]")
         max_q = min(n_q, MAX_NODES) if max_q is None else int(max_q)
@@ -741,14 +759,15 @@ def attn_tree(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len: 
         tok = stride[1] if bl > 1 else stride[0] if rows > 1 else H * 64
         require(rows <= 1 or stride[0] == bl * tok or n_q == 0, "q's rows must follow each other")
     require(n_q * H == 0 or (stride[-1] == 1 and (H == 1 or stride[-2] == 64)), "q's heads must be packed")
-    require_cuda(mask, "mask", torch.int64, dev)
-    require(mask.shape == shape[:-2], "mask must be q's shape without heads")
     bits = kv_bits(pool)
-    check_pool(pool, "pool", torch.uint8 if bits == 8 else torch.bfloat16, dev, H)
-    require_cuda(kv_len, "kv_len", torch.int32, dev)
-    require(kv_len.numel() >= rows, "kv_len must have rows entries")
-    require_cuda(out, "out", torch.bfloat16, dev)
-    require(out.shape == shape, "out must match q")
+    check_pool(pool, "pool", torch.uint8 if bits == 8 else bf16, dev, H)
+    require_cuda(mask, "mask", torch.int64, dev)
+    require_cuda(kv_len, "kv_len", i32, dev)
+    require_cuda(out, "out", bf16, dev)
+    if mask.shape != shape[:-2] or out.shape != shape or kv_len.numel() < rows:
+        require(mask.shape == shape[:-2], "mask must be q's shape without heads")
+        require(out.shape == shape, "out must match q")
+        raise ValueError("kv_len must have rows entries")
     window = WINDOW_CAP if window is None else min(int(window), WINDOW_CAP)
     sinks = min(int(sinks), WINDOW_CAP)
     require(window >= 1 and sinks >= 0, "need window >= 1 and sinks >= 0")
@@ -756,19 +775,20 @@ def attn_tree(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len: 
         return
     cols, pitch = check_table(table, "table", dev, rows)
     kv_max = cols * 16 if max_kv is None else min(int(max_kv), cols * 16)
-    require(kv_max >= 1, "max_kv must be >= 1")
     max_q = min(max_q, n_q)
     lib = load_library()
+    floats = 0
     if workspace is None:
-        need = lib.yapd_attn_tree_workspace(rows, max_q, n_q, H, window, sinks, kv_max, bits)
-        if need > 0:
-            workspace = torch.empty(need, dtype=torch.float32, device=dev)
+        floats = lib.yapd_attn_tree_workspace(rows, max_q, n_q, H, window, sinks, kv_max, bits)
+        if floats > 0:
+            workspace = torch.empty(floats, dtype=torch.float32, device=dev)
     else:
         require_cuda(workspace, "workspace", torch.float32, dev)
+        floats = workspace.numel()
     check(lib.yapd_attn_tree(
         q.data_ptr(), tok, pool.data_ptr(), bits, pool.shape[0], table.data_ptr(), pitch, cols, kv_len.data_ptr(),
-        ptr(q_start), mask.data_ptr(), rows, max_q, n_q, H, window, sinks, kv_max, scale, ptr(workspace),
-        0 if workspace is None else workspace.numel(), out.data_ptr(), stream_ptr(dev)))
+        None if q_start is None else q_start.data_ptr(), mask.data_ptr(), rows, max_q, n_q, H, window, sinks, kv_max, scale,
+        None if workspace is None else workspace.data_ptr(), floats, out.data_ptr(), stream_ptr(dev)))
 
 
 def kv_keep(pools, table: torch.Tensor, base: torch.Tensor, kept: torch.Tensor, n_kept: torch.Tensor) -> None:
@@ -781,7 +801,7 @@ def kv_keep(pools, table: torch.Tensor, base: torch.Tensor, kept: torch.Tensor, 
     order.  Positions that the table does not map to a page of the pool are left out.  The written pages
     must belong to one row alone."""
     ptrs, shape, dev = pool_pointers(pools)
-    if dev.index != torch.cuda.current_device():
+    if elsewhere(pools[0]):
         with torch.cuda.device(dev):  # the launch goes to the current device
             return kv_keep(pools, table, base, kept, n_kept)
     i32 = torch.int32
@@ -789,16 +809,17 @@ def kv_keep(pools, table: torch.Tensor, base: torch.Tensor, kept: torch.Tensor, 
     require_cuda(kept, "kept", i32, dev, contiguous=False)
     require_cuda(n_kept, "n_kept", i32, dev)
     rows = base.numel()
-    require(kept.dim() == 2 and kept.shape[0] == rows and kept.shape[1] <= MAX_NODES
-            and (kept.shape[1] <= 1 or kept.stride(1) == 1) and (rows <= 1 or kept.stride(0) >= kept.shape[1]),
-            f"kept must be [rows, at most {MAX_NODES}] with unit column stride")
+    shape_k, stride_k = kept.shape, kept.stride()
+    if not (len(shape_k) == 2 and shape_k[0] == rows and shape_k[1] <= MAX_NODES and (shape_k[1] <= 1 or stride_k[1] == 1)
+            and (rows <= 1 or stride_k[0] >= shape_k[1])):
+        raise ValueError(f"kept must be [rows, at most {MAX_NODES}] with unit column stride")
     require(n_kept.numel() == rows, "n_kept must have rows entries")
     cols, pitch = check_table(table, "table", dev, rows)
-    if rows == 0 or kept.shape[1] == 0:
+    if rows == 0 or shape_k[1] == 0:
         return
     check(load_library().yapd_kv_keep(
         ptrs.buffer_info()[0], len(ptrs), 16 if shape[3] == 1024 else 8, shape[0], shape[2], table.data_ptr(), pitch, cols,
-        base.data_ptr(), kept.data_ptr(), max(kept.stride(0), kept.shape[1]), kept.shape[1], n_kept.data_ptr(), rows, stream_ptr(dev)))
+        base.data_ptr(), kept.data_ptr(), max(stride_k[0], shape_k[1]), shape_k[1], n_kept.data_ptr(), rows, stream_ptr(dev)))
 
 
 # --------------------------------------------------------------------------- #
