@@ -47,6 +47,17 @@ def test_rows(dev, V, wide, std):
     check(dev, x, settings(n, V + wide))
 
 
+@pytest.mark.parametrize("n,V", [(600, 300), (530, 2057), (1100, 8194), (300, 12000)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_many_rows(dev, n, V, wide):
+    """More rows than CUs, and than twice as many: other workgroups a row."""
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, V, generator=g) * torch.tensor([3.0, 0.05, 8.0]).repeat(n)[:n, None]
+    x[::7, : V // 3] = -math.inf
+    x[3::50] = x[3, 0]
+    check(dev, (x if wide else x.bfloat16()).to(dev), settings(n, V), min_margin=0.0)
+
+
 @pytest.mark.parametrize("V,wide", [(100003, True), (131072, False), (300007, False)])
 def test_large_vocabularies(dev, V, wide):
     g = torch.Generator().manual_seed(V)
@@ -125,6 +136,30 @@ def test_adversarial_ranges(dev):
             s = dict(u=torch.rand(8, generator=g), T=torch.full((8,), T), k=torch.full((8,), k, dtype=torch.int32),
                      p=torch.full((8,), p), m=torch.full((8,), 0.0))
             check(dev, x, s, min_margin=1e-10)
+
+
+@pytest.mark.parametrize("V", [90, 700, 9000])
+def test_bf16_values_of_any_size(dev, V):
+    """Rows far outside the usual size of logits: tiny ones and subnormals, huge ones, all below zero, zeros of either
+    sign among tiny values, masks of the lowest value; temperatures that leave one token, some, and all."""
+    g = torch.Generator().manual_seed(V)
+    base = torch.randn(V, generator=g)
+    some = torch.rand(V, generator=g) < 0.3
+    low = float(torch.finfo(torch.bfloat16).min)
+    rows = [base * 1e-4, base * 3e-3, base * 1e-20, base * 1e-39, base * 40, base * 1e4, base * 1e30, base * 1e37,
+            -base.abs() - 0.01, -base.abs() * 1e-3, -base.abs() * 100 - 70, -base.abs() * 1e36, base - 100, base + 200,
+            torch.where(some, 0.0, base * 1e-4), torch.where(some, -0.0, -base.abs() * 1e-3), torch.where(some, 0.0, -base.abs()),
+            torch.where(some, low, base), torch.where(some, low, base * 1e36), torch.where(some, low, -math.inf),
+            torch.where(some, 2.0 ** -10, 2.0 ** -11), torch.where(some, 64.0, 63.5), torch.where(some, -64.0, -63.5),
+            torch.where(torch.arange(V) == V // 2, 3e38, base), torch.where(some, 1e-4, 20.0)]
+    x = torch.stack(rows).bfloat16().to(dev)
+    n = len(rows)
+    spread = x.cpu().float().where(x.cpu() > -1e30, 0.0).abs().amax(1).clamp_min(1e-38)
+    for i, (factor, k, p, m) in enumerate([(1.0, 0, 1.0, 0.0), (0.05, 0, 0.9, 0.0), (0.3, 40, 0.8, 0.1), (1e-4, 0, 1.0, 0.0),
+                                           (100.0, 0, 0.97, 0.0), (3.0, V // 2, 1.0, 0.3), (0.0, 0, 1.0, 0.0)]):
+        full = lambda v, dt=torch.float32: torch.full((n,), v, dtype=dt)  # noqa: E731
+        check(dev, x, dict(u=torch.rand(n, generator=g), T=(spread * factor).clamp_max(1e38), k=full(k, torch.int32), p=full(p),
+                           m=full(m)), min_margin=0.0)
 
 
 def test_rows_without_a_distribution(dev):

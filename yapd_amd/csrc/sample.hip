@@ -632,7 +632,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   const float min_p = P.min_p ? P.min_p[item] : P.min_p_all;
   const float u = P.u[item];
   if constexpr (!kWide) {
-    if (sample_values<NT, 4>(P, S, granules, off, n_gran, Settings{T, k, top_p, min_p, u}, item)) return;
+    if (sample_values<NT, NT == 512 ? 2 : 4>(P, S, granules, off, n_gran, Settings{T, k, top_p, min_p, u}, item)) return;
     __syncthreads();
   }
   for (int b = tid; b < kBins; b += NT) {
@@ -795,15 +795,15 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   } else if (by_min && !(top_p < 1.f)) {
     cut = static_cast<int>(fmin(t_min / scale * static_cast<double>(per_x) + 1.0, kBins - 1.0));  // one more for rounding
   }
-  const float small = static_cast<float>(scale);  // weights from 2^-64 on are 0
   uint64_t z_min = 0;  // the weight of what min-p keeps
   each([&](const u32x4_t& v, int) {
 #pragma unroll
     for (int e = 0; e < G; ++e) {
       const float x = element(v, e);
       const int b = bin_of(x);
-      if (b > cut || !(x > -INFINITY) || (mx - x) * small >= 64.f) continue;
-      const double t = t_of(x);
+      if (b > cut || !(x > -INFINITY)) continue;
+      const double t = t_of(x);  // mx - x may be past fp32's range
+      if (t >= 64.0) continue;   // a weight of 0
       const uint64_t w = weight_of(t, P.shift);
       atomicAdd(reinterpret_cast<unsigned long long*>(&S.mass[b]), static_cast<unsigned long long>(w));
       if (by_min && t <= t_min) z_min += w;
@@ -945,12 +945,29 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   }
 }
 
-template <bool kWide>
+template <bool kWide, int NT>
 void launch(const SampleParams& P, hipStream_t st) {
-  if (P.vocab <= 10000)
-    hipLaunchKernelGGL((sample_kernel<kWide, 256>), dim3(P.items), dim3(256), 0, st, P);
-  else
-    hipLaunchKernelGGL((sample_kernel<kWide, 1024>), dim3(P.items), dim3(1024), 0, st, P);
+  hipLaunchKernelGGL((sample_kernel<kWide, NT>), dim3(P.items), dim3(NT), 0, st, P);
+}
+
+// Threads a row.  What a row does in turn (bins, sums, searches) is most of a short row's time, and more threads shorten it
+// where a CU has a row or two; where it has more, small workgroups fill it better.  us with 256, 512 and 1024, top-k,
+// top-p and min-p together, bf16 of 8194: one row 14.7, 11.3, 11.6; 256 rows 17.2, 13.5, 13.8; 512 18.4, 15.9, 25.8; 768
+// 20.9, 25.9, 37.3; 4096 77, 103.  Longer rows, with 512 and 1024: 256 rows of 100003 bf16 37.0, 35.7, fp32 134, 92; 300 46.5,
+// 63.6 and 139, 153 (temperature alone 214, 183); 1024 of 32000 bf16 46.8, 69.2, fp32 117, 129.
+template <bool kWide>
+void launch_rows(const SampleParams& P, hipStream_t st) {
+  constexpr uint32_t kCUs = 256;
+  if (P.vocab <= 10000) {
+    if (P.items > 2 * kCUs)
+      launch<kWide, 256>(P, st);
+    else
+      launch<kWide, 512>(P, st);
+  } else if (P.items > kCUs && (!kWide || P.vocab <= 50000)) {
+    launch<kWide, 512>(P, st);
+  } else {
+    launch<kWide, 1024>(P, st);
+  }
 }
 
 }  // namespace
@@ -977,9 +994,9 @@ extern "C" int yapd_sample_tokens(const void* logits, int wide, int64_t seq_stri
                              top_p_all, min_p, min_p_all, token, logprob};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (wide)
-    yapd::launch<true>(P, st);
+    yapd::launch_rows<true>(P, st);
   else
-    yapd::launch<false>(P, st);
+    yapd::launch_rows<false>(P, st);
   YAPD_LAUNCH_CHECK("sample_kernel launch");
   return YAPD_OK;
 }
