@@ -65,6 +65,20 @@ def test_large_vocabularies(dev, V, wide):
     check(dev, (x if wide else x.bfloat16()).to(dev), settings(6, V))
 
 
+def test_rows_inside_one_granule_at_the_end_of_a_buffer(dev):
+    """Rows shorter than 16 bytes at any offset: only granules that hold one of their elements are read."""
+    g = torch.Generator().manual_seed(0)
+    for wide in (False, True):
+        n = 4 if wide else 8
+        buf = torch.empty(2**21 // (4 if wide else 2), dtype=torch.float32 if wide else torch.bfloat16, device=dev)
+        for off in range(n):
+            for V in range(1, n - off + 1):
+                x = torch.randn(V, generator=g).to(buf.dtype)
+                row = buf[buf.numel() - n + off:][:V].view(1, V)
+                row.copy_(x)
+                check(dev, row, settings(1, off + V), min_margin=0.0)
+
+
 def test_strides_and_offsets(dev):
     """Rows that start at any element, a padded pitch, positions of a block."""
     g = torch.Generator().manual_seed(0)

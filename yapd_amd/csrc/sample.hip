@@ -179,7 +179,7 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
   u32x4_t held[RD], edge = {0, 0, 0, 0};
   auto load_tile = [&](int t0) {
 #pragma unroll
-    for (int j = 0; j < RD; ++j) held[j] = granules[f0 + min(t0 + tid + j * NT, max(n_full - 1, 0))];
+    for (int j = 0; j < RD; ++j) held[j] = granules[min(f0 + t0 + tid + j * NT, n_gran - 1)];
   };
   load_tile(0);
   if (has_edge) {
