@@ -7,10 +7,10 @@
 // W_m), and the token is the first whose inclusive sum exceeds u Z.  No token's membership is ever asked: three
 // sums are looked for, in the same order.
 //
-// The row is not sorted.  Its weights are added up in kBins bins of equal width in x (in fp32, which keeps the order),
+// The row is not sorted.  Its weights are added up in four bins a thread, of equal width in x (in fp32, which keeps the order),
 // the bins' prefix sums find the bin where a sum crosses a target, and that bin's elements, usually a few dozen, go to
 // a list where each adds up what precedes it.  A bin of more than kList elements (many equal or nearly equal
-// logits) is divided again, by the bits of (value, index), 10 a time.
+// logits) is divided again, by the bits of (value, index), 10 to 12 a time.
 // Weights are fixed-point numbers of 64 bits, rounded from 64-bit exponentials: their sums are exact, so they do not
 // depend on the order of LDS atomics, and a border is off by V roundings of 2^-52 to 2^-39 at most.
 #include "attn_tile.h"
@@ -19,7 +19,6 @@
 namespace yapd {
 namespace {
 
-constexpr int kBins = 1024;
 constexpr int kList = 256;
 constexpr double kLn2 = 0.69314718055994530942, kLog2e = 1.44269504088896340736;
 
@@ -108,6 +107,7 @@ constexpr int kFloor = (127 - 10) * 128;  // |x| <= 2^-10 is tiny, 64 and above 
 
 template <int NT>
 struct Shared {
+  static constexpr int kBins = 4 * NT;
   union {
     struct {
       uint64_t mass[kBins], mass2[kBins];
@@ -574,7 +574,7 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
 // One workgroup a row, which every pass reads again (from the caches: a speech vocabulary's row is 16 KB).
 template <bool kWide, int NT>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sample_kernel(const SampleParams P) {
-  constexpr int G = kWide ? 4 : 8, kBytes = kWide ? 4 : 2;
+  constexpr int G = kWide ? 4 : 8, kBytes = kWide ? 4 : 2, kBins = Shared<NT>::kBins;
   __shared__ Shared<NT> S;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t item = blockIdx.x;
@@ -795,6 +795,83 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   } else if (by_min && !(top_p < 1.f)) {
     cut = static_cast<int>(fmin(t_min / scale * static_cast<double>(per_x) + 1.0, kBins - 1.0));  // one more for rounding
   }
+  // Where the bins up to `cut` hold few elements (a small top-k, or min-p alone), all of them go to the list, and the three
+  // sums are found there: no weights in bins, no further pass.
+  if (by_count ? S.count[cut] <= kList : cut < kBins - 1) {
+    if (tid == 0) S.n = 0;
+    __syncthreads();
+    each([&](const u32x4_t& v, int i0) {
+#pragma unroll
+      for (int e = 0; e < G; ++e) {
+        const float x = element(v, e);
+        if (!(x > -INFINITY) || bin_of(x) > cut) continue;
+        const uint32_t to = atomicAdd(&S.n, 1u);
+        if (to < kList) S.key[to] = key_of(x, i0 + e);
+      }
+    });
+    __syncthreads();
+    const int n = static_cast<int>(S.n);
+    if (n <= kList) {
+      for (int i = tid; i < n; i += NT) {  // in order
+        const uint64_t key = S.key[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += S.key[j] > key;
+        S.w[rank] = key;
+      }
+      __syncthreads();
+      if (wave == 0) {  // inclusive sums of the weights, four a lane, into S.key
+        uint64_t sum[kList / 64], all = 0;
+#pragma unroll
+        for (int j = 0; j < kList / 64; ++j) {
+          const int i = lane * (kList / 64) + j;
+          sum[j] = all += i < n ? weight_of(t_of(value_of(S.w[i])), P.shift) : 0;
+        }
+        uint64_t to = all;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+          const uint64_t left = shfl_up64(to, d);
+          if (lane >= d) to += left;
+        }
+#pragma unroll
+        for (int j = 0; j < kList / 64; ++j) S.key[lane * (kList / 64) + j] = to - all + sum[j];
+      }
+      __syncthreads();
+      if (tid == 0) {
+        // the first of [0, end) at which f holds; it holds from there on, and at end - 1
+        auto first = [&](int end, auto f) {
+          int lo = 0, hi = end - 1;
+          while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (f(mid))
+              hi = mid;
+            else
+              lo = mid + 1;
+          }
+          return lo;
+        };
+        int kept = by_count ? min(n, k) : n;
+        uint64_t z = S.key[kept - 1];
+        if (top_p < 1.f) {
+          const double target = fmax(static_cast<double>(top_p) * static_cast<double>(z), 0.5);
+          kept = first(kept, [&](int i) { return static_cast<double>(S.key[i]) >= target; }) + 1;
+        }
+        if (by_min) {
+          const int out = first(n + 1, [&](int i) { return i >= n || t_of(value_of(S.w[i])) > t_min; });
+          kept = min(kept, max(out, 1));
+        }
+        z = S.key[kept - 1];
+        const double target = static_cast<double>(fminf(fmaxf(u, 0.f), 0x1.fffffep-1f)) * static_cast<double>(z);
+        const uint64_t key = S.w[first(kept, [&](int i) { return static_cast<double>(S.key[i]) > target; })];
+        P.token[item] = 0xffffffffu - static_cast<uint32_t>(key);
+        P.logprob[item] = static_cast<float>(-t_of(value_of(key)) * kLn2 - log(__builtin_ldexp(static_cast<double>(z), -P.shift)));
+      }
+      return;
+    }
+  }
+  if (by_count) {  // the search for cut is over: S.bin may be used again
+    __syncthreads();
+  }
+
   uint64_t z_min = 0;  // the weight of what min-p keeps
   each([&](const u32x4_t& v, int) {
 #pragma unroll
@@ -828,7 +905,9 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
     const int bin = S.bin;
     uint64_t base = S.base, klo = 0, khi = ~uint64_t{0};
     uint32_t base_count = S.base_count;
-    for (;;) {  // at most 7 times: each further one leaves an interval of keys a thousandth as long
+    constexpr int kLog = NT == 1024 ? 12 : NT == 512 ? 11 : 10;  // of kBins
+    static_assert(1 << kLog == kBins, "an interval of keys fills the bins");
+    for (;;) {  // at most 7 times: each further one leaves an interval of keys a thousandth as long, or less
       if (tid == 0) S.n = 0;
       __syncthreads();
       each([&](const u32x4_t& v, int i0) {
@@ -894,7 +973,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
       }
       klo = lo;
       khi = hi;
-      const int bits = max(64 - __clzll(static_cast<long long>(khi - klo)) - 10, 0);  // khi > klo: keys differ
+      const int bits = max(64 - __clzll(static_cast<long long>(khi - klo)) - kLog, 0);  // khi > klo: keys differ
       each_key([&](float x, uint64_t key) {
         if (bin_of(x) != bin || key < klo || key > khi) return;
         const int b = static_cast<int>((khi - key) >> bits);
