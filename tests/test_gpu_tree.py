@@ -78,6 +78,15 @@ def test_rows_longer_than_max_q(dev, max_q, bits):
 
 
 @pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("max_q,window", [(4, 4), (20, 20), (20, 45), (40, 41)])
+def test_masks_deeper_than_the_window(dev, max_q, window, bits):
+    """A row of more than max_q nodes may have masks of more nodes than the window is long: it bounds the context alone."""
+    c = Case(n_nodes=[50, 3, 64], kv_lens=[120, 80, 300], H=4, bits=bits, packed=True, max_q=max_q, window=window, sinks=3,
+             kind="full")
+    c.check(c.run(dev, kernels))
+
+
+@pytest.mark.parametrize("bits", [16, 8])
 def test_lengths_past_the_table(dev, bits):
     """kv_len is held to what the table maps: nodes keep their distance from the end."""
     c = Case(n_nodes=[5], kv_lens=[48], H=4, bits=bits, extra_cols=0)

@@ -8,13 +8,21 @@
 //
 // A wave takes up to 16 NQT nodes of a row, so a key is read once for most trees.  The keys seen
 // are a list of chunks (the sinks', then those from the window's begin on), cut into `parts` (workgroups) and each
-// part into KS runs (waves); runs join in LDS, parts through a workspace and a second launch.  S^T = K Q^T and
+// part into W runs (waves); runs join in LDS, parts through a workspace and a second launch.  S^T = K Q^T and
 // O^T += V^T P^T on v_mfma_f32_16x16x32_bf16, every lane owning one query and kKeys consecutive keys of a chunk:
 //   bf16: chunks of 32 keys (two pages), 8 keys a lane;
 //   8 bits: chunks of 64 keys (four pages), lane group g owning page g: 16 bytes are 16 head dims of a key, 16
 //     tokens of a head dim or 16 tokens' scales, so every load is 16 bytes.  Which head dims a step of the product
 //     with K takes is free as long as Q's fragments take the same.  Codes become bf16 (exact); K's scales
 //     multiply the scores, V's the weights before they are rounded to bf16.
+//
+// Single tokens and long rows are bound by memory: 256 ragged rows of 60 to 4000 keys x 16 heads at 8 bits 202 us, 5.4
+// TB/s (half of the vector unit's cycles are free; in bf16 the same takes 350); three rows of 13 nodes on 20000 to 30000 keys
+// in bf16 57 us, 5.4 TB/s, 5 of it the join.  Trees at 8 bits are not: 130 rows of 1 to 64 nodes on up to 2033 keys
+// 136 us, 3.0 TB/s.  A chunk costs a wave 230 vector instructions and a tile of 16 queries 110 more with 16 exponentials, at
+// two waves a SIMD (223 registers) their chains are not hidden behind each other.  Measured and left out there: K's
+// product on v_mfma_i32_16x16x64_i8 with Q in two bytes (no conversion of K; 184 registers) 145 us with one set of
+// loads and 133 with two, but Q would be rounded; three waves a SIMD 208 (spills); 512 threads a head 179.
 #include <algorithm>
 #include <type_traits>
 
@@ -231,7 +239,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NQT > 1 ? 2
 #pragma unroll
     for (int qt = 0; qt < NQT; ++qt) {
       const int q = min(q0 + qt * 16 + n, t.qc - 1);  // lanes without a node repeat the last
-      q_lo[qt] = t.ctx + __popcll(mask[qt] & nodes & ~(uint64_t{1} << q)) - P.window + 1;
+      // at most ctx: the window bounds the context, and a row's first nodes may be deeper than it
+      const int depth = static_cast<int>(__popcll(mask[qt] & nodes & ~(uint64_t{1} << q)));
+      q_lo[qt] = t.ctx + min(depth - P.window + 1, 0);
       lo = min(lo, q_lo[qt]);
       all_lo = max(all_lo, q_lo[qt]);
     }
