@@ -113,9 +113,10 @@ int yapd_token_logprobs(const void* logits, int wide, int64_t seq_stride, int64_
  * A row that holds a NaN or +inf, or -inf alone: token -1, logprob NaN.
  * uniform [rows * bl] fp32; temperature, top_p, min_p (fp32) and top_k (int32) are
  * [rows * bl], or NULL: the number beside it holds for every row.  token int64, logprob fp32.
- * Weights are rounded to 64-bit fixed point (2^-51, with more than 2^11 tokens
- * 2^-62 times the next power of two), their sums are exact: the same call gives the same
- * token.  vocab <= 2^24.  One launch, no workspace. */
+ * Weights are right to 4e-12 of themselves; those of fp32 logits are rounded to 64-bit
+ * fixed point besides (2^-51, with more than 2^11 tokens 2^-62 times the next power of
+ * two).  They are summed in an order that depends on nothing else: the same call gives
+ * the same token.  vocab <= 2^24.  One launch, no workspace. */
 int yapd_sample_tokens(const void* logits, int wide, int64_t seq_stride, int64_t pos_stride, int rows, int bl,
                        int vocab, const float* uniform, const float* temperature, float temperature_all,
                        const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all, const float* min_p,

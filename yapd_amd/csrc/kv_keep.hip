@@ -4,8 +4,10 @@
 // (row, head, layer)'s values, at most 64 tokens, before it writes the first, so any indices may be given: a
 // position may be read after the call has given it another token.
 //
-// Bound by the lines that V's columns touch: a token is 128 consecutive bytes of K and two bytes in
-// each of 64 pieces of V.
+// Bound by the lines that V's columns touch: a token is 128 consecutive bytes of K and two bytes in each of 64
+// pieces of V, every line of a page's head.  130 rows that keep 5 of 64 nodes on average, 30 layers of 16 heads, 147 us: 360 MB
+// read and 183 written for 85 each of tokens, 3.7 TB/s.  Destination pages of V read, merged and written whole, 16
+// values in registers instead of 64, 151 us; 16 values with plain stores 156.
 #include "attn_tile.h"
 #include "common.h"
 #include "kv_layout.h"
