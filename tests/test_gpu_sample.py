@@ -274,3 +274,17 @@ def test_captured_call(dev):
         torch.cuda.synchronize()
         want = check(dev, x, n)
         assert torch.equal(token.cpu(), want)
+
+
+@pytest.mark.parametrize("value", [-math.inf, float(torch.finfo(torch.bfloat16).min), -1e4, -100.0])
+@pytest.mark.parametrize("n", [300, 700])
+def test_rows_masked_for_the_most_part(dev, n, value):
+    """Most tokens masked, as -inf, by the lowest value, or by one that a high temperature lets in; rows at any offset."""
+    V = 1000
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, V + 9, generator=g) * 2
+    x = x.masked_fill(torch.rand(n, V + 9, generator=g) < 0.9, value).bfloat16().to(dev)
+    s = settings(n, 3)
+    s["T"] = torch.tensor([0.8, 2.0, 30.0, 1e3]).repeat(n)[:n]
+    for off in (0, 1, 4, 9):
+        check(dev, x[:, off:off + V], s, min_margin=0.0)

@@ -113,7 +113,7 @@ __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d) {
 enum Cross { kCount, kReach, kExceed };  // the first element whose inclusive count, or sum, is at least, or exceeds, a target
 
 constexpr int kValues = 4096;             // bins of the bf16 form: one a value, 2047 on either side of the tiny ones
-constexpr int kTiny = kValues / 2, kLow = kValues - 1;
+constexpr int kTiny = kValues / 2, kLow = kValues - 1;  // low ones are counted in kLow + lane: a mask's in one word would queue there
 constexpr int kFloor = (127 - 10) * 128;  // |x| <= 2^-10 is tiny, 64 and above high: bits of the usual window's floor
 
 template <int NT>
@@ -124,7 +124,7 @@ struct Shared {
       uint64_t mass[kBins], mass2[kBins];
       uint32_t count[kBins], count2[kBins];
     };
-    uint32_t values[kValues];
+    uint32_t values[kValues + 63];
   };
   uint64_t key[kList], w[kList];
   uint64_t part[NT / 64], part2[NT / 64], z_min[NT / 64];
@@ -173,7 +173,7 @@ struct Settings {
 // moves the window there and counts again).  Elements are only counted; a bin's weight is its count times its
 // value's, the values of 16 consecutive bins being an arithmetic progression (so their weights are a geometric one),
 // and of equal logits the n-th is found by division.  Tiny values other than 0 go to a list as they are counted and are
-// weighed one by one; low ones are -inf or weigh less than 2^-60 together.  false, for the general form: low values that
+// weighed one by one; low ones weigh less than 2^-60 together.  false, for the general form: low values that
 // weigh more, more tiny ones than the list holds, or a token among several values of the tiny bin.
 template <int NT, int RD>
 __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>& S, const u32x4_t* granules, int off,
@@ -187,7 +187,6 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
   const bool tail = (off + V) % 8 != 0 && (n_gran > 1 || off == 0);
   const bool has_edge = (tid == 0 && off > 0) || (tid == 1 && tail);
   const int edge_gi = tid == 0 ? 0 : n_gran - 1;
-  const uint32_t pads = static_cast<uint32_t>((f0 + (tail ? 1 : 0)) * 8 - (V - n_full * 8));
   u32x4_t held[RD], edge = {0, 0, 0, 0};
   auto load_tile = [&](int t0) {
 #pragma unroll
@@ -222,7 +221,8 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
   auto bins_of = [&](uint32_t word, uint32_t above) {
     const s16x2 sign = __builtin_bit_cast(s16x2, word) >> 15;
     const s16x2 y = (__builtin_bit_cast(s16x2, above) ^ sign) - sign;
-    const s16x2 mid = {kTiny, kTiny}, top = {kLow, kLow}, zero = {0, 0};
+    const short end = static_cast<short>(kLow + lane);
+    const s16x2 mid = {kTiny, kTiny}, top = {end, end}, zero = {0, 0};
     return __builtin_elementwise_max(__builtin_elementwise_min(__builtin_elementwise_sub_sat(mid, y), top), zero);
   };
   auto value_of_bin = [&](int b) {
@@ -232,10 +232,11 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
 
   uint32_t c[kPer];  // elements of this thread's bins, tid * kPer and on
   float mx = 0.f;
-  uint32_t tiny, low;
+  uint32_t tiny;
   for (int round = 0;; ++round) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) S.values[tid + j * NT] = 0;
+    if (tid < 63) S.values[kValues + tid] = 0;
     if (tid == 0) {
       S.first = kValues;
       S.bad = S.n = 0;
@@ -280,18 +281,17 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[j + i] = four[i];
     }
-    if (tid == NT - 1) c[kPer - 1] -= pads;  // pads count as low
+    if (tid == NT - 1) c[kPer - 1] = 0;
 #pragma unroll
     for (int j = kPer - 1; j >= 0; --j)
       if (c[j]) first = tid * kPer + j;
     for (int d = 1; d < 64; d <<= 1) first = min(first, __shfl_xor(first, d));
     if (lane == 0) atomicMin(&S.first, first);
     tiny = S.values[kTiny];
-    low = S.values[kLow] - pads;
     const uint32_t high = S.values[0];
     __syncthreads();
     first = S.first;
-    if (high == 0 && first != kTiny && first != kLow) {
+    if (high == 0 && first < kLow && first != kTiny) {
       mx = value_of_bin(first);
       break;
     }
@@ -329,8 +329,7 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
   const bool by_min = s.min_p > 0.f;
   const double min_p = fminf(s.min_p, 1.f);
 
-  // Tiny values other than 0 were listed; low ones are -inf, or weigh nothing next to the largest, or else are counted
-  // one by one below (by returning false).
+  // Tiny values other than 0 were listed; low ones weigh nothing next to the largest, or the row goes to the general form.
   double tiny_mass = 0.0, tiny_min = 0.0;
   const uint32_t listed = S.n;
   if (tiny && !greedy) {
@@ -343,29 +342,36 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
         const uint64_t mine = S.key[i];
         uint32_t rank = 0;
         for (uint32_t j = 0; j < listed; ++j) rank += S.key[j] < mine || (S.key[j] == mine && j < i);
-        S.w[rank] = mine;
+        S.w[rank] = __builtin_bit_cast(uint64_t, exp2_neg(t_of(__uint_as_float(static_cast<uint32_t>(mine) << 16))));
       }
       __syncthreads();
       for (uint32_t i = 0; i < listed; ++i) {
-        const double w = exp2_neg(t_of(__uint_as_float(static_cast<uint32_t>(S.w[i]) << 16)));
+        const double w = __builtin_bit_cast(double, S.w[i]);
         tiny_mass += w;
         tiny_min += w >= min_p ? w : 0.0;
       }
     }
   }
-  if (low && !greedy) {
-    // the weight of all low elements is below 2^-60 of the largest's: what top-k and top-p keep of them counts for nothing
-    const double t = t_of(-__uint_as_float(static_cast<uint32_t>(fl + 2047) << 16));
-    if (t < 60.0 + 24.0) {
-      bool finite = false;
+  // From 84 octaves below the largest on, 2^24 of them weigh less than 2^-60: what top-k and top-p keep of those counts
+  // for nothing.  Masked tokens are there, as -inf or as the type's lowest value.
+  constexpr double kFar = 60.0 + 24.0;
+  if (!greedy && t_of(-__uint_as_float(static_cast<uint32_t>(fl + 2047) << 16)) < kFar) {
+    // what is beside the row was counted by the first two threads
+    const uint32_t pads = static_cast<uint32_t>((f0 + (tail ? 1 : 0)) * 8 - (V - n_full * 8));
+    const uint32_t pads_head = off > 0 ? (tail ? off : pads) : 0;
+    if (__any(S.values[kLow + lane] > (lane == 0 ? pads_head : lane == 1 ? pads - pads_head : 0))) {
+      // magnitudes up to here, rounded up, are nearer than that
+      const float far = static_cast<float>(kFar / scale - static_cast<double>(mx));
+      const uint32_t near = min((__float_as_uint(far) >> 16) + 1, 0x7f7fu);
+      bool counts = false;
       each([&](const u32x4_t& v, int) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const s16x2 b = bins_of(v[w], above_floor(__builtin_bit_cast(u16x2, v[w] & 0x7fff7fffu)));
-          finite |= (b[0] == kLow && (v[w] & 0xffffu) != 0xff80u) || (b[1] == kLow && v[w] >> 16 != 0xff80u);
+          counts |= (b[0] >= kLow && (v[w] & 0x7fffu) <= near) || (b[1] >= kLow && (v[w] >> 16 & 0x7fffu) <= near);
         }
       });
-      if (__any(finite) && lane == 0) atomicOr(&S.bad, 1u);
+      if (__any(counts) && lane == 0) atomicOr(&S.bad, 1u);
       __syncthreads();
       if (S.bad) return false;
     }
@@ -389,7 +395,7 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
     int j_first = kPer;
 #pragma unroll
     for (int j = kPer - 1; j >= 0; --j)
-      if (c[j] && b0 + j != kTiny && b0 + j != kLow) j_first = j;  // what is low counts for nothing
+      if (c[j] && b0 + j != kTiny) j_first = j;
     if (j_first < kPer) {
       w_first = exp2_neg(t_of(value_of_bin(b0 + j_first)));
       r = exp2_neg((static_cast<double>(value_of_bin(b0 + 1)) - static_cast<double>(value_of_bin(b0 + 2))) * scale);
@@ -399,7 +405,7 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const int b = b0 + j;
-        const uint32_t n = b == kLow ? 0 : c[j];
+        const uint32_t n = c[j];
         if (j == 0 && b == kTiny) {
           f(b, n, tiny_each, tiny_mass);
         } else if (j >= j_first) {
