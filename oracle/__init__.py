@@ -24,6 +24,10 @@ Modules (each function cites the reference file:line it restates):
   calls ``mlx.nn.quantize``; the documented MLX formula is restated).
 * :mod:`oracle.serve` -- the continuous-batching tick bookkeeping of
   server/engine.py:522-620 (commit / denoise transitions, clamps, flags).
+* :mod:`oracle.kv8`, :mod:`oracle.tree` -- the 8-bit cache's codes and
+  scales, and attention for trees of drafted tokens, by their definitions.
+* :mod:`oracle.sample` -- tokens drawn with given random numbers (temperature,
+  top-k, top-p, min-p), with the margin to the next outcome.
 * :mod:`oracle.vocoder` -- the HiFT vocoder's Snake / bias / residual /
   mean3 elementwise family of server/kernels.py:35-67.
 """
