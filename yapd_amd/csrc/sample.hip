@@ -121,7 +121,7 @@ struct Shared {
   static constexpr int kBins = 4 * NT;
   union {
     struct {
-      uint64_t mass[kBins], mass2[kBins];
+      uint64_t mass[kBins], mass2[kBins];  // mass2 also holds keys, see `held`
       uint32_t count[kBins], count2[kBins];
     };
     uint32_t values[kValues + 63];
@@ -130,7 +130,7 @@ struct Shared {
   uint64_t part[NT / 64], part2[NT / 64], z_min[NT / 64];
   double sum_a[NT / 64], sum_b[NT / 64];
   float fmx[NT / 64], fmn[NT / 64];
-  uint32_t n, bad;
+  uint32_t n, bad, n_held;
   // what a search found
   int bin;
   uint64_t base, sum;
@@ -886,17 +886,26 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
       return;
     }
   }
-  if (by_count) {  // the search for cut is over: S.bin may be used again
-    __syncthreads();
-  }
+  // Searches read the row's elements of a bin again, from memory, unless mass2 holds them (until a bin is divided): all of
+  // the bins up to `cut` where they fit, put there as they are weighed, else those of top-p's bin and of the ones
+  // that the last search can end in, fetched in one pass for both.  (fp32 rows only: bf16 ones seldom come here.)
+  bool held = kWide && by_count && S.count[cut] <= kBins;
+  int held_to = held ? cut : -1, held_p = -1, held_lo = 0, held_hi = -1;  // bins up to held_to, held_p, held_lo to held_hi
+  auto hold = [&](float x, int index) {
+    const uint32_t to = atomicAdd(&S.n_held, 1u);
+    if (to < kBins) S.mass2[to] = key_of(x, index);
+  };
+  if (tid == 0) S.n_held = 0;
+  if (by_count || held) __syncthreads();  // the search for cut is over: S.bin may be used again
 
   uint64_t z_min = 0;  // the weight of what min-p keeps
-  each([&](const u32x4_t& v, int) {
+  each([&](const u32x4_t& v, int i0) {
 #pragma unroll
     for (int e = 0; e < G; ++e) {
       const float x = element(v, e);
       const int b = bin_of(x);
       if (b > cut || !(x > -INFINITY)) continue;
+      if (kWide && held) hold(x, i0 + e);
       const double t = t_of(x);  // mx - x may be past fp32's range
       if (t >= 64.0) continue;   // a weight of 0
       const uint64_t w = weight_of(t, P.shift);
@@ -928,17 +937,26 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
     for (;;) {  // at most 7 times: each further one leaves an interval of keys a thousandth as long, or less
       if (tid == 0) S.n = 0;
       __syncthreads();
-      each([&](const u32x4_t& v, int i0) {
-#pragma unroll
-        for (int e = 0; e < G; ++e) {
-          const float x = element(v, e);
-          if (!(x > -INFINITY) || bin_of(x) != bin) continue;
-          const uint64_t key = key_of(x, i0 + e);
-          if (key < klo || key > khi) continue;
-          const uint32_t to = atomicAdd(&S.n, 1u);
-          if (to < kList) S.key[to] = key;
+      auto list = [&](uint64_t key) {
+        const uint32_t to = atomicAdd(&S.n, 1u);
+        if (to < kList) S.key[to] = key;
+      };
+      if (kWide && held && (bin <= held_to || bin == held_p || (bin >= held_lo && bin <= held_hi))) {
+        for (int i = tid; i < static_cast<int>(S.n_held); i += NT) {
+          const uint64_t key = S.mass2[i];
+          if (bin_of(value_of(key)) == bin) list(key);
         }
-      });
+      } else {
+        each([&](const u32x4_t& v, int i0) {
+#pragma unroll
+          for (int e = 0; e < G; ++e) {
+            const float x = element(v, e);
+            if (!(x > -INFINITY) || bin_of(x) != bin) continue;
+            const uint64_t key = key_of(x, i0 + e);
+            if (key >= klo && key <= khi) list(key);
+          }
+        });
+      }
       __syncthreads();
       const int n = static_cast<int>(S.n);
       if (n <= kList) {
@@ -965,6 +983,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
         __syncthreads();
         return;
       }
+      held = false;  // mass2 has another use now
       // the interval of the keys, then bins of it
       uint64_t lo = ~uint64_t{0}, hi = 0;
       each_key([&](float x, uint64_t key) {
@@ -1013,6 +1032,31 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   };
 
   uint64_t z = S.mass[kBins - 1];
+  // u is held to [0, 1 - 2^-24] (a NaN to 0)
+  const double share = static_cast<double>(fminf(fmaxf(u, 0.f), 0x1.fffffep-1f));
+  if (kWide && !by_count && top_p < 1.f) {
+    find_bin(S.mass, S.count, false, kReach, 0, 0, fmax(static_cast<double>(top_p) * static_cast<double>(z), 0.5));
+    held_p = S.bin;
+    // what top-p keeps weighs at least S.base and at most S.mass[held_p]: the last search's target is between these shares
+    const uint64_t least = by_min ? min(S.base, z_min) : S.base, most = by_min ? min(S.mass[held_p], z_min) : S.mass[held_p];
+    __syncthreads();
+    find_bin(S.mass, S.count, false, kExceed, 0, 0, share * static_cast<double>(least));
+    held_lo = S.bin;
+    __syncthreads();
+    find_bin(S.mass, S.count, false, kExceed, 0, 0, share * static_cast<double>(most));
+    held_hi = S.bin;
+    each([&](const u32x4_t& v, int i0) {
+#pragma unroll
+      for (int e = 0; e < G; ++e) {
+        const float x = element(v, e);
+        const int b = bin_of(x);
+        if (x > -INFINITY && (b == held_p || (b >= held_lo && b <= held_hi))) hold(x, i0 + e);
+      }
+    });
+    held = true;
+    __syncthreads();
+  }
+  if (S.n_held > kBins) held = false;
   for (int step = 0; step < 3; ++step) {
     Cross mode = kExceed;
     double target;
@@ -1026,8 +1070,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
       target = fmax(static_cast<double>(top_p) * static_cast<double>(z), 0.5);
     } else {
       if (by_min) z = min(z, z_min);
-      // u is held to [0, 1 - 2^-24] (a NaN to 0)
-      target = static_cast<double>(fminf(fmaxf(u, 0.f), 0x1.fffffep-1f)) * static_cast<double>(z);
+      target = share * static_cast<double>(z);
     }
     cross(mode, target);
     if (step < 2) {
