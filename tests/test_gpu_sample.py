@@ -288,3 +288,22 @@ def test_rows_masked_for_the_most_part(dev, n, value):
     s["T"] = torch.tensor([0.8, 2.0, 30.0, 1e3]).repeat(n)[:n]
     for off in (0, 1, 4, 9):
         check(dev, x[:, off:off + V], s, min_margin=0.0)
+
+
+@pytest.mark.parametrize("V", [1003, 9001, 20011])
+def test_fp32_rows_of_any_range(dev, V):
+    """The least logits at the row's ends, which fill no 16 bytes; ranges past fp32's; temperatures whose bins are wide."""
+    g = torch.Generator().manual_seed(V)
+    base = torch.randn(V, generator=g)
+    ends = base * 0.1
+    ends[0], ends[-1] = -15.0, -20.0
+    rows = [ends, ends - 1e5, (base * 1.5e38).clamp(-3.3e38, 3.3e38), base * 1e37, base * 1e-37, base * 3e-38,
+            torch.where(base > 0, 3e38, -3e38)]
+    temps = [5.0, 7.0, 1e38, 1e36, 1e-37, 1e-37, 2e38]
+    buf = torch.zeros(len(rows), V + 3, device=dev)
+    for off in (0, 1, 3):
+        buf[:, off:off + V] = torch.stack(rows).to(dev)
+        for k, p, m in ((0, 1.0, 0.0), (0, 0.9, 0.0), (V // 3, 0.8, 0.0), (0, 0.95, 0.01), (0, 1.0, 0.2), (900, 1.0, 0.001)):
+            full = lambda v, dt=torch.float32: torch.full((len(rows),), v, dtype=dt)  # noqa: E731
+            check(dev, buf[:, off:off + V], dict(u=torch.rand(len(rows), generator=g), T=torch.tensor(temps),
+                                                 k=full(k, torch.int32), p=full(p), m=full(m)), min_margin=0.0)

@@ -21,9 +21,10 @@
 // Measured, on the GPU alone.  One bf16 row of 8194: 10 us, a chain of some 15 steps between barriers, as long for
 // any number of rows up to the CUs'.  4096 of them with all three filters, each row its own: 69 us, where the
 // bytes take 13: four workgroups a CU, of whose time the vector unit's instructions are half and counting in LDS (two
-// atomics a word) nearly as much, and each row's chain is hidden by three others only.  fp32, 300 rows of 100003, 120 MB, 23 us
-// as bytes: temperature alone 135 us (a 64-bit LDS atomic an element), all filters with a small top-k 89 (counts of 32
-// bits, and the rest on one list), a row with its own settings each 124; 300 rows on 256 CUs are two turns.
+// atomics a word) nearly as much, and each row's chain is hidden by three others only.  fp32, a row of 100003: 15 us for the
+// largest, 50 with a temperature, 57 with top-p (three passes; instructions bound it: 67 an element before its weight was a
+// polynomial within its bin, then 62 us).  300 such rows, 120 MB, 23 us as bytes: 110 us with a temperature, all filters with a
+// small top-k 88, settings of their own 103 to 107; 300 rows on 256 CUs are two turns, and every pass fetches the rows again.
 #include "attn_tile.h"
 #include "common.h"
 
@@ -116,7 +117,7 @@ constexpr int kValues = 4096;             // bins of the bf16 form: one a value,
 constexpr int kTiny = kValues / 2, kLow = kValues - 1;  // low ones are counted in kLow + lane: a mask's in one word would queue there
 constexpr int kFloor = (127 - 10) * 128;  // |x| <= 2^-10 is tiny, 64 and above high: bits of the usual window's floor
 
-template <int NT>
+template <int NT, bool kWide>
 struct Shared {
   static constexpr int kBins = 4 * NT;
   union {
@@ -126,6 +127,7 @@ struct Shared {
     };
     uint32_t values[kValues + 63];
   };
+  double power[kWide ? kBins : 1];  // the weight at a bin's begin, times 2^shift
   uint64_t key[kList], w[kList];
   uint64_t part[NT / 64], part2[NT / 64], z_min[NT / 64];
   double sum_a[NT / 64], sum_b[NT / 64];
@@ -176,7 +178,7 @@ struct Settings {
 // weighed one by one; low ones weigh less than 2^-60 together.  false, for the general form: low values that
 // weigh more, more tiny ones than the list holds, or a token among several values of the tiny bin.
 template <int NT, int RD>
-__device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>& S, const u32x4_t* granules, int off,
+__device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT, false>& S, const u32x4_t* granules, int off,
                                               int n_gran, const Settings& s, uint32_t item) {
   constexpr int kPer = kValues / NT;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -592,8 +594,8 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT>&
 // One workgroup a row, which every pass reads again (from the caches: a speech vocabulary's row is 16 KB).
 template <bool kWide, int NT>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sample_kernel(const SampleParams P) {
-  constexpr int G = kWide ? 4 : 8, kBytes = kWide ? 4 : 2, kBins = Shared<NT>::kBins;
-  __shared__ Shared<NT> S;
+  constexpr int G = kWide ? 4 : 8, kBytes = kWide ? 4 : 2, kBins = Shared<NT, kWide>::kBins;
+  __shared__ Shared<NT, kWide> S;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t item = blockIdx.x;
   const uint32_t r = item / P.bl;
@@ -659,9 +661,18 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   }
   if (tid == 0) S.bad = 0;
 
-  // the largest logit, the least of whole granules (it only decides the bins' width), and whether there is a NaN
+  // the largest and the least logit, and whether there is a NaN
   float mx = -INFINITY, mn = INFINITY;
   bool bad = false;
+  if (tid < 2) {  // the ends' least
+    const int gi = tid ? n_gran - 1 : 0;
+    const u32x4_t v = granules[gi];
+#pragma unroll
+    for (int e = 0; e < G; ++e) {
+      const int i = gi * G + e - off;
+      if (i >= 0 && i < V) mn = fminf(mn, element(v, e));
+    }
+  }
   each([&](const u32x4_t& v, int i0) {
     float lo = INFINITY;
 #pragma unroll
@@ -717,13 +728,35 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   }
 
   const double scale = kLog2e / static_cast<double>(T);
-  // bins: the row's range, or 64 octaves of weight where that is less (smaller weights than the last bin's are 0)
-  const float per_x = fminf(fmaxf((kBins - 1) / (mx - mn), static_cast<float>((kBins - 1) / 64.0 * scale)), 1e30f);
-  auto bin_of = [&](float x) { return static_cast<int>(fminf((mx - x) * per_x, static_cast<float>(kBins - 1))); };
+  // bins: the row's range, or 64 octaves of weight where that is less; the last one holds weights of 0 alone
+  // by halves: mx - x may be past fp32's range
+  const float half = 0.5f * mx;
+  const float per_half = fminf(fmaxf((kBins - 1.5f) / __builtin_fmaf(-0.5f, mn, half), static_cast<float>((kBins - 1) / 32.0 * scale)), 1e30f);
+  const double per_x = 0.5 * static_cast<double>(per_half);
+  auto bin_of = [&](float x) {
+    return static_cast<int>(fminf(__builtin_fmaf(-0.5f, x, half) * per_half, static_cast<float>(kBins - 1)));
+  };
   auto t_of = [&](float x) { return (static_cast<double>(mx) - static_cast<double>(x)) * scale; };
   bool by_count = k > 0 && k < V;
   const bool by_min = min_p > 0.f;
   const double t_min = by_min ? -log2(static_cast<double>(fminf(min_p, 1.f))) : 0.0;
+  // An element's weight, times 2^shift, in bins but the last: that at its bin's begin times a Taylor polynomial of what is
+  // left, at most 64 octaves / kBins.  Weighing is what a row of fp32 costs: the vector unit is busy for three quarters
+  // of a lone row's time.  Only temperatures below 1e-36 have wider bins; bf16 rows seldom come here.
+  const double inv_T = 1.0 / static_cast<double>(T), width = inv_T / per_x;
+  const bool narrow = kWide && width <= 64.0 * kLn2 / (kBins - 1) * 1.01;
+  auto weigh = [&](float x, int b) -> uint64_t {
+    const double far = static_cast<double>(x) - static_cast<double>(mx);  // may be past fp32's range
+    if (!narrow) return weight_of(far * -scale, P.shift);
+    const double a = __builtin_fma(far, inv_T, static_cast<double>(b) * width);
+    double p = kBins < 2048 ? __builtin_fma(1.0 / 720, a, 1.0 / 120) : 1.0 / 120;  // off by 2e-13 at most
+    p = __builtin_fma(p, a, 1.0 / 24);
+    p = __builtin_fma(p, a, 1.0 / 6);
+    p = __builtin_fma(p, a, 0.5);
+    p = __builtin_fma(p, a, 1.0);
+    p = __builtin_fma(p, a, 1.0);
+    return __builtin_bit_cast(uint64_t, __builtin_fma(p, S.power[b], 0x1p52)) - (uint64_t{0x433} << 52);
+  };
 
   // bins' sums and counts become inclusive prefix sums
   auto scan = [&](uint64_t* mass, uint32_t* count, bool counts) {
@@ -811,7 +844,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
       cut = S.bin;
     }
   } else if (by_min && !(top_p < 1.f)) {
-    cut = static_cast<int>(fmin(t_min / scale * static_cast<double>(per_x) + 1.0, kBins - 1.0));  // one more for rounding
+    cut = static_cast<int>(fmin(t_min / scale * per_x + 1.0, kBins - 1.0));  // one more for rounding
   }
   // Where the bins up to `cut` hold few elements (a small top-k, or min-p alone), all of them go to the list, and the three
   // sums are found there: no weights in bins, no further pass.
@@ -887,7 +920,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
     }
   }
   // Searches read the row's elements of a bin again, from memory, unless mass2 holds them (until a bin is divided): all of
-  // the bins up to `cut` where they fit, put there as they are weighed, else those of top-p's bin and of the ones
+  // the bins up to `cut` where they fit, put there before they are weighed, else those of top-p's bin and of the ones
   // that the last search can end in, fetched in one pass for both.  (fp32 rows only: bf16 ones seldom come here.)
   bool held = kWide && by_count && S.count[cut] <= kBins;
   int held_to = held ? cut : -1, held_p = -1, held_lo = 0, held_hi = -1;  // bins up to held_to, held_p, held_lo to held_hi
@@ -896,23 +929,41 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
     if (to < kBins) S.mass2[to] = key_of(x, index);
   };
   if (tid == 0) S.n_held = 0;
-  if (by_count || held) __syncthreads();  // the search for cut is over: S.bin may be used again
+  if constexpr (kWide)
+    for (int b = tid; b <= cut; b += NT) S.power[b] = __builtin_ldexp(exp2_neg(b * width * kLog2e), P.shift);
+  __syncthreads();  // the search for cut is over, too: S.bin may be used again
 
   uint64_t z_min = 0;  // the weight of what min-p keeps
-  each([&](const u32x4_t& v, int i0) {
+  const int weighty = min(cut, kBins - 2);
+  auto add = [&](float x, int b) {
+    const uint64_t w = weigh(x, b);
+    atomicAdd(reinterpret_cast<unsigned long long*>(&S.mass[b]), static_cast<unsigned long long>(w));
+    if (by_min && t_of(x) <= t_min) z_min += w;
+  };
+  if (held) {
+    each([&](const u32x4_t& v, int i0) {
 #pragma unroll
-    for (int e = 0; e < G; ++e) {
-      const float x = element(v, e);
+      for (int e = 0; e < G; ++e) {
+        const float x = element(v, e);
+        if (bin_of(x) <= cut && x > -INFINITY) hold(x, i0 + e);
+      }
+    });
+    __syncthreads();
+    for (int i = tid; i < static_cast<int>(S.n_held); i += NT) {
+      const float x = value_of(S.mass2[i]);
       const int b = bin_of(x);
-      if (b > cut || !(x > -INFINITY)) continue;
-      if (kWide && held) hold(x, i0 + e);
-      const double t = t_of(x);  // mx - x may be past fp32's range
-      if (t >= 64.0) continue;   // a weight of 0
-      const uint64_t w = weight_of(t, P.shift);
-      atomicAdd(reinterpret_cast<unsigned long long*>(&S.mass[b]), static_cast<unsigned long long>(w));
-      if (by_min && t <= t_min) z_min += w;
+      if (b <= weighty) add(x, b);
     }
-  });
+  } else {
+    each([&](const u32x4_t& v, int) {
+#pragma unroll
+      for (int e = 0; e < G; ++e) {
+        const float x = element(v, e);
+        const int b = bin_of(x);  // -inf is in the last
+        if (b <= weighty) add(x, b);
+      }
+    });
+  }
   if (by_min) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) z_min += shfl_xor64(z_min, d);
@@ -960,7 +1011,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
       __syncthreads();
       const int n = static_cast<int>(S.n);
       if (n <= kList) {
-        for (int i = tid; i < n; i += NT) S.w[i] = weight_of(t_of(value_of(S.key[i])), P.shift);
+        for (int i = tid; i < n; i += NT) S.w[i] = bin == kBins - 1 ? 0 : weigh(value_of(S.key[i]), bin);
         __syncthreads();
         for (int i = tid; i < n; i += NT) {
           const uint64_t key = S.key[i], w = S.w[i];
@@ -1015,7 +1066,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
         if (bin_of(x) != bin || key < klo || key > khi) return;
         const int b = static_cast<int>((khi - key) >> bits);
         atomicAdd(reinterpret_cast<unsigned long long*>(&S.mass2[b]),
-                  static_cast<unsigned long long>(weight_of(t_of(x), P.shift)));
+                  static_cast<unsigned long long>(bin == kBins - 1 ? 0 : weigh(x, bin)));
         atomicAdd(&S.count2[b], 1u);
       });
       __syncthreads();
@@ -1093,8 +1144,10 @@ void launch(const SampleParams& P, hipStream_t st) {
 // Threads a row.  What a row does in turn (bins, sums, searches) is most of a short row's time, and more threads shorten it
 // where a CU has a row or two; where it has more, small workgroups fill it better.  us with 256, 512 and 1024, top-k,
 // top-p and min-p together, bf16 of 8194: one row 14.7, 11.3, 11.6; 256 rows 17.2, 13.5, 13.8; 512 18.4, 15.9, 25.8; 768
-// 20.9, 25.9, 37.3; 4096 77, 103.  Longer rows, with 512 and 1024: 256 rows of 100003 bf16 37.0, 35.7, fp32 134, 92; 300 46.5,
-// 63.6 and 139, 153 (temperature alone 214, 183); 1024 of 32000 bf16 46.8, 69.2, fp32 117, 129.
+// 20.9, 25.9, 37.3; 4096 77, 103.  Longer rows, with 512 and 1024: 256 rows of 100003 bf16 37.0, 35.7; 300 46.5, 63.6; 1024 of
+// 32000 46.8, 69.2.  fp32, temperature alone: 256 rows of 100003 98, 67; 300 107, 110 (settings of
+// their own, so that a third ends early, 110, 103); 600 183, 169; 300 of 50003 54, 61; 64 of 32000 28, 23; 1024 of 32000
+// 81, 97.
 template <bool kWide>
 void launch_rows(const SampleParams& P, hipStream_t st) {
   constexpr uint32_t kCUs = 256;
@@ -1103,7 +1156,7 @@ void launch_rows(const SampleParams& P, hipStream_t st) {
       launch<kWide, 256>(P, st);
     else
       launch<kWide, 512>(P, st);
-  } else if (P.items > kCUs && (!kWide || P.vocab <= 50000)) {
+  } else if (P.items > kCUs && (!kWide || P.vocab <= 60000)) {
     launch<kWide, 512>(P, st);
   } else {
     launch<kWide, 1024>(P, st);
