@@ -303,7 +303,7 @@ int64_t yapd_attn_tree_workspace(int rows, int max_q, int n_q, int n_heads, int 
  * before the first is written.  base, kept, n_kept: device int32; kv_pools: a
  * host array of pool addresses.  Entries whose source or destination the table
  * does not map to a page in [0, n_pages) are left out.  The pages written must belong to
- * one row alone.  max_kept <= 64, rows <= 65535. */
+ * one row alone; pools that overlap are refused.  max_kept <= 64, rows <= 65535. */
 int yapd_kv_keep(void* const* kv_pools, int n_layers, int bits, int64_t n_pages, int n_heads,
                  const int32_t* page_table, int table_stride, int table_cols, const int32_t* base,
                  const int32_t* kept, int kept_stride, int max_kept, const int32_t* n_kept, int rows, void* stream);

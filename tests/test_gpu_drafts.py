@@ -243,3 +243,40 @@ def test_a_captured_round_follows_its_buffers(dev, bits):
         torch.cuda.synchronize()
         for x, y in zip(got, (out, token, lp, *kv.pools)):
             assert torch.equal(x, y)
+
+
+def test_calls_on_two_streams_at_once(dev):
+    """Attention in parts (a workspace each), writing, drawing: two streams that wait for nothing of each other."""
+    g = torch.Generator(device=dev).manual_seed(3)
+    pages, rows = 200, 2
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(1)).int().view(rows, -1).to(dev)
+    kv_len = i32([1500, 900])
+    mask = torch.ones(rows, 1, dtype=torch.int64, device=dev)
+    inputs = []
+    for _ in range(2):
+        pool = torch.randint(0, 256, (pages, 2, H, 1040), generator=g, dtype=torch.uint8, device=dev)
+        pool[..., 1024:] = 120
+        x = torch.randn(3, rows, 1, H, 64, generator=g, device=dev).bfloat16()
+        logits = torch.randn(rows, 5000, generator=g, device=dev)
+        inputs.append((pool, x, logits, torch.rand(rows, generator=g, device=dev)))
+
+    def step(pool, x, logits, u):
+        q, k, v = x
+        out = torch.empty_like(q)
+        kernels.kv8_write(k[:, 0], v[:, 0], pool, table, kv_len - 1)
+        kernels.attn_tree(q, pool, table, kv_len, mask, out, SCALE)
+        return out, scoring.sample_tokens(logits, u, temperature=0.8, top_p=0.9).token
+
+    want = [step(*a) for a in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(step(*inputs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out, token in got[i]:
+            assert torch.equal(out, want[i][0]) and torch.equal(token, want[i][1])

@@ -121,6 +121,16 @@ def test_kv_keep_refuses(over, msg):
     assert b"layer 1" in lib.yapd_last_error()
 
 
+@pytest.mark.parametrize("bits,tile", [(8, 1040), (16, 2048)])
+def test_kv_keep_refuses_a_pool_given_twice(bits, tile):
+    size = 9 * 2 * 16 * tile
+    lib = kernels.load_library()
+    for addresses in ((P, P), (P, P + size, P + size - 16), (P + size - 16, P + 2 * size, P)):
+        pools = (ctypes.c_void_p * len(addresses))(*addresses)
+        assert lib.yapd_kv_keep(pools, len(addresses), bits, 9, 16, P, 4, 4, P, P, 4, 4, P, 3, None) == EINVAL
+        assert b"overlap" in lib.yapd_last_error()
+
+
 def test_kv8_copy_pages_refuses():
     pools = (ctypes.c_void_p * 1)(P)
     ids = (ctypes.c_int32 * 2)(1, 9)

@@ -126,6 +126,13 @@ extern "C" int yapd_kv_keep(void* const* kv_pools, int n_layers, int bits, int64
   for (int l = 0; l < n_layers; ++l)
     YAPD_REQUIRE(kv_pools[l] && (reinterpret_cast<uintptr_t>(kv_pools[l]) & 15u) == 0,
                  "kv_keep: layer %d's pool must be non-NULL and 16-byte aligned", l);
+  // a pool given twice would be moved twice, in no order
+  const uintptr_t bytes = static_cast<uintptr_t>(n_pages) * 2 * n_heads * (bits == 8 ? yapd::kTile8 : yapd::kHeadTile * 2);
+  for (int l = 1; l < n_layers; ++l)
+    for (int m = 0; m < l; ++m) {
+      const uintptr_t x = reinterpret_cast<uintptr_t>(kv_pools[l]), y = reinterpret_cast<uintptr_t>(kv_pools[m]);
+      YAPD_REQUIRE((x > y ? x - y : y - x) >= bytes, "kv_keep: the pools of layers %d and %d overlap", m, l);
+    }
   yapd::KeepParams P;
   P.n_pages = n_pages;
   P.table = page_table;
