@@ -96,6 +96,15 @@ def test_lengths_past_the_table(dev, bits):
     c.check(out)
 
 
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("n,kv,window,sinks", [(5, [0, 3, 4, 5], None, 0), (5, [2, 0, 40, 1], 5, 2), (40, [0, 17, 39], 50, 3),
+                                               (64, [1, 0], None, 0)])
+def test_rows_of_fewer_keys_than_nodes(dev, n, kv, window, sinks, bits):
+    """The first nodes then stand before the row's begin: nobody sees them, and a row without keys gives zeros."""
+    c = Case(n_nodes=[n] * len(kv), kv_lens=kv, H=4, bits=bits, window=window, sinks=sinks, seed=n)
+    c.check(c.run(dev, kernels))
+
+
 def test_a_slice_of_a_wider_buffer(dev):
     c = Case(n_nodes=[9, 9], kv_lens=[40, 100], H=8, bits=8)
     t = c.device(dev)
