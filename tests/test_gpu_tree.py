@@ -70,6 +70,18 @@ def test_packed_rows(dev, n, kv, H, window, sinks, bits):
 
 
 @pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("rows", [130, 256, 257])
+def test_many_ragged_rows(dev, rows, bits):
+    """More workgroups than the chip holds: up to 256 rows are taken by cost, each once; rows of no nodes or no keys among them."""
+    n = [(0, 1, 3, 40, 2, 17)[i * i % 6] for i in range(rows)]
+    kv = [n[i] + i * 37 % 190 for i in range(rows)]
+    c = Case(n_nodes=n, kv_lens=kv, H=12, bits=bits, window=120, sinks=5, packed=True, tail_q=3, seed=rows)
+    c.check(c.run(dev, kernels))
+    c = Case(n_nodes=[1] * rows, kv_lens=[1 + i * 61 % 700 for i in range(rows)], H=32, bits=bits, seed=rows)
+    c.check(c.run(dev, kernels))
+
+
+@pytest.mark.parametrize("bits", [16, 8])
 @pytest.mark.parametrize("max_q", [1, 20, 40])
 def test_rows_longer_than_max_q(dev, max_q, bits):
     """The first max_q nodes of a row are computed as the row's first, a row of more nodes than a mask has bits too."""

@@ -17,12 +17,12 @@
 //     multiply the scores, V's the weights before they are rounded to bf16.
 //
 // Single tokens and long rows are bound by memory: 256 ragged rows of 60 to 4000 keys x 16 heads at 8 bits 202 us, 5.4
-// TB/s (half of the vector unit's cycles are free; in bf16 the same takes 350); three rows of 13 nodes on 20000 to 30000 keys
+// TB/s (half of the vector unit's cycles are free; in bf16 the same takes 331); three rows of 13 nodes on 20000 to 30000 keys
 // in bf16 57 us, 5.4 TB/s, 5 of it the join.  Trees at 8 bits are not: 130 rows of 1 to 64 nodes on up to 2033 keys
-// 136 us, 3.0 TB/s.  A chunk costs a wave 230 vector instructions and a tile of 16 queries 110 more with 16 exponentials, at
-// two waves a SIMD (223 registers) their chains are not hidden behind each other.  Measured and left out there: K's
-// product on v_mfma_i32_16x16x64_i8 with Q in two bytes (no conversion of K; 184 registers) 145 us with one set of
-// loads and 133 with two, but Q would be rounded; three waves a SIMD 208 (spills); 512 threads a head 179.
+// 127 us, 3.2 TB/s.  A chunk costs a wave 230 vector instructions and a tile of 16 queries 110 more with 16 exponentials, at
+// two waves a SIMD (223 registers) their chains are not hidden behind each other.  Measured and left out there (against
+// 138): K's product on v_mfma_i32_16x16x64_i8 with Q in two bytes (no conversion of K; 184 registers) 145 us with one set
+// of loads and 133 with two, but Q would be rounded; three waves a SIMD 208 (spills); 512 threads a head 179.
 #include <algorithm>
 #include <type_traits>
 
@@ -49,6 +49,7 @@ struct TreeParams {
   int rows, max_q, n_q, H;
   int window, sinks;
   int parts;
+  float class_scale;  // of a row's cost (row_by_cost); 0: rows are taken as they come
   float* part_o;   // [parts, n_q, H, 64]
   float* part_ml;  // [parts, n_q, H, 2]
   float scale_log2;
@@ -70,6 +71,57 @@ __device__ __forceinline__ bool find_tree(const TreeParams& P, int row, Tree& t)
   t.kvl = min(max(P.kv_len[row], 0), P.table_cols * kPageSize);
   t.ctx = t.kvl - t.n;
   return t.qc > 0;
+}
+
+constexpr int kSorted = 256;  // rows that are ordered by cost, four a lane
+constexpr int kClasses = 64;
+
+// Row `slot` by cost, the costliest first: the keys that it sees times what a chunk of them costs it.  A launch of more
+// workgroups than the chip holds ends when the last one started does, and that one should be small.  Rows of one of 64
+// classes stay as they come.  Every wave finds its row by itself, by halving the classes.
+// us as they come, and so: 16 heads, 256 single tokens on 60 to 4000 keys at 8 bits 213, 202, bf16 352, 331; 130 trees of 1 to 64
+// nodes 136, 127; 64 of 64 nodes on 200 to 1500 keys 66, 55, bf16 89, 78; 128 of them 116, 108, bf16 163, 146; equal rows lose
+// up to 0.5.
+template <int NQT>
+__device__ __forceinline__ int row_by_cost(const TreeParams& P, int slot, int lane) {
+  int cls[kSorted / 64];
+#pragma unroll
+  for (int j = 0; j < kSorted / 64; ++j) {
+    const int r = lane + 64 * j;
+    cls[j] = -1;
+    if (r >= P.rows) continue;
+    int n = P.max_q;
+    if (P.q_start != nullptr) n = min(max(P.q_start[r + 1], 0), P.n_q) - min(max(P.q_start[r], 0), P.n_q);
+    const int kvl = min(max(P.kv_len[r], 0), P.table_cols * kPageSize);
+    // of two query tiles a chunk takes 230 instructions and 110 a tile; of more than 32 nodes half the waves go over it
+    const float each = NQT == 1 ? 1.f : n > 32 ? 900.f : n > 16 ? 450.f : 340.f;
+    const float keys = fminf(static_cast<float>(kvl), static_cast<float>(P.window) + static_cast<float>(P.sinks) + n);
+    cls[j] = n > 0 ? static_cast<int>(fminf(keys * each * P.class_scale, kClasses - 1.f)) : 0;
+  }
+  int lo = 0, hi = kClasses, above = 0;  // more than `slot` rows are in classes from lo on, `above` of them from hi on
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < kSorted / 64; ++j) c += static_cast<int>(__popcll(__ballot(cls[j] >= mid)));
+    if (c > slot) {
+      lo = mid;
+    } else {
+      hi = mid;
+      above = c;
+    }
+  }
+  int k = slot - above, row = 0;  // the k-th row of class lo
+#pragma unroll
+  for (int j = 0; j < kSorted / 64; ++j) {
+    const uint64_t in = __ballot(cls[j] == lo);
+    const int c = static_cast<int>(__popcll(in));
+    const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(in >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(in), 0));
+    const uint64_t at = __ballot(cls[j] == lo && before == k);
+    if (k >= 0 && k < c) row = 64 * j + __ffsll(static_cast<unsigned long long>(at)) - 1;
+    k -= c;
+  }
+  return __builtin_amdgcn_readfirstlane(row);
 }
 
 // Bits of the keys from `shift` positions behind the tree's first node on (before it where negative: the
@@ -209,7 +261,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NQT > 1 ? 2
   const int groups = P.H / HPW;
   const int item = static_cast<int>(blockIdx.x) / groups;
   const int h = (static_cast<int>(blockIdx.x) - item * groups) * HPW + hsub;
-  const int row = item / P.parts, part = item - row * P.parts;
+  int row = item / P.parts;
+  const int part = item - row * P.parts;
+  if (P.class_scale > 0.f) row = row_by_cost<NQT>(P, row, lane);
   Tree t;
   if (!find_tree(P, row, t)) return;  // the whole workgroup
   const int g = lane >> 4, n = lane & 15;
@@ -688,6 +742,14 @@ extern "C" int yapd_attn_tree(const void* q, int64_t q_tok_stride, const void* k
   P.window = std::min(window, yapd::kCap);
   P.sinks = std::min(sinks, yapd::kCap);
   P.parts = c.parts;
+  // Workgroups that the chip does not hold at once: two a CU with two query tiles, else four.
+  const int64_t groups = static_cast<int64_t>(rows) * n_heads * c.w / 4, held = c.nqt == 1 ? 1024 : 512;
+  P.class_scale = 0.f;
+  if (c.parts == 1 && rows > 1 && rows <= yapd::kSorted && groups > held) {
+    const double most = std::min<double>(std::min<double>(max_kv, table_cols * 16.0),
+                                         static_cast<double>(P.window) + P.sinks + max_q);
+    P.class_scale = static_cast<float>(yapd::kClasses / (most * (c.nqt == 1 ? 1.0 : 900.0)));
+  }
   P.part_o = workspace;
   P.part_ml = c.parts == 1 ? nullptr : workspace + tokens * yapd::kHeadDim;
   P.scale_log2 = scale * 1.4426950408889634f;
