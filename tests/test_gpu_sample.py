@@ -307,3 +307,20 @@ def test_fp32_rows_of_any_range(dev, V):
             full = lambda v, dt=torch.float32: torch.full((len(rows),), v, dtype=dt)  # noqa: E731
             check(dev, buf[:, off:off + V], dict(u=torch.rand(len(rows), generator=g), T=torch.tensor(temps),
                                                  k=full(k, torch.int32), p=full(p), m=full(m)), min_margin=0.0)
+
+
+@pytest.mark.parametrize("n", [257, 600, 1025])
+def test_many_long_fp32_rows_of_different_settings(dev, n):
+    """More rows than CUs with a vocabulary of one row a CU: up to 1024 are taken by what their settings cost, each once."""
+    V = 60011
+    base = torch.randn(5, V, generator=torch.Generator().manual_seed(n)) * 2
+    x = base.to(dev)[torch.arange(n, device=dev) % 5] + torch.arange(n, device=dev)[:, None] / 64
+    s = settings(n, n)
+    r = scoring.sample_tokens(x, s["u"].to(dev), temperature=s["T"].to(dev), top_k=s["k"].to(dev), top_p=s["p"].to(dev),
+                              min_p=s["m"].to(dev))
+    for i in range(n):  # a row alone gives the same
+        one = {k: v[i:i + 1].to(dev) for k, v in s.items()}
+        a = scoring.sample_tokens(x[i:i + 1], one["u"], temperature=one["T"], top_k=one["k"], top_p=one["p"], min_p=one["m"])
+        assert torch.equal(a.token, r.token[i:i + 1]) and torch.equal(a.logprob, r.logprob[i:i + 1])
+    few = torch.arange(0, n, max(n // 25, 1))
+    check(dev, x[few.to(dev)], {k: v[few] for k, v in s.items()}, min_margin=0.0)

@@ -49,6 +49,7 @@ struct SampleParams {
   float top_p_all;
   const float* min_p;
   float min_p_all;
+  bool by_cost;  // rows are taken by cost (row_by_cost)
   int64_t* token;
   float* logprob;
 };
@@ -591,13 +592,53 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT, 
   return true;
 }
 
+// Row `slot` by cost, the costliest first, where a CU holds one row, rows are more than CUs and settings differ: those
+// with a temperature (three or four passes), then those of a small top-k, whose few elements are soon in a list, then those
+// that want the largest logit alone.  What starts last should end soon.  A thread a row, at most NT of them.
+template <int NT, bool kWide>
+__device__ __forceinline__ uint32_t row_by_cost(const SampleParams& P, Shared<NT, kWide>& S, uint32_t slot) {
+  const uint32_t i = threadIdx.x;
+  const int lane = i & 63, wave = i >> 6;
+  int cls = 3;  // no row
+  if (i < P.items) {
+    const float T = P.temperature ? P.temperature[i] : P.temperature_all;
+    const int k = P.top_k ? P.top_k[i] : P.top_k_all;
+    cls = !(T > 0.f) || k == 1 ? 2 : k > 0 && k <= kList ? 1 : 0;
+  }
+  uint64_t before = 0;  // of this wave's rows, those of its class that come before, and counts of the classes, 16 bits each
+  uint64_t counts = 0;
+#pragma unroll
+  for (int c = 0; c < 3; ++c) {
+    const uint64_t in = __ballot(cls == c);
+    counts |= static_cast<uint64_t>(__popcll(in)) << (16 * c);
+    if (cls == c) before = __popcll(in & ((uint64_t{1} << lane) - 1));
+  }
+  if (lane == 0) S.part[wave] = counts;
+  __syncthreads();
+  uint64_t all = 0, earlier = 0;
+  for (int w = 0; w < NT / 64; ++w) {
+    if (w == wave) earlier = all;
+    all += S.part[w];
+  }
+  if (cls < 3) {
+    uint32_t place = static_cast<uint32_t>(before + (earlier >> (16 * cls) & 0xffffu));
+    for (int c = 0; c < cls; ++c) place += static_cast<uint32_t>(all >> (16 * c) & 0xffffu);
+    if (place == slot) S.first = i;
+  }
+  __syncthreads();
+  return S.first;
+}
+
 // One workgroup a row, which every pass reads again (from the caches: a speech vocabulary's row is 16 KB).
 template <bool kWide, int NT>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sample_kernel(const SampleParams P) {
   constexpr int G = kWide ? 4 : 8, kBytes = kWide ? 4 : 2, kBins = Shared<NT, kWide>::kBins;
   __shared__ Shared<NT, kWide> S;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const uint32_t item = blockIdx.x;
+  uint32_t item = blockIdx.x;
+  if constexpr (kWide && NT == 1024) {
+    if (P.by_cost) item = row_by_cost<NT, kWide>(P, S, item);
+  }
   const uint32_t r = item / P.bl;
   const int64_t at = (r * P.seq_stride + static_cast<int64_t>(item - r * P.bl) * P.pos_stride) * kBytes;
   const uintptr_t row = reinterpret_cast<uintptr_t>(P.logits) + at;
@@ -1149,7 +1190,7 @@ void launch(const SampleParams& P, hipStream_t st) {
 // their own, so that a third ends early, 110, 103); 600 183, 169; 300 of 50003 54, 61; 64 of 32000 28, 23; 1024 of 32000
 // 81, 97.
 template <bool kWide>
-void launch_rows(const SampleParams& P, hipStream_t st) {
+void launch_rows(SampleParams& P, hipStream_t st) {
   constexpr uint32_t kCUs = 256;
   if (P.vocab <= 10000) {
     if (P.items > 2 * kCUs)
@@ -1159,6 +1200,7 @@ void launch_rows(const SampleParams& P, hipStream_t st) {
   } else if (P.items > kCUs && (!kWide || P.vocab <= 60000)) {
     launch<kWide, 512>(P, st);
   } else {
+    P.by_cost = kWide && P.items > kCUs && P.items <= 1024 && (P.temperature != nullptr || P.top_k != nullptr);
     launch<kWide, 1024>(P, st);
   }
 }
@@ -1182,9 +1224,9 @@ extern "C" int yapd_sample_tokens(const void* logits, int wide, int64_t seq_stri
   YAPD_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (wide ? 3u : 1u)) == 0, "sample_tokens: misaligned logits");
   int bits = 0;  // vocab <= 2^bits, so that all weights together stay below 2^63
   while ((int64_t{1} << bits) < vocab) ++bits;
-  const yapd::SampleParams P{logits, seq_stride, pos_stride, static_cast<uint32_t>(items), static_cast<uint32_t>(bl), vocab,
+  yapd::SampleParams P{logits, seq_stride, pos_stride, static_cast<uint32_t>(items), static_cast<uint32_t>(bl), vocab,
                              62 - bits < 51 ? 62 - bits : 51, uniform, temperature, temperature_all, top_k, top_k_all, top_p,
-                             top_p_all, min_p, min_p_all, token, logprob};
+                             top_p_all, min_p, min_p_all, false, token, logprob};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (wide)
     yapd::launch_rows<true>(P, st);
