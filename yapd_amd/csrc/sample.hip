@@ -24,7 +24,8 @@
 // atomics a word) nearly as much, and each row's chain is hidden by three others only.  fp32, a row of 100003: 15 us for the
 // largest, 50 with a temperature, 57 with top-p (three passes; instructions bound it: 67 an element before its weight was a
 // polynomial within its bin, then 62 us).  300 such rows, 120 MB, 23 us as bytes: 110 us with a temperature, all filters with a
-// small top-k 88, settings of their own 103 to 107; 300 rows on 256 CUs are two turns, and every pass fetches the rows again.
+// small top-k 88, 300 rows on 256 CUs are two turns, and every pass fetches the rows again. With
+// settings of their own 103 as they come and 75 the costliest first.
 #include "attn_tile.h"
 #include "common.h"
 
@@ -769,8 +770,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void sa
   }
 
   const double scale = kLog2e / static_cast<double>(T);
-  // bins: the row's range, or 64 octaves of weight where that is less; the last one holds weights of 0 alone
-  // by halves: mx - x may be past fp32's range
+  // bins: the row's range, or 64 octaves of weight where that is less; the last one holds weights of 0 alone.
+  // By halves: mx - x may be past fp32's range.
   const float half = 0.5f * mx;
   const float per_half = fminf(fmaxf((kBins - 1.5f) / __builtin_fmaf(-0.5f, mn, half), static_cast<float>((kBins - 1) / 32.0 * scale)), 1e30f);
   const double per_x = 0.5 * static_cast<double>(per_half);
@@ -1187,7 +1188,7 @@ void launch(const SampleParams& P, hipStream_t st) {
 // top-p and min-p together, bf16 of 8194: one row 14.7, 11.3, 11.6; 256 rows 17.2, 13.5, 13.8; 512 18.4, 15.9, 25.8; 768
 // 20.9, 25.9, 37.3; 4096 77, 103.  Longer rows, with 512 and 1024: 256 rows of 100003 bf16 37.0, 35.7; 300 46.5, 63.6; 1024 of
 // 32000 46.8, 69.2.  fp32, temperature alone: 256 rows of 100003 98, 67; 300 107, 110 (settings of
-// their own, so that a third ends early, 110, 103); 600 183, 169; 300 of 50003 54, 61; 64 of 32000 28, 23; 1024 of 32000
+// their own 110, 103, and 75 by cost); 600 183, 169; 300 of 50003 54, 61; 64 of 32000 28, 23; 1024 of 32000
 // 81, 97.
 template <bool kWide>
 void launch_rows(SampleParams& P, hipStream_t st) {
