@@ -24,8 +24,8 @@
 // atomics a word) nearly as much, and each row's chain is hidden by three others only.  fp32, a row of 100003: 15 us for the
 // largest, 50 with a temperature, 57 with top-p (three passes; instructions bound it: 67 an element before its weight was a
 // polynomial within its bin, then 62 us).  300 such rows, 120 MB, 23 us as bytes: 110 us with a temperature, all filters with a
-// small top-k 88, 300 rows on 256 CUs are two turns, and every pass fetches the rows again. With
-// settings of their own 103 as they come and 75 the costliest first.
+// small top-k 88 (300 rows on 256 CUs are two turns, and every pass fetches the rows again), settings of their own 103
+// as the rows come and 75 the costliest first.
 #include "attn_tile.h"
 #include "common.h"
 
