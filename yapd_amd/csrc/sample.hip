@@ -425,13 +425,17 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT, 
       n += count;
       if (by_min && b != kTiny && w >= min_p) min_mass += m;
     });
+    // Sums are rounded, so they are added up in an order in which they never fall: the upper half of every 2d lanes adds
+    // the lower half's sum to its own.  Rounding keeps order, so a lane's sum is at least the one before it, and the same
+    // where the lane has no elements.  (Else a target between two roundings of one sum is met by a lane without any.)
     double mi = mass;
     uint32_t ni = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const double ml = __shfl_up(mi, d);
-      const uint32_t nl = __shfl_up(ni, d);
-      if (lane >= d) {
+      const int from = (lane & -2 * d) + d - 1;  // the lower half's last
+      const double ml = __shfl(mi, from);
+      const uint32_t nl = __shfl(ni, from);
+      if (lane & d) {
         mi += ml;
         ni += nl;
       }
@@ -458,7 +462,9 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT, 
       z_min += S.sum_a[w];
       n_total += static_cast<uint32_t>(S.part[w]);
     }
-    me += before;  // the sums up to this thread's values; a thread's end is the next one's begin to the last bit
+    // The sums up to this thread's values; a thread's end is the next one's begin to the last bit, and the ends never
+    // fall: exactly one thread meets a target, and it has elements.
+    me += before;
     mi += before;
     ne += n_before;
     ni += n_before;
