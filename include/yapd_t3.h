@@ -113,6 +113,7 @@ int yapd_token_logprobs(const void* logits, int wide, int64_t seq_stride, int64_
  * A row that holds a NaN or +inf, or -inf alone: token -1, logprob NaN.
  * uniform [rows * bl] fp32; temperature, top_p, min_p (fp32) and top_k (int32) are
  * [rows * bl], or NULL: the number beside it holds for every row.  token int64, logprob fp32.
+ * Outputs that share memory with an input, or with each other, are refused.
  * Weights are right to 4e-12 of themselves; those of fp32 logits are rounded to 64-bit
  * fixed point besides (2^-51, with more than 2^11 tokens 2^-62 times the next power of
  * two).  They are summed in an order that depends on nothing else: the same call gives

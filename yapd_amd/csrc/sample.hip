@@ -1212,6 +1212,25 @@ void launch_rows(SampleParams& P, hipStream_t st) {
   }
 }
 
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + b_bytes && y < x + a_bytes;
+}
+
+// Whether [b, b + b_bytes) shares a byte with a row of the logits.  Rows are gone through only where it lies among them.
+bool overlaps_logits(const SampleParams& P, int64_t elem, const void* b, int64_t b_bytes) {
+  const char* base = static_cast<const char*>(P.logits);
+  const int64_t rows = P.items / P.bl, seq = P.seq_stride * elem, pos = P.pos_stride * elem, row_bytes = P.vocab * elem;
+  const int64_t seq_end = (rows - 1) * seq, pos_end = (P.bl - 1) * pos;
+  const int64_t lo = (seq_end < 0 ? seq_end : 0) + (pos_end < 0 ? pos_end : 0);
+  const int64_t hi = (seq_end > 0 ? seq_end : 0) + (pos_end > 0 ? pos_end : 0) + row_bytes;
+  if (!overlap(base + lo, hi - lo, b, b_bytes)) return false;
+  for (int64_t r = 0; r < rows; ++r)
+    for (int64_t i = 0; i < P.bl; ++i)
+      if (overlap(base + r * seq + i * pos, row_bytes, b, b_bytes)) return true;
+  return false;
+}
+
 }  // namespace
 }  // namespace yapd
 
@@ -1234,6 +1253,18 @@ extern "C" int yapd_sample_tokens(const void* logits, int wide, int64_t seq_stri
   yapd::SampleParams P{logits, seq_stride, pos_stride, static_cast<uint32_t>(items), static_cast<uint32_t>(bl), vocab,
                              62 - bits < 51 ? 62 - bits : 51, uniform, temperature, temperature_all, top_k, top_k_all, top_p,
                              top_p_all, min_p, min_p_all, false, token, logprob};
+  // a row's output is written while other rows are still read, and rows by cost read every row's settings
+  const void* const outs[2] = {token, logprob};
+  for (int o = 0; o < 2; ++o) {
+    const int64_t bytes = items * (o == 0 ? 8 : 4);
+    for (const void* in : {static_cast<const void*>(uniform), static_cast<const void*>(temperature),
+                           static_cast<const void*>(top_k), static_cast<const void*>(top_p), static_cast<const void*>(min_p)})
+      YAPD_REQUIRE(!in || !yapd::overlap(in, items * 4, outs[o], bytes),
+                   "sample_tokens: token and logprob must not overlap uniform or the settings");
+    YAPD_REQUIRE(!yapd::overlaps_logits(P, wide ? 4 : 2, outs[o], bytes),
+                 "sample_tokens: token and logprob must not overlap the logits");
+  }
+  YAPD_REQUIRE(!yapd::overlap(token, items * 8, logprob, items * 4), "sample_tokens: token and logprob overlap");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (wide)
     yapd::launch_rows<true>(P, st);

@@ -302,7 +302,7 @@ def launch_token_logprobs(logits, tokens, k: int, logprob, entropy, top_logprob,
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, token: torch.Tensor, logprob: torch.Tensor, *,
                   temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> None:
     """A token drawn from every row of ``logits`` with the random number ``uniform`` (``yapd_sample_tokens``), into
-    caller tensors; see :func:`yapd_amd.scoring.sample_tokens`."""
+    caller tensors that share no memory with the inputs; see :func:`yapd_amd.scoring.sample_tokens`."""
     dev = logits.device
     if elsewhere(logits):
         with torch.cuda.device(dev):  # the launch goes to the current device
