@@ -283,7 +283,8 @@ int yapd_kv8_unpack(const void* kv_pool8, int64_t n_pages8, const int32_t* page_
  * number of other bits set in its mask.  out = softmax(q K^T * scale) V over the
  * keys seen; a node that sees none gets zeros.
  *   q, out, page tables, kv_len, q_start, max_q, n_q, max_kv and workspace: as
- *   yapd_attn_window; max_q <= 64 and window >= max_q.  mask: device int64 [n_q].
+ *   yapd_attn_window; max_q <= 64.  window >= max_q; with q_start, where max_q only bounds the rows' nodes,
+ *   window >= 1.  mask: device int64 [n_q].
  *   kv_pool: bits = 16 the bf16 pool, bits = 8 the 8-bit pool.  K and V have to be
  *   finite where any node of the row sees them.
  * Scores, sums and statistics are fp32; the weights (of an 8-bit pool times V's
@@ -295,7 +296,7 @@ int yapd_attn_tree(const void* q, int64_t q_tok_stride, const void* kv_pool, int
                    void* stream);
 
 /* Floats of workspace that yapd_attn_tree needs for a call of these sizes; 0 if
- * none, -1 on a bad argument. */
+ * none, -1 on a bad argument.  For a packed call with a window below max_q: what max_q as the window needs. */
 int64_t yapd_attn_tree_workspace(int rows, int max_q, int n_q, int n_heads, int window, int sinks, int max_kv, int bits);
 
 /* Accepted nodes moved together, in every layer: position base[r] + i of row r

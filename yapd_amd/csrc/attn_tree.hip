@@ -676,14 +676,16 @@ bool overlap(const void* a, int64_t n, int64_t pitch, int64_t bytes, const void*
   return first < n && first * pitch < from + b_bytes;
 }
 
-int tree_checks(int rows, int max_q, int n_q, int n_heads, int window, int sinks, int max_kv, int bits) {
+// packed: max_q is only a bound of the rows' nodes, which does not bound the window
+int tree_checks(int rows, int max_q, int n_q, int packed, int n_heads, int window, int sinks, int max_kv, int bits) {
   YAPD_REQUIRE(bits == 8 || bits == 16, "attn_tree: bits must be 8 or 16 (got %d)", bits);
   YAPD_REQUIRE(rows >= 1 && max_q >= 1 && n_q >= 1, "attn_tree: need rows, max_q and n_q >= 1 (got %d, %d, %d)", rows,
                max_q, n_q);
   YAPD_REQUIRE(max_q <= kMaxNodes, "attn_tree: a tree has at most 64 nodes (got max_q = %d)", max_q);
   YAPD_REQUIRE(n_heads >= 4 && n_heads % 4 == 0 && n_heads <= 1024,
                "attn_tree: n_heads must be a multiple of 4, at most 1024 (got %d)", n_heads);
-  YAPD_REQUIRE(window >= max_q && sinks >= 0, "attn_tree: need window >= max_q and sinks >= 0 (got %d, %d)", window, sinks);
+  YAPD_REQUIRE(window >= (packed ? 1 : max_q) && sinks >= 0, "attn_tree: need window >= %s and sinks >= 0 (got %d, %d)",
+               packed ? "1" : "max_q", window, sinks);
   YAPD_REQUIRE(max_kv >= 1, "attn_tree: max_kv must be >= 1 (got %d)", max_kv);
   return YAPD_OK;
 }
@@ -693,7 +695,7 @@ int tree_checks(int rows, int max_q, int n_q, int n_heads, int window, int sinks
 
 extern "C" int64_t yapd_attn_tree_workspace(int rows, int max_q, int n_q, int n_heads, int window, int sinks, int max_kv,
                                             int bits) {
-  if (yapd::tree_checks(rows, max_q, n_q, n_heads, window, sinks, max_kv, bits) != YAPD_OK) return -1;
+  if (yapd::tree_checks(rows, max_q, n_q, 0, n_heads, window, sinks, max_kv, bits) != YAPD_OK) return -1;
   const yapd::Cut c = yapd::cut_of(rows, max_q, n_heads, window, sinks, max_kv, bits);
   return c.parts == 1 ? 0 : static_cast<int64_t>(c.parts) * n_q * n_heads * (yapd::kHeadDim + 2);
 }
@@ -704,7 +706,7 @@ extern "C" int yapd_attn_tree(const void* q, int64_t q_tok_stride, const void* k
                               int window, int sinks, int max_kv, float scale, float* workspace, int64_t workspace_floats,
                               void* out, void* stream) {
   YAPD_REQUIRE(q && kv_pool && page_table && kv_len && mask && out, "attn_tree: NULL pointer");
-  if (int rc = yapd::tree_checks(rows, max_q, n_q, n_heads, window, sinks, max_kv, bits)) return rc;
+  if (int rc = yapd::tree_checks(rows, max_q, n_q, q_start != nullptr, n_heads, window, sinks, max_kv, bits)) return rc;
   YAPD_REQUIRE(yapd::al16(q) && yapd::al16(kv_pool) && yapd::al16(out),
                "attn_tree: q, kv_pool and out must be 16-byte aligned");
   YAPD_REQUIRE(q_tok_stride >= static_cast<int64_t>(n_heads) * yapd::kHeadDim && q_tok_stride % 8 == 0,

@@ -730,8 +730,8 @@ def attn_tree(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len: 
 
     Lengths and masks are read on the device: a captured call follows them.  ``max_q`` (default: all, at most 64) and
     ``max_kv`` (default: all positions the table maps) are the host's upper bounds; ``window`` (default: none) is at least
-    ``max_q``.  Scores have to stay below 2^30 in magnitude.  Few nodes over many keys need a float32 ``workspace``
-    (``yapd_attn_tree_workspace``), allocated here unless given."""
+    ``n``, of packed nodes at least 1.  Scores have to stay below 2^30 in magnitude.  Few nodes over many keys need a
+    float32 ``workspace`` (``yapd_attn_tree_workspace``), allocated here unless given."""
     dev = q.device
     if elsewhere(q):
         with torch.cuda.device(dev):  # the launch goes to the current device
@@ -779,7 +779,8 @@ def attn_tree(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, kv_len: 
     lib = load_library()
     floats = 0
     if workspace is None:
-        floats = lib.yapd_attn_tree_workspace(rows, max_q, n_q, H, window, sinks, kv_max, bits)
+        floats = lib.yapd_attn_tree_workspace(rows, max_q, n_q, H, window if q_start is None else max(window, max_q), sinks,
+                                              kv_max, bits)
         if floats > 0:
             workspace = torch.empty(floats, dtype=torch.float32, device=dev)
     else:
