@@ -261,7 +261,9 @@ int yapd_kv8_copy_pages(void* const* kv_pools, int n_layers, int64_t n_pages, in
  * each or (q_start, device int32 [rows + 1], not decreasing) tokens [q_start[r],
  * q_start[r + 1]), go to positions pos0[r], pos0[r] + 1, ...; positions that the
  * table does not map to a page in [0, n_pages) are left out, and no other
- * byte of the pool is written.  Two tokens of one position: either's. */
+ * byte of the pool is written.  A position that gets two tokens of one call (rows
+ * that share its page) may hold the codes of one and the scale of the other: the positions written
+ * must belong to one row alone, or hold nothing. */
 int yapd_kv8_write(const void* k, const void* v, int64_t k_tok_stride, int64_t v_tok_stride, void* kv_pool8,
                    int64_t n_pages, const int32_t* page_table, int table_stride, int table_cols, const int32_t* pos0,
                    const int32_t* q_start, int rows, int n_tokens, int n_heads, void* stream);

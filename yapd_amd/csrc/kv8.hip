@@ -45,6 +45,8 @@ __device__ __forceinline__ void finite16(u32x4_t a, u32x4_t b, float (&f)[16]) {
   for (int i = 0; i < 16; ++i) f[i] = f[i] == f[i] ? fminf(fmaxf(f[i], -top), top) : 0.f;
 }
 
+// Codes and scale bytes are stored apart, so a slot that two rows write may end with one's codes and the other's scale: the
+// caller gives every position to one row.
 // A wave: the tokens of one row on one page, one head.  Lane (t = lane % 16, g = lane / 16) has values 16g .. 16g + 15 of
 // the page's token t.  Row r's pages are the slots from f(r) on, f(r) = q_start[r] / 16 + 2 r: n tokens touch at
 // most n / 16 + 2 pages, which end at or before f(r + 1).

@@ -640,7 +640,8 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: torch
     Row ``r``'s tokens go to positions ``pos0[r], pos0[r] + 1, ...``: ``tokens / rows`` of them each (``rows`` the entries
     of ``pos0``), or packed ``[q_start[r], q_start[r + 1])`` (int32, not decreasing).  Positions that the table does not
     map to a page of the pool are left out; every other byte of the pool stays.  NaN is written as 0, infinities as
-    the largest finite value."""
+    the largest finite value.  The positions written must belong to one row alone: two tokens of one position may leave
+    the codes of one and the scale of the other."""
     dev = k.device
     if elsewhere(k):
         with torch.cuda.device(dev):  # the launch goes to the current device
