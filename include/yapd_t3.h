@@ -245,7 +245,7 @@ int64_t yapd_attn_window_workspace(int rows, int max_q, int n_q, int packed, int
  *
  * 8-bit pool (one per layer): [n_pages][2][H][16*64 + 16] bytes.  A head's plane
  * holds its 16 tokens' codes in the bf16 pool's order (signed bytes in [-127,
- * 127]), then a scale byte e for each token: value = code * 2^(e - 127).
+ * 127]), then a scale byte e for each token, 1 to 248: value = code * 2^(e - 127).  A page of zeros holds zeros.
  * n_heads is a multiple of 4, at most 1024, in all of these.
  * ------------------------------------------------------------------------ */
 
@@ -256,7 +256,8 @@ int yapd_kv8_copy_pages(void* const* kv_pools, int n_layers, int64_t n_pages, in
 /* Quantise k, v (bf16 [n_tokens, H, 64] with token strides k_tok_stride,
  * v_tok_stride) into the pages.  For the 64 values x of a token's head: e - 127 =
  * max(floor(log2 max|x|) - 6, -126), code = x 2^(127 - e) rounded to the nearest
- * (ties to even) and held to [-127, 127]: off by at most 2^(e - 128) <= max|x| / 128.
+ * (ties to even) and held to [-127, 127]: off by at most 2^(e - 128), which is at most max|x| / 128
+ * for max|x| >= 2^-120 and 2^-127 below.
  * NaN counts as 0, an infinity as the largest finite bf16.  Row r's tokens, n_tokens / rows
  * each or (q_start, device int32 [rows + 1], not decreasing) tokens [q_start[r],
  * q_start[r + 1]), go to positions pos0[r], pos0[r] + 1, ...; positions that the

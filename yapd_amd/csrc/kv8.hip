@@ -3,7 +3,8 @@
 //
 // One scale a (token, head, plane), a power of two.  For the 64 values x of a token's head:
 //   e = max(floor(log2 max|x|) - 6, -126),  c = clamp(round to even(x 2^-e), -127, 127),  value = c 2^e.
-// The largest code is at least 64, so |x - value| <= 2^(e-1) <= max|x| / 128.  x 2^-e is exact, so a code is
+// |x - value| <= 2^(e-1), for max|x| >= 2^-120 (where e is not held to -126 and the largest code is at least 64) at most
+// max|x| / 128; smaller vectors are off by up to 2^-127 whatever their size.  x 2^-e is exact, so a code is
 // the same whoever computes it, and c 2^e is a bf16 value (7 bits), so reading back rounds nothing: attention
 // over the codes and over the pages read back see the same keys.  (A scale of max|x| / 127 would halve the
 // step for vectors just above a power of two, at the price of codes that depend on a division's rounding.)
