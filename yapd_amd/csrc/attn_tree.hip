@@ -401,8 +401,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NQT > 1 ? 2
             for (int j = 0; j < 4; ++j) sv[4 * i + j] = __builtin_ldexpf(s[j], exponent_of(ks[i], j));
           }
           weights(qt, key0, edge, sv);
-          // The weights times V's scales in bf16: the operand type of the product with V, a rounding of 2^-9 of each.  A key
-          // that a query does not see has a weight of 0 there whatever its scale byte is.
+          // The weights times V's scales in bf16, the operand type of the product with V: each is off by at most 2^-8 of
+          // itself.  A key that a query does not see has a weight of 0 there whatever its scale byte is.
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             pw[qt][i >> 2][i & 3] = pack_bf16x2(__builtin_ldexpf(sv[2 * i], exponent_of(vs[i >> 1], 2 * i & 3)),
@@ -468,7 +468,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NQT > 1 ? 2
             for (int j = 0; j < 4; ++j) sv[4 * i + j] = s[j];
           }
           weights(qt, key0, edge, sv);
-          // P in bf16: the operand type of the product with V, a rounding of 2^-9 of each weight
+          // P in bf16, the operand type of the product with V: each weight is off by at most 2^-8 of itself
           u32x4_t pw;
 #pragma unroll
           for (int i = 0; i < 4; ++i) pw[i] = pack_bf16x2(sv[2 * i], sv[2 * i + 1]);

@@ -262,7 +262,7 @@ attn_window_kernel(const WindowParams P) {
         }
         l[qt] = l[qt] * alpha + ps;
         m[qt] = mn;
-        // P in bf16: the operand type of the product with V (a rounding of 2^-9 of each weight, averaged over keys)
+        // P in bf16, the operand type of the product with V: each weight is off by at most 2^-8 of itself
         u32x4_t pw;
 #pragma unroll
         for (int w = 0; w < 4; ++w) pw[w] = pack_bf16x2(p[2 * w], p[2 * w + 1]);
