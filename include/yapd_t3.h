@@ -307,7 +307,8 @@ int64_t yapd_attn_tree_workspace(int rows, int max_q, int n_q, int n_heads, int 
  * max_kept), K, V and (bits = 8) their scales.  A row's values are all read
  * before the first is written.  base, kept, n_kept: device int32; kv_pools: a
  * host array of pool addresses.  Entries whose source or destination the table
- * does not map to a page in [0, n_pages) are left out.  The pages written must belong to
+ * does not map to a page in [0, n_pages) are left out; a table that names page 0 for
+ * what it does not map has it copied like any other.  The pages written must belong to
  * one row alone; pools that overlap are refused.  max_kept <= 64, rows <= 65535. */
 int yapd_kv_keep(void* const* kv_pools, int n_layers, int bits, int64_t n_pages, int n_heads,
                  const int32_t* page_table, int table_stride, int table_cols, const int32_t* base,

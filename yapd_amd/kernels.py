@@ -800,8 +800,8 @@ def kv_keep(pools, table: torch.Tensor, base: torch.Tensor, kept: torch.Tensor, 
 
     ``base [rows]``, ``kept [rows, m]`` (``m <= 64``) and ``n_kept [rows]`` are device int32, so a verification on the
     device needs no synchronisation.  A row's values are all read before the first is written: any nodes in any
-    order.  Positions that the table does not map to a page of the pool are left out.  The written pages
-    must belong to one row alone."""
+    order.  Positions that the table does not map to a page of the pool are left out (page 0 is one, also where a table names
+    it for positions that hold nothing).  The written pages must belong to one row alone."""
     ptrs, shape, dev = pool_pointers(pools)
     if elsewhere(pools[0]):
         with torch.cuda.device(dev):  # the launch goes to the current device

@@ -112,7 +112,9 @@ class PagedKV:
 
     def keep_nodes(self, base: torch.Tensor, kept: torch.Tensor, n_kept: torch.Tensor) -> None:
         """Move the accepted nodes of every row's drafted tree to the positions from ``base`` on, in every layer (see
-        :func:`kernels.kv_keep`; entry ``r`` of the device tensors is the cache's row ``r``), on the current stream."""
+        :func:`kernels.kv_keep`; entry ``r`` of the device tensors is the cache's row ``r``), on the current stream.  A
+        :class:`SharedPagedKV` must have all of a tree's positions reserved: an unmapped one is page 0's, whose
+        bytes would be kept as the node's."""
         kernels.kv_keep(self.pools, self.table, base, kept, n_kept)
 
     def copy_row_pages(self, src_row: int, dst_row: int, n_positions: int) -> None:
