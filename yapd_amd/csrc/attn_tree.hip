@@ -73,7 +73,7 @@ __device__ __forceinline__ bool find_tree(const TreeParams& P, int row, Tree& t)
   return t.qc > 0;
 }
 
-constexpr int kSorted = 256;  // rows that are ordered by cost, four a lane
+constexpr int kSorted = 256;  // rows that are ordered by cost, four a lane; more of them were not measured
 constexpr int kClasses = 64;
 
 // Row `slot` by cost, the costliest first: the keys that it sees times what a chunk of them costs it.  A launch of more
@@ -94,6 +94,7 @@ __device__ __forceinline__ int row_by_cost(const TreeParams& P, int slot, int la
     if (P.q_start != nullptr) n = min(max(P.q_start[r + 1], 0), P.n_q) - min(max(P.q_start[r], 0), P.n_q);
     const int kvl = min(max(P.kv_len[r], 0), P.table_cols * kPageSize);
     // of two query tiles a chunk takes 230 instructions and 110 a tile; of more than 32 nodes half the waves go over it
+    // (at 8 bits; a bf16 chunk converts nothing and takes fewer, and is ordered by the same numbers)
     const float each = NQT == 1 ? 1.f : n > 32 ? 900.f : n > 16 ? 450.f : 340.f;
     const float keys = fminf(static_cast<float>(kvl), static_cast<float>(P.window) + static_cast<float>(P.sinks) + n);
     cls[j] = n > 0 ? static_cast<int>(fminf(keys * each * P.class_scale, kClasses - 1.f)) : 0;

@@ -601,7 +601,8 @@ __device__ __forceinline__ bool sample_values(const SampleParams& P, Shared<NT, 
 
 // Row `slot` by cost, the costliest first, where a CU holds one row, rows are more than CUs and settings differ: those
 // with a temperature (three or four passes), then those of a small top-k, whose few elements are soon in a list, then those
-// that want the largest logit alone.  What starts last should end soon.  A thread a row, at most NT of them.
+// that want the largest logit alone.  What starts last should end soon.  A thread a row, at most NT of them.  Rows of
+// bf16 or of fewer threads come as they are; ordering those was not measured.
 template <int NT, bool kWide>
 __device__ __forceinline__ uint32_t row_by_cost(const SampleParams& P, Shared<NT, kWide>& S, uint32_t slot) {
   const uint32_t i = threadIdx.x;
