@@ -274,7 +274,7 @@ int yapd_kv8_write(const void* k, const void* v, int64_t k_tok_stride, int64_t v
  * the values of page page_table8[r][c] of kv_pool8, all 16 slots as they
  * stand.  Exact: code * 2^(e - 127) is a bf16 value.  Columns that either table does not map
  * to a page of its pool are left out.  Rows that share a page on both
- * sides write the same bytes.  kv_len: device int32 [rows]. */
+ * sides write the same bytes; a page of kv_pool that two pages of kv_pool8 go to may hold some of each.  kv_len: device int32 [rows]. */
 int yapd_kv8_unpack(const void* kv_pool8, int64_t n_pages8, const int32_t* page_table8, int table8_stride,
                     int table8_cols, const int32_t* kv_len, int rows, int max_kv, int n_heads, void* kv_pool,
                     int64_t n_pages, const int32_t* page_table, int table_stride, int table_cols, void* stream);

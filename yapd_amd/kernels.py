@@ -677,7 +677,8 @@ def kv8_unpack(pool8: torch.Tensor, table8: torch.Tensor, kv_len: torch.Tensor, 
     times its scale is a bf16 value.  A page's slots past ``kv_len`` are converted as they stand.
 
     ``kv_len`` is read on the device; ``max_kv`` is the host's upper bound (default: all that both tables map),
-    past which nothing is converted.  Columns that either table does not map to a page of its pool are left out."""
+    past which nothing is converted.  Columns that either table does not map to a page of its pool are left out.  A page
+    of ``pool`` that two pages of ``pool8`` go to may hold some of each."""
     dev = pool8.device
     if elsewhere(pool8):
         with torch.cuda.device(dev):  # the launch goes to the current device
